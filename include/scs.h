@@ -322,6 +322,57 @@ int scs_eval_batch(scs_handle h, const float* ax_dev, const float* co_dev, const
                    const float* atlas_dev, const uint8_t* y_dev, int64_t n,
                    double* loss_sum_host, int64_t* n_correct_host, void* stream);
 
+/* ---- operators beside the net: site adapters and the optimiser that trains them ------------------------------------------------- */
+
+/* Element types beside SCS_F32 that these operators take. */
+#define SCS_BF16 6
+#define SCS_F16 7
+
+/* AdamW over many tensors at once (decoupled weight decay; the lasagne Adam of nets.py:236-237 is scs_adam_apply):
+ *   c = grad_scale * min(1, max_norm / (norm + 1e-6)), norm = |grad_scale| * sqrt(sum g^2) over ALL tensors (max_norm 0: c = grad_scale)
+ *   m' = b1 m + (1 - b1) c g;  v' = b2 v + (1 - b2) (c g)^2;
+ *   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps),  t = the steps taken, this one included
+ * computed in f32, every operation rounded once; a 16-bit parameter is read as f32 and rounded to the nearest at the end, or, where
+ * `master` is given, is the rounded copy of that f32 value.
+ *
+ * Tensor i of n elements owns ceil(n / 256) BLOCKS of 256 elements of the moment arenas, behind the blocks of the tensors before it (the
+ * elements between its end and its last block's end are zeros and stay so).  state_bits 32: m, v are float [blocks * 256].  state_bits 8:
+ * m is int8, v is uint8 [blocks * 256], m_scale / v_scale float [blocks], and an element stands for
+ *   m = q |q| m_scale,   v = (q^2 v_scale)^2,      m_scale = max|m| / 127^2, v_scale = max sqrt(v) / 255^2 over its block. */
+typedef struct scs_adamw_ctx* scs_adamw;
+typedef struct {
+    void* param;            /* device, n elements of `type`, contiguous, aligned to its elements */
+    float* master;          /* device, f32 [n], or NULL (16-bit parameters only) */
+    int64_t n;              /* 0 is allowed: the tensor is passed over */
+    double weight_decay;
+    int32_t type;           /* SCS_F32, SCS_BF16, SCS_F16 */
+    int32_t reserved;
+} scs_adamw_tensor;
+
+/* The table is host memory and is copied; the device memory that it and the arenas name is the caller's and must stay until
+ * scs_adamw_destroy.  Two tensors that share memory are refused.  `step`: steps already taken (0 for a new optimiser; the caller zeroes
+ * the arenas).  The optimiser lives on h's device and does not need h afterwards. */
+int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, int state_bits, void* m_dev, void* v_dev,
+                     float* m_scale_dev, float* v_scale_dev, int64_t step, scs_adamw* out);
+/* (frees device memory: waits for the device; not while a stream is being captured) */
+int scs_adamw_destroy(scs_adamw o);
+
+/* One step.  grads, grad_types: host arrays of one device pointer (n elements, contiguous) and one type per tensor; they are read before
+ * the call returns.  Gradients are not changed.  max_norm > 0 clips by the norm over all tensors and leaves it (before clipping) in
+ * *norm_dev (device float, may be NULL); where that norm is not finite NOTHING changes - neither parameters, moments nor the step count.
+ * Without max_norm a gradient that is not finite makes its element's m, v and p NaN (8 bits: its block's m and v).
+ * The step count lives on the device, so that a captured call counts at every replay; lr and the other numbers are the captured call's.
+ * Steps of one optimiser must be ordered (one stream, or events): they update the same memory.  The result is the same bits every time. */
+int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_types, double lr, double beta1, double beta2, double eps,
+                   double grad_scale, double max_norm, float* norm_dev, void* stream);
+
+/* The values that 8-bit moments stand for: f32 [blocks * 256] each, in the arenas' layout (checkpoints, inspection). */
+int scs_adamw_states(scs_adamw o, float* m_out_dev, float* v_out_dev, void* stream);
+
+/* Steps taken.  get waits for the stream; set enqueues. */
+int scs_adamw_get_step(scs_adamw o, int64_t* step_host, void* stream);
+int scs_adamw_set_step(scs_adamw o, int64_t step, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

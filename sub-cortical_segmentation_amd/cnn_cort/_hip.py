@@ -61,6 +61,12 @@ SIGNATURES = {
     'scs_set_fused_adam': (_c.c_int, [_vp, _c.c_int, _c.c_float, _c.c_float, _c.c_float, _c.c_float]),
     'scs_eval_batch': (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int64, _c.POINTER(_c.c_double),
                                   _c.POINTER(_c.c_int64), _vp]),
+    'scs_adamw_create': (_c.c_int, [_vp, _vp, _c.c_int32, _c.c_int, _vp, _vp, _vp, _vp, _c.c_int64, _c.POINTER(_vp)]),
+    'scs_adamw_destroy': (_c.c_int, [_vp]),
+    'scs_adamw_step': (_c.c_int, [_vp, _vp, _vp, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _c.c_double, _vp, _vp]),
+    'scs_adamw_states': (_c.c_int, [_vp, _vp, _vp, _vp]),
+    'scs_adamw_get_step': (_c.c_int, [_vp, _c.POINTER(_c.c_int64), _vp]),
+    'scs_adamw_set_step': (_c.c_int, [_vp, _c.c_int64, _vp]),
 }
 
 

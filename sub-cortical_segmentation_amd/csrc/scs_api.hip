@@ -35,6 +35,8 @@ void set_error(const char* fmt, ...) {
     va_end(ap);
 }
 
+int handle_device(scs_handle h) { return h->device; }
+
 // ----------------------------------------------------------------------------- layer configurations
 // <CIN, COUT, HIN, patches per workgroup, epilogue, source, LDS plane stride, bands, workgroups per CU>
 using CfgConv12 = ConvCfg<20, 20, 30, 1, EPI_BIAS_RELU_POOL, SRC_CONV1, 496, 2, 2>;    // half a patch per workgroup
