@@ -328,6 +328,46 @@ int scs_eval_batch(scs_handle h, const float* ax_dev, const float* co_dev, const
 #define SCS_BF16 6
 #define SCS_F16 7
 
+/* A shared projection with a low-rank adapter per request.  The rows of one call belong to requests: request q owns rows
+ * [offsets[q], offsets[q + 1]) and uses adapter s = adapters[q] (-1, or any number outside the table: none).  For row i of request q
+ *   forward   y_i = x_i W + bias + scale_s (x_i A_s^T) B_s
+ *   backward  dx_i = dy_i W^T + u_i A_s,  u_i = scale_s dy_i B_s^T;   dA_s = sum_i u_i^T x_i;   dB_s = scale_s sum_i (x_i A_s^T)^T dy_i
+ * over the rows of all requests that use s (an adapter that none uses gets zeros).  W and bias are shared and fixed: no gradients of them.
+ * Products are summed in f32 whatever the type, x_i A_s^T is kept in f32, and each output is rounded once; for 16-bit types the adapters'
+ * products scale_s x_i A_s^T (u_i) enter the matrix cores as two 16-bit pieces.
+ * Beside the net's dense layers (nets.py:179, 217, 227): W in (in, out) order, as the parameter arena holds it. */
+typedef struct {
+    int32_t dtype;                 /* SCS_F32, SCS_BF16 or SCS_F16: x, W, bias, A, B, y, dy, dx */
+    int32_t rank;                  /* 1..128; adapters of lower rank are filled up with zeros */
+    int32_t n_adapters;            /* 1..65535 */
+    int32_t n_requests;            /* 0..2^24 */
+    int64_t rows;                  /* rows of x, y, dy, dx: 0..2^30 */
+    int64_t in_features, out_features;      /* 1..2^20 each */
+    int64_t ldw;                   /* row stride of W in elements, >= out_features */
+    const void* w;                 /* [in][out] */
+    const void* bias;              /* [out] or NULL */
+    const void* a;                 /* [n_adapters][rank][in], contiguous */
+    const void* b;                 /* [n_adapters][rank][out], contiguous */
+    const float* scale;            /* [n_adapters] or NULL (1) */
+    const int32_t* offsets;        /* [n_requests + 1], ascending.  Rows outside [offsets[0], offsets[n_requests]) are left as they were.  The offsets are
+                                    * read on the device and clamped to the rows there: others than ascending ones give wrong rows, not wrong addresses */
+    const int32_t* adapters;       /* [n_requests] */
+} scs_lowrank;
+
+/* Bytes of workspace that a call needs (device memory, aligned to 16 bytes; it may be shared by calls that run one after the other). */
+int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward, size_t* bytes);
+
+/* x [rows][in] with row stride ldx >= in (elements), y [rows][out] with ldy >= out; y must not overlap the inputs.
+ * hidden: f32 [rows][rank] or NULL; receives x_i A_s^T (0 where a row has no adapter) for the backward call. */
+int scs_lowrank_forward(scs_handle h, const scs_lowrank* p, const void* x_dev, int64_t ldx, void* y_dev, int64_t ldy, float* hidden_dev,
+                        void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* hidden: what the forward call left, or NULL (formed again from x).  Each of dx [rows][in], da [n_adapters][rank][in] and
+ * db [n_adapters][rank][out] (both f32, written whole) may be NULL and is then not formed.  Sums are formed in a fixed order: the same call gives the same bits. */
+int scs_lowrank_backward(scs_handle h, const scs_lowrank* p, const void* x_dev, int64_t ldx, const void* dy_dev, int64_t lddy,
+                         const float* hidden_dev, void* dx_dev, int64_t lddx, float* da_dev, float* db_dev,
+                         void* workspace_dev, size_t workspace_bytes, void* stream);
+
 /* AdamW over many tensors at once (decoupled weight decay; the lasagne Adam of nets.py:236-237 is scs_adam_apply):
  *   c = grad_scale * min(1, max_norm / (norm + 1e-6)), norm = |grad_scale| * sqrt(sum g^2) over ALL tensors (max_norm 0: c = grad_scale)
  *   m' = b1 m + (1 - b1) c g;  v' = b2 v + (1 - b2) (c g)^2;

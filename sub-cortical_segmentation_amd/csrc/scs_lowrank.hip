@@ -1,0 +1,572 @@
+// A shared projection with a low-rank adapter per request, forward and backward (scs_lowrank_*, include/scs.h).
+//
+//   y_i  = x_i W + bias + scale_s (x_i A_s^T) B_s                      s = the adapter of row i's request
+//   dx_i = dy_i W^T + scale_s (dy_i B_s^T) A_s
+//   dA_s = scale_s sum_i (dy_i B_s^T)^T x_i          dB_s = scale_s sum_i (x_i A_s^T)^T dy_i
+//
+// A and B are both [rank][features], so that one set of kernels serves both directions:
+//   shrink  H = X P_s^T     (X = x, P = A, or X = dy, P = B): rows to rank, f32 result
+//   project Y = X W' + scale_s H P_s   (W' = W, P = B, or W' = W^T, P = A)
+//   wgrad   G_s = scale_s sum H^T X    (H of dy with X = x: dA; H of x with X = dy: dB)
+// A row's request is found from the offsets inside the kernels.  A 16-row tile that several requests share is multiplied with each one's
+// adapter, and every product is added under the mask of its own rows: an adapter that holds infinities touches its own requests only.
+#include <algorithm>
+#include <vector>
+
+#include "scs_ops.h"
+
+namespace scs {
+namespace {
+
+struct Requests {
+    const int32_t* offsets;
+    const int32_t* adapters;
+    const float* scale;
+    int32_t n, n_adapters, rank;
+    int32_t rows;
+};
+
+__device__ __forceinline__ int clamp_row(int o, int rows) { return o < 0 ? 0 : o > rows ? rows : o; }
+
+// smallest q with offsets[q + 1] > row (n if there is none): binary search down to one wave's width, then one load a lane
+__device__ __forceinline__ int first_request(const Requests& r, int row) {
+    int lo = 0, hi = r.n;
+    while (hi - lo > 64) {
+        const int mid = (lo + hi) >> 1;
+        if (r.offsets[mid + 1] <= row) lo = mid + 1; else hi = mid;
+    }
+    const int q = lo + (int)(threadIdx.x & 63);
+    const unsigned long long below = __ballot(q < hi && r.offsets[q + 1] <= row);
+    const int add = ~below == 0ull ? 64 : __builtin_ctzll(~below);
+    return min(lo + add, hi);
+}
+
+struct Span { int lo, hi, s; float scale; };           // rows of request q inside [m0, m1) and its adapter (-1: none)
+__device__ __forceinline__ Span span_of(const Requests& r, int q, int m0, int m1) {
+    Span p;
+    p.lo = max(m0, clamp_row(r.offsets[q], r.rows));
+    p.hi = min(m1, clamp_row(r.offsets[q + 1], r.rows));
+    const int s = r.adapters[q];
+    p.s = (unsigned)s < (unsigned)r.n_adapters ? s : -1;
+    p.scale = p.s >= 0 && r.scale ? r.scale[p.s] : 1.f;
+    return p;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ shrink
+// H[row][j] = sum_k X[row][k] P_s[j][k] (0 without an adapter).  Many rows: a workgroup owns 16 rows, its four waves a quarter of the
+// contraction each, joined through LDS; operands go from global memory to the f32 matrix cores without a stop (both are contiguous along the
+// contraction: a lane's 16 or 8 bytes are its operand of four MFMAs, whose contraction indices are permuted alike on both sides).
+template <class T, int JT>
+__global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r) {
+    __shared__ float s_part[4][JT * 4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, kq = lane >> 4;
+    const int m0 = blockIdx.x * 16, m1 = min(m0 + 16, r.rows);
+    const int slab = (K + 15) / 16, per = (slab + 3) / 4;
+    const int k_lo = wave * per * 16, k_hi = min(K, (wave + 1) * per * 16);
+    const int row = min(m0 + lr, r.rows - 1);
+    const T* xr = x + (int64_t)row * ldx;
+    for (int q = first_request(r, m0); q < r.n; ++q) {
+        const Span sp = span_of(r, q, m0, m1);
+        if (r.offsets[q] >= m1) break;
+        if (sp.lo >= sp.hi) continue;
+        f32x4 acc[JT];
+#pragma unroll
+        for (int t = 0; t < JT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (sp.s >= 0) {
+            const T* ps = p + (int64_t)sp.s * r.rank * K;
+            for (int k0 = k_lo; k0 < k_hi; k0 += 16) {
+                const int k = k0 + 4 * kq, left = K - k;
+                typename Vec4<T>::raw ra, rb[JT];
+                raw_load<T>(ra, xr + k, left);
+#pragma unroll
+                for (int t = 0; t < JT; ++t) {
+                    const int j = min(t * 16 + lr, r.rank - 1);
+                    raw_load<T>(rb[t], ps + (int64_t)j * K + k, left);
+                }
+                float a[4];
+                unpack<T>(ra, a);
+#pragma unroll
+                for (int t = 0; t < JT; ++t) {
+                    float b[4];
+                    unpack<T>(rb[t], b);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc[t], 0, 0, 0);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < JT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s_part[wave][t * 4 + i][lane] = acc[t][i];
+        __syncthreads();
+        for (int e = wave; e < JT * 4; e += 4) {
+            const float v = (s_part[0][e][lane] + s_part[1][e][lane]) + (s_part[2][e][lane] + s_part[3][e][lane]);
+            const int m = m0 + 4 * kq + (e & 3), j = (e >> 2) * 16 + lr;
+            if (m >= sp.lo && m < sp.hi && j < r.rank) h[(int64_t)m * r.rank + j] = v;
+        }
+    }
+}
+
+// Few rows: a wave per (row, direction) reads both vectors along the contraction and adds up over its lanes.
+template <class T>
+__global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int row = blockIdx.x, j = blockIdx.y * 4 + wave;
+    const int q = first_request(r, row);
+    if (q >= r.n || j >= r.rank) return;
+    const Span sp = span_of(r, q, row, row + 1);
+    if (sp.lo >= sp.hi) return;
+    float sum = 0.f;
+    if (sp.s >= 0) {
+        const T* xr = x + (int64_t)row * ldx;
+        const T* pr = p + ((int64_t)sp.s * r.rank + j) * K;
+#pragma unroll 4
+        for (int k = lane * 4; k < K; k += 256) {
+            typename Vec4<T>::raw ra, rb;
+            raw_load<T>(ra, xr + k, K - k);
+            raw_load<T>(rb, pr + k, K - k);
+            float a[4], b[4];
+            unpack<T>(ra, a);
+            unpack<T>(rb, b);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum = fmaf(a[i], b[i], sum);
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    }
+    if (lane == 0) h[(int64_t)row * r.rank + j] = sum;
+}
+
+// ------------------------------------------------------------------------------------------------------------------ project, f32 matrix cores
+// Any type, any size, any stride: 128 rows x 16 NT columns a workgroup of four waves (32 rows each), the contraction in slabs of 32 staged
+// through LDS as f32 (registers hold the next slab while this one is multiplied).
+template <class T>
+struct ProjectArgs {
+    const T* x; int64_t ldx;
+    const T* w; int64_t ldw;          // W' as stored: [K][N], or [N][K] where TRANS
+    const T* bias;
+    const T* low;                     // P: [n_adapters][rank][N]
+    const float* h;                   // [rows][rank]
+    T* y; int64_t ldy;
+    int32_t K, N;
+    Requests r;
+};
+
+constexpr int kPBM = 128, kPBK = 32, kPAS = 36;
+
+template <class T, int NT, bool TRANS>
+__global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
+    constexpr int BN = 16 * NT, BS = BN + 4;                 // (4 BS % 64 == 16: the four k-rows of a fragment lie on disjoint banks)
+    constexpr int B_FLOATS = TRANS ? (BN * kPAS > kPBK * BS ? BN * kPAS : kPBK * BS) : kPBK * BS;
+    __shared__ __attribute__((aligned(16))) float s_a[2][kPBM * kPAS];
+    __shared__ __attribute__((aligned(16))) float s_b[2][B_FLOATS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lr = lane & 15, kq = lane >> 4;
+    const int m0 = blockIdx.x * kPBM, n0 = blockIdx.y * BN;
+    const Requests& r = g.r;
+
+    constexpr int A_PER = kPBM * kPBK / 1024, B_PER = (BN * kPBK / 4 + 255) / 256;
+    typename Vec4<T>::raw ra[A_PER], rb[B_PER];
+    auto load_slab = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < A_PER; ++i) {                    // 8 vectors a row, 32 rows at a time
+            const int row = m0 + (tid >> 3) + 32 * i, k = k0 + (tid & 7) * 4;
+            raw_load<T>(ra[i], g.x + (int64_t)row * g.ldx + k, row < r.rows ? g.K - k : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < B_PER; ++i) {
+            const int e = tid + 256 * i;
+            if constexpr (TRANS) {
+                const int n = n0 + (e >> 3), k = k0 + (e & 7) * 4;
+                raw_load<T>(rb[i], g.w + (int64_t)n * g.ldw + k, (e >> 3) < BN && n < g.N ? g.K - k : 0);
+            } else {
+                const int kr = e / (BN / 4), n = n0 + (e - kr * (BN / 4)) * 4, k = k0 + kr;
+                raw_load<T>(rb[i], g.w + (int64_t)k * g.ldw + n, kr < kPBK && k < g.K ? g.N - n : 0);
+            }
+        }
+    };
+    auto store_slab = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < A_PER; ++i) {
+            float f[4];
+            unpack<T>(ra[i], f);
+            *(f32x4*)&s_a[buf][((tid >> 3) + 32 * i) * kPAS + (tid & 7) * 4] = f32x4{f[0], f[1], f[2], f[3]};
+        }
+#pragma unroll
+        for (int i = 0; i < B_PER; ++i) {
+            const int e = tid + 256 * i;
+            float f[4];
+            unpack<T>(rb[i], f);
+            if constexpr (TRANS) {
+                if ((e >> 3) < BN) *(f32x4*)&s_b[buf][(e >> 3) * kPAS + (e & 7) * 4] = f32x4{f[0], f[1], f[2], f[3]};
+            } else {
+                const int kr = e / (BN / 4), c = (e - kr * (BN / 4)) * 4;
+                if (kr < kPBK) *(f32x4*)&s_b[buf][kr * BS + c] = f32x4{f[0], f[1], f[2], f[3]};
+            }
+        }
+    };
+
+    f32x4 acc[2][NT];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int slabs = (g.K + kPBK - 1) / kPBK;
+    load_slab(0);
+    store_slab(0);
+    __syncthreads();
+    for (int s = 0; s < slabs; ++s) {
+        if (s + 1 < slabs) load_slab((s + 1) * kPBK);
+        const float* sa = s_a[s & 1] + (wave * 32 + lr) * kPAS + 4 * kq;
+        const float* sb = s_b[s & 1];
+#pragma unroll
+        for (int ks = 0; ks < kPBK; ks += 16) {
+            const f32x4 a0 = *(const f32x4*)(sa + ks), a1 = *(const f32x4*)(sa + 16 * kPAS + ks);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                f32x4 b;
+                if constexpr (TRANS) b = *(const f32x4*)(sb + (t * 16 + lr) * kPAS + ks + 4 * kq);
+                else
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) b[j] = sb[(ks + 4 * kq + j) * BS + t * 16 + lr];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[j], b[j], acc[0][t], 0, 0, 0);
+                    acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[j], b[j], acc[1][t], 0, 0, 0);
+                }
+            }
+        }
+        if (s + 1 < slabs) store_slab((s + 1) & 1);
+        __syncthreads();
+    }
+
+    // the adapters' products, request by request, each under the mask of its rows
+    const int m1 = min(m0 + kPBM, r.rows);
+    for (int q = first_request(r, m0); q < r.n; ++q) {
+        const Span sp = span_of(r, q, m0, m1);
+        if (r.offsets[q] >= m1) break;
+        if (sp.lo >= sp.hi || sp.s < 0) continue;
+        const T* ps = g.low + (int64_t)sp.s * r.rank * g.N;
+        for (int j0 = 0; j0 < r.rank; j0 += kPBK) {
+            for (int e = tid; e < kPBM * kPBK; e += 256) {
+                const int m = e / kPBK, j = e % kPBK, row = m0 + m;
+                const bool in = row >= sp.lo && row < sp.hi && j0 + j < r.rank;
+                s_a[0][m * kPAS + j] = in ? sp.scale * g.h[(int64_t)row * r.rank + j0 + j] : 0.f;
+            }
+            for (int e = tid; e < kPBK * BN; e += 256) {
+                const int j = e / BN, c = e % BN;
+                s_b[0][j * BS + c] = j0 + j < r.rank && n0 + c < g.N ? to_f32(ps[(int64_t)(j0 + j) * g.N + n0 + c]) : 0.f;
+            }
+            __syncthreads();
+            const float* sa = s_a[0] + (wave * 32 + lr) * kPAS + 4 * kq;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+                    for (int ks = 0; ks < kPBK && j0 + ks < r.rank; ks += 16) {
+                        const f32x4 a = *(const f32x4*)(sa + i * 16 * kPAS + ks);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            part = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], s_b[0][(ks + 4 * kq + j) * BS + t * 16 + lr], part, 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = m0 + wave * 32 + i * 16 + 4 * kq + e;
+                        if (row >= sp.lo && row < sp.hi) acc[i][t][e] += part[e];
+                    }
+                }
+            __syncthreads();
+        }
+    }
+
+    const int live_lo = r.n ? clamp_row(r.offsets[0], r.rows) : 0, live_hi = r.n ? clamp_row(r.offsets[r.n], r.rows) : 0;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int col = n0 + t * 16 + lr;
+        if (col >= g.N) continue;
+        const float bv = g.bias ? to_f32(g.bias[col]) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int row = m0 + wave * 32 + i * 16 + 4 * kq + e;
+                if (row >= live_lo && row < live_hi) g.y[(int64_t)row * g.ldy + col] = from_f32<T>(acc[i][t][e] + bv);
+            }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ wgrad
+// G_s[j][k] = scale_s sum over the rows of s of H[row][j] X[row][k], f32.  A workgroup owns 64 columns of one adapter and one slice of the
+// rows; a lane's vector of X is its operand of four MFMAs (columns 4 c + t of MFMA t), the four waves take every fourth group of four rows
+// and are joined through LDS in a fixed order.  Slices: [slice][adapter][rank][F] partial sums, added up by wgrad_join_kernel.
+template <class T, int JT>
+__global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ h, const T* __restrict__ x, int64_t ldx, int F, int slices,
+                                                    float* __restrict__ out, Requests r) {
+    __shared__ float s_part[3][JT * 16][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lr = lane & 15, kq = lane >> 4;
+    const int c0 = blockIdx.x * 64, s = blockIdx.y, slice = blockIdx.z;
+    const int per = (int)(((int64_t)r.rows + slices - 1) / slices);
+    const int m0 = min((int64_t)slice * per, (int64_t)r.rows), m1 = min((int64_t)m0 + per, (int64_t)r.rows);
+    f32x4 acc[JT][4];
+#pragma unroll
+    for (int t = 0; t < JT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int col = c0 + 4 * lr, left = F - col;
+
+    for (int q0 = first_request(r, m0); q0 < r.n; q0 += 64) {
+        // the requests of this adapter among 64
+        const int q = q0 + lane;
+        bool mine = false;
+        if (q < r.n) mine = r.adapters[q] == s && r.offsets[q] < m1 && r.offsets[q + 1] > m0;
+        unsigned long long todo = __ballot(mine);
+        while (todo) {
+            const Span sp = span_of(r, q0 + __builtin_ctzll(todo), m0, m1);
+            todo &= todo - 1;
+            for (int b = sp.lo + wave * 4; b < sp.hi; b += 16) {
+                const int row = b + kq;
+                const bool in = row < sp.hi;
+                typename Vec4<T>::raw rx;
+                raw_load<T>(rx, x + (int64_t)row * ldx + col, in ? left : 0);
+                float f[4];
+                unpack<T>(rx, f);
+#pragma unroll
+                for (int t = 0; t < JT; ++t) {
+                    const int j = t * 16 + lr;
+                    const float a = in && j < r.rank ? h[(int64_t)row * r.rank + j] : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, f[i], acc[t][i], 0, 0, 0);
+                }
+            }
+        }
+    }
+    if (wave) {
+#pragma unroll
+        for (int t = 0; t < JT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s_part[wave - 1][t * 16 + i * 4 + e][lane] = acc[t][i][e];
+    }
+    __syncthreads();
+    if (wave) return;
+    const float sc = r.scale ? r.scale[s] : 1.f;
+    float* o = out + ((int64_t)slice * r.n_adapters + s) * r.rank * F;
+#pragma unroll
+    for (int t = 0; t < JT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = t * 16 + 4 * kq + e;
+            f32x4 v;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int at = t * 16 + i * 4 + e;
+                v[i] = sc * (((acc[t][i][e] + s_part[0][at][lane]) + s_part[1][at][lane]) + s_part[2][at][lane]);
+            }
+            if (j < r.rank) raw_store<float>(v, o + (int64_t)j * F + col, left);
+        }
+}
+
+__global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ part, int slices, int64_t n, float* __restrict__ out) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        float v = part[i];
+        for (int s = 1; s < slices; ++s) v += part[s * n + i];
+        out[i] = v;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------ host side
+constexpr int kDotRows = 512;               // up to so many rows the shrink is a wave per row and direction
+
+size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
+
+int wgrad_slices(const scs_lowrank& p, int64_t F) {
+    // workgroups: 64 columns x adapters x slices; more slices until there are enough for the card, none under 256 rows
+    const int64_t tiles = (F + 63) / 64 * p.n_adapters;
+    const int64_t s = std::min<int64_t>(1024 / std::max<int64_t>(tiles, 1), p.rows / 256);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+}
+
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, bytes = 0; };
+Layout layout_of(const scs_lowrank& p, bool backward) {
+    Layout l;
+    size_t at = 0;
+    auto take = [&](size_t b) { const size_t o = at; at += up(b); return o; };
+    l.hid = take((size_t)p.rows * p.rank * 4);
+    if (backward) {
+        l.hid2 = take((size_t)p.rows * p.rank * 4);
+        size_t part = 0;
+        for (const int64_t F : {p.in_features, p.out_features}) {
+            const int s = wgrad_slices(p, F);
+            if (s > 1) part = std::max(part, (size_t)s * p.n_adapters * p.rank * F * 4);
+        }
+        l.part = take(part);
+    }
+    l.bytes = at;
+    return l;
+}
+
+int check(const scs_lowrank* p) {
+    SCS_ARG(p != nullptr, "the call's description is NULL");
+    SCS_ARG(p->dtype == SCS_F32 || p->dtype == SCS_BF16 || p->dtype == SCS_F16, "dtype is SCS_F32, SCS_BF16 or SCS_F16");
+    SCS_ARG(p->rank >= 1 && p->rank <= 128, "rank lies in 1..128");
+    SCS_ARG(p->n_adapters >= 1 && p->n_adapters <= 65535, "n_adapters lies in 1..65535");
+    SCS_ARG(p->n_requests >= 0 && p->n_requests <= (1 << 24), "n_requests lies in 0..2^24");
+    SCS_ARG(p->rows >= 0 && p->rows <= (1 << 30), "rows lies in 0..2^30");
+    SCS_ARG(p->in_features >= 1 && p->in_features <= (1 << 20) && p->out_features >= 1 && p->out_features <= (1 << 20), "features lie in 1..2^20");
+    SCS_ARG(p->ldw >= p->out_features, "ldw is below out_features");
+    SCS_ARG(p->w && p->a && p->b && p->offsets && (p->adapters || p->n_requests == 0), "a table is NULL");
+    const size_t e = p->dtype == SCS_F32 ? 4 : 2;
+    SCS_ARG((uintptr_t)p->w % e == 0 && (uintptr_t)p->bias % e == 0 && (uintptr_t)p->a % e == 0 && (uintptr_t)p->b % e == 0, "a matrix is not aligned to its elements");
+    SCS_ARG((uintptr_t)p->scale % 4 == 0 && (uintptr_t)p->offsets % 4 == 0 && (uintptr_t)p->adapters % 4 == 0, "a table is not aligned to its elements");
+    return SCS_OK;
+}
+
+Requests requests_of(const scs_lowrank& p) { return Requests{p.offsets, p.adapters, p.scale, p.n_requests, p.n_adapters, p.rank, (int32_t)p.rows}; }
+
+template <class F> void by_tiles(int rank, F&& f) {
+    const int t = (rank + 15) / 16;
+    if (t <= 1) f(std::integral_constant<int, 1>{});
+    else if (t <= 2) f(std::integral_constant<int, 2>{});
+    else if (t <= 4) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 8>{});
+}
+
+template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st) {
+    const Requests r = requests_of(p);
+    if (p.rows <= kDotRows) {
+        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r);
+        return;
+    }
+    by_tiles(p.rank, [&](auto jt) {
+        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r);
+    });
+}
+
+template <class T, bool TRANS> void project(const ProjectArgs<T>& g, hipStream_t st) {
+    // the column tile with the least padding, the widest among equals
+    int best = 8, waste = 1 << 30;
+    for (const int nt : {8, 6, 4}) {
+        const int w = (g.N + 16 * nt - 1) / (16 * nt) * 16 * nt;
+        if (w < waste) { waste = w; best = nt; }
+    }
+    const dim3 grid((unsigned)((g.r.rows + kPBM - 1) / kPBM), (unsigned)((g.N + 16 * best - 1) / (16 * best)));
+    if (best == 8) hipLaunchKernelGGL((project_f32_kernel<T, 8, TRANS>), grid, dim3(256), 0, st, g);
+    else if (best == 6) hipLaunchKernelGGL((project_f32_kernel<T, 6, TRANS>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((project_f32_kernel<T, 4, TRANS>), grid, dim3(256), 0, st, g);
+}
+
+template <class T> void wgrad(const scs_lowrank& p, const float* h, const T* x, int64_t ldx, int F, float* out, float* part, hipStream_t st) {
+    const Requests r = requests_of(p);
+    const int s = wgrad_slices(p, F);
+    by_tiles(p.rank, [&](auto jt) {
+        hipLaunchKernelGGL((wgrad_kernel<T, jt.value>), dim3((F + 63) / 64, p.n_adapters, s), dim3(256), 0, st, h, x, ldx, F, s, s > 1 ? part : out, r);
+    });
+    if (s > 1) {
+        const int64_t n = (int64_t)p.n_adapters * p.rank * F;
+        hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, st, part, s, n, out);
+    }
+}
+
+template <class T>
+int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t ldy, float* hidden, unsigned char* ws, hipStream_t st) {
+    const Layout l = layout_of(p, false);
+    float* h = hidden ? hidden : (float*)(ws + l.hid);
+    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st);
+    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)}, st);
+    SCS_HIP(hipGetLastError());
+    return SCS_OK;
+}
+
+template <class T>
+int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* hidden, void* dx, int64_t lddx, float* da, float* db,
+             unsigned char* ws, hipStream_t st) {
+    const Layout l = layout_of(p, true);
+    float* u = (float*)(ws + l.hid);
+    float* part = (float*)(ws + l.part);
+    const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
+    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st);
+    if (dx)
+        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)}, st);
+    if (da) wgrad<T>(p, u, (const T*)x, ldx, (int)p.in_features, da, part, st);
+    if (db) {
+        const float* h = hidden;
+        if (!h) {
+            h = (float*)(ws + l.hid2);
+            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), st);
+        }
+        wgrad<T>(p, h, (const T*)dy, lddy, (int)p.out_features, db, part, st);
+    }
+    SCS_HIP(hipGetLastError());
+    return SCS_OK;
+}
+
+}  // namespace
+}  // namespace scs
+
+using namespace scs;
+
+extern "C" {
+
+int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward_call, size_t* bytes) {
+    SCS_ARG(h && bytes, "null handle or output");
+    const int rc = check(p);
+    if (rc != SCS_OK) return rc;
+    *bytes = layout_of(*p, backward_call != 0).bytes;
+    return SCS_OK;
+}
+
+int scs_lowrank_forward(scs_handle h, const scs_lowrank* p, const void* x_dev, int64_t ldx, void* y_dev, int64_t ldy, float* hidden_dev,
+                        void* workspace_dev, size_t workspace_bytes, void* stream) {
+    SCS_ARG(h != nullptr, "null handle");
+    int rc = check(p);
+    if (rc != SCS_OK) return rc;
+    if (p->rows == 0 || p->n_requests == 0) return SCS_OK;
+    const size_t e = p->dtype == SCS_F32 ? 4 : 2;
+    SCS_ARG(x_dev && y_dev, "x or y is NULL");
+    SCS_ARG(ldx >= p->in_features && ldy >= p->out_features, "a row stride is below the row's length");
+    SCS_ARG((uintptr_t)x_dev % e == 0 && (uintptr_t)y_dev % e == 0 && (uintptr_t)hidden_dev % 4 == 0, "a matrix is not aligned to its elements");
+    const size_t need = layout_of(*p, false).bytes;
+    SCS_ARG(workspace_bytes >= need && workspace_dev && (uintptr_t)workspace_dev % 16 == 0, "the workspace is too small, NULL or not aligned to 16 bytes (scs_lowrank_workspace)");
+    DeviceGuard dev(handle_device(h));
+    if (dev.rc != SCS_OK) return dev.rc;
+    unsigned char* ws = (unsigned char*)workspace_dev;
+    hipStream_t st = (hipStream_t)stream;
+    if (p->dtype == SCS_F32) return forward<float>(*p, x_dev, ldx, y_dev, ldy, hidden_dev, ws, st);
+    if (p->dtype == SCS_BF16) return forward<__bf16>(*p, x_dev, ldx, y_dev, ldy, hidden_dev, ws, st);
+    return forward<_Float16>(*p, x_dev, ldx, y_dev, ldy, hidden_dev, ws, st);
+}
+
+int scs_lowrank_backward(scs_handle h, const scs_lowrank* p, const void* x_dev, int64_t ldx, const void* dy_dev, int64_t lddy,
+                         const float* hidden_dev, void* dx_dev, int64_t lddx, float* da_dev, float* db_dev,
+                         void* workspace_dev, size_t workspace_bytes, void* stream) {
+    SCS_ARG(h != nullptr, "null handle");
+    int rc = check(p);
+    if (rc != SCS_OK) return rc;
+    SCS_ARG(dx_dev || da_dev || db_dev, "no output is asked for");
+    const size_t e = p->dtype == SCS_F32 ? 4 : 2;
+    const bool none = p->rows == 0 || p->n_requests == 0;
+    SCS_ARG(none || (dy_dev && lddy >= p->out_features), "dy is NULL or its row stride below the row's length");
+    SCS_ARG(none || (!da_dev && !(db_dev && !hidden_dev)) || (x_dev && ldx >= p->in_features), "x is NULL or its row stride below the row's length");
+    SCS_ARG(none || !dx_dev || lddx >= p->in_features, "the row stride of dx is below the row's length");
+    SCS_ARG((uintptr_t)x_dev % e == 0 && (uintptr_t)dy_dev % e == 0 && (uintptr_t)dx_dev % e == 0 && (uintptr_t)hidden_dev % 4 == 0 &&
+            (uintptr_t)da_dev % 4 == 0 && (uintptr_t)db_dev % 4 == 0, "a matrix is not aligned to its elements");
+    const size_t need = layout_of(*p, true).bytes;
+    SCS_ARG(need == 0 || (workspace_bytes >= need && workspace_dev && (uintptr_t)workspace_dev % 16 == 0),
+            "the workspace is too small, NULL or not aligned to 16 bytes (scs_lowrank_workspace)");
+    DeviceGuard dev(handle_device(h));
+    if (dev.rc != SCS_OK) return dev.rc;
+    unsigned char* ws = (unsigned char*)workspace_dev;
+    hipStream_t st = (hipStream_t)stream;
+    if (none) dx_dev = nullptr;
+    if (p->dtype == SCS_F32) return backward<float>(*p, x_dev, ldx, dy_dev, lddy, hidden_dev, dx_dev, lddx, da_dev, db_dev, ws, st);
+    if (p->dtype == SCS_BF16) return backward<__bf16>(*p, x_dev, ldx, dy_dev, lddy, hidden_dev, dx_dev, lddx, da_dev, db_dev, ws, st);
+    return backward<_Float16>(*p, x_dev, ldx, dy_dev, lddy, hidden_dev, dx_dev, lddx, da_dev, db_dev, ws, st);
+}
+
+}  // extern "C"

@@ -15,6 +15,46 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ _Float16 from_f32<_Float16>(float x) { return (_Float16)x; }
 template <> __device__ __forceinline__ __bf16 from_f32<__bf16>(float x) { return (__bf16)x; }
 
+// ---- four consecutive elements of a type, held as loaded
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+template <class T> struct Vec4;
+template <> struct Vec4<float> { typedef f32x4 raw; };
+template <> struct Vec4<__bf16> { typedef u32x2 raw; };
+template <> struct Vec4<_Float16> { typedef u32x2 raw; };
+// four consecutive elements at any element alignment (the global loads of gfx950 need none)
+template <class R> struct __attribute__((packed, aligned(2))) Loose { R v; };
+
+template <class T> __device__ __forceinline__ void raw_load(typename Vec4<T>::raw& r, const T* p, int left) {
+    if (left >= 4) r = reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v;
+    else {
+        T e[4] = {};
+        for (int i = 0; i < 3; ++i) if (i < left) e[i] = p[i];
+        __builtin_memcpy(&r, e, sizeof(r));
+    }
+}
+template <class T> __device__ __forceinline__ void raw_store(const typename Vec4<T>::raw& r, T* p, int left) {
+    if (left >= 4) reinterpret_cast<Loose<typename Vec4<T>::raw>*>(p)->v = r;
+    else {
+        T e[4];
+        __builtin_memcpy(e, &r, sizeof(r));
+        for (int i = 0; i < 3; ++i) if (i < left) p[i] = e[i];
+    }
+}
+template <class T> __device__ __forceinline__ void unpack(const typename Vec4<T>::raw& r, float (&f)[4]) {
+    T e[4];
+    __builtin_memcpy(e, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = to_f32(e[i]);
+}
+template <class T> __device__ __forceinline__ typename Vec4<T>::raw pack(const float (&f)[4]) {
+    T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(f[i]);           // to the nearest, ties to even
+    typename Vec4<T>::raw r;
+    __builtin_memcpy(&r, e, sizeof(r));
+    return r;
+}
+
 int handle_device(scs_handle h);          // (scs_api.hip)
 
 // The handle's device is current inside a call and the caller's again behind it.

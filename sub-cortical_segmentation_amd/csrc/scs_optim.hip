@@ -108,45 +108,6 @@ __device__ __forceinline__ float block_scale(float amax, float k) {
     return s < 0x1p-126f ? 0.f : s;              // (a subnormal scale has no reciprocal: such a block holds zeros)
 }
 
-typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
-template <class T> struct Vec4;
-template <> struct Vec4<float> { typedef f32x4 raw; };
-template <> struct Vec4<__bf16> { typedef u32x2 raw; };
-template <> struct Vec4<_Float16> { typedef u32x2 raw; };
-// four consecutive elements at any element alignment (the global loads of gfx950 need none)
-template <class R> struct __attribute__((packed, aligned(2))) Loose { R v; };
-
-template <class T> __device__ __forceinline__ void raw_load(typename Vec4<T>::raw& r, const T* p, int left) {
-    if (left >= 4) r = reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v;
-    else {
-        T e[4] = {};
-        for (int i = 0; i < 3; ++i) if (i < left) e[i] = p[i];
-        __builtin_memcpy(&r, e, sizeof(r));
-    }
-}
-template <class T> __device__ __forceinline__ void raw_store(const typename Vec4<T>::raw& r, T* p, int left) {
-    if (left >= 4) reinterpret_cast<Loose<typename Vec4<T>::raw>*>(p)->v = r;
-    else {
-        T e[4];
-        __builtin_memcpy(e, &r, sizeof(r));
-        for (int i = 0; i < 3; ++i) if (i < left) p[i] = e[i];
-    }
-}
-template <class T> __device__ __forceinline__ void unpack(const typename Vec4<T>::raw& r, float (&f)[4]) {
-    T e[4];
-    __builtin_memcpy(e, &r, sizeof(r));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = to_f32(e[i]);
-}
-template <class T> __device__ __forceinline__ typename Vec4<T>::raw pack(const float (&f)[4]) {
-    T e[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) e[i] = from_f32<T>(f[i]);           // to the nearest, ties to even
-    typename Vec4<T>::raw r;
-    __builtin_memcpy(&r, e, sizeof(r));
-    return r;
-}
-
 // one wave's blocks of one chunk; the moments' arenas are padded to whole blocks, the pads hold zeros and are written as such
 template <class PT, class GT, int BITS>
 __device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptTensor& t, const GT* __restrict__ g, int block, const Coef& k) {

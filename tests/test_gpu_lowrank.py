@@ -1,0 +1,137 @@
+"""The shared projection with a low-rank adapter per request (cnn_cort.adapters.Projection, scs_lowrank_*) against the same formulas in
+float64.  Needs an MI355X.
+
+Tolerances, in units of u = 2^-24 (float32) and r = eps / 2 of the outputs' type.  A sum of n products of exact operands, formed in float32
+in any order, is off by at most n u sum |products|; the bounds below use |x| |W| sums formed in float64 ("big"), the inner value
+h = x A^T has n_in u big_h, and its way through scale (1 u), the two 16-bit pieces (2 r^2: below u for bf16's r = 2^-9 only up to
+2^-17, which is counted), B and the sum adds the rest.  The output's own rounding is r |y| (on the value with its error)."""
+import numpy as np
+import pytest
+import torch
+
+from cnn_cort import _hip
+from cnn_cort.adapters import Projection
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+TYPES = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+HALF = {'f32': 2.0 ** -24, 'bf16': 2.0 ** -8, 'f16': 2.0 ** -11}                      # half a step, relative
+PIECES = {'f32': 0.0, 'bf16': 2.0 ** -16, 'f16': 2.0 ** -22}                          # what two 16-bit pieces leave of a float32
+
+
+def data(t, rows, n_in, n_out, rank, adapters, seed, bias=True):
+    g = torch.Generator().manual_seed(seed)
+    mk = lambda *s, std=1.0: (torch.randn(s, generator=g) * std).to(TYPES[t]).to('cuda:0')
+    return {'x': mk(rows, n_in), 'dy': mk(rows, n_out), 'w': mk(n_in, n_out, std=n_in ** -0.5), 'a': mk(adapters, rank, n_in, std=n_in ** -0.5),
+            'b': mk(adapters, rank, n_out, std=0.3), 'bias': mk(n_out) if bias else None,
+            'scale': (0.5 + torch.rand((adapters,), generator=g)).to('cuda:0')}
+
+
+def requests(off, ids):
+    return torch.tensor(off, dtype=torch.int32, device='cuda:0'), torch.tensor(ids, dtype=torch.int32, device='cuda:0')
+
+
+def f64(t):
+    return None if t is None else t.detach().double().cpu().numpy()
+
+
+def reference(d, off, ids, t, hidden=None):
+    """Values and bounds of the forward and backward results on the live rows."""
+    x, dy, w, a, b = (f64(d[k]) for k in ('x', 'dy', 'w', 'a', 'b'))
+    sc = f64(d['scale']) if d['scale'] is not None else np.ones(a.shape[0])
+    bias = f64(d['bias']) if d['bias'] is not None else np.zeros(w.shape[1])
+    rows, n_in, n_out, rank = x.shape[0], x.shape[1], w.shape[1], a.shape[1]
+    half, pc = HALF[t], PIECES[t]
+    y, by = x @ w + bias, (n_in + 2) * U * (np.abs(x) @ np.abs(w) + np.abs(bias))
+    dx, bdx = dy @ w.T, (n_out + 2) * U * (np.abs(dy) @ np.abs(w).T)
+    h = np.zeros((rows, rank))
+    bh = np.zeros((rows, rank))
+    da, db = np.zeros_like(a), np.zeros_like(b)
+    bda, bdb = np.zeros_like(a), np.zeros_like(b)
+    live = np.zeros(rows, bool)
+    for q, s in enumerate(ids):
+        lo, hi = off[q], off[q + 1]
+        live[lo:hi] = True
+        if s < 0 or s >= a.shape[0] or hi <= lo:
+            continue
+        X, D = x[lo:hi], dy[lo:hi]
+        h[lo:hi] = X @ a[s].T
+        bh[lo:hi] = n_in * U * (np.abs(X) @ np.abs(a[s]).T)
+        H, BH = h[lo:hi], bh[lo:hi]
+        k = (rank + 4) * U + pc
+        y[lo:hi] += sc[s] * H @ b[s]
+        by[lo:hi] += abs(sc[s]) * (BH + k * np.abs(H)) @ np.abs(b[s]) + 2 * U * abs(sc[s]) * np.abs(H) @ np.abs(b[s])
+        G, BG = D @ b[s].T, n_out * U * (np.abs(D) @ np.abs(b[s]).T)
+        dx[lo:hi] += sc[s] * G @ a[s]
+        bdx[lo:hi] += abs(sc[s]) * (BG + (k + 2 * U) * np.abs(G)) @ np.abs(a[s])
+        da[s] += sc[s] * G.T @ X
+        db[s] += sc[s] * H.T @ D
+        bda[s] += abs(sc[s]) * (BG + (rows + 4) * U * np.abs(G)).T @ np.abs(X)
+        bdb[s] += abs(sc[s]) * (BH + (rows + 4) * U * np.abs(H)).T @ np.abs(D)
+    by += half * (np.abs(y) + by) + 1e-30
+    bdx += half * (np.abs(dx) + bdx) + 1e-30
+    if t == 'f16':                                                       # f16's smallest steps
+        by, bdx = by + 2.0 ** -25, bdx + 2.0 ** -25
+    return {'y': (y, by), 'dx': (dx, bdx), 'h': (h, bh + 1e-30), 'da': (da, bda + 1e-30), 'db': (db, bdb + 1e-30), 'live': live}
+
+
+def within(got, ref, bound, what):
+    got = f64(got)
+    bad = ~(np.abs(got - ref) <= bound)
+    if bad.any():
+        i = np.unravel_index(np.argmax(np.where(bad, np.abs(got - ref) / bound, 0)), got.shape)
+        raise AssertionError('%s: %d of %d beyond their bound; worst at %r: %r for %r (bound %.3g)' % (what, bad.sum(), bad.size, i, got[i], ref[i], bound[i]))
+
+
+def check_all(handle, d, off, ids, t, with_hidden=True):
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    o, i = requests(off, ids)
+    rows = d['x'].shape[0]
+    ref = reference(d, off, ids, t)
+    live = ref['live']
+    out = torch.full((rows, p.n_out), 3.0, dtype=TYPES[t], device='cuda:0')
+    hidden = torch.full((rows, p.rank), 5.0, device='cuda:0')
+    y = p.forward(d['x'], o, i, out=out, hidden=hidden)
+    assert y is out
+    within(y[torch.from_numpy(live).cuda()], ref['y'][0][live], ref['y'][1][live], 'y')
+    within(hidden[torch.from_numpy(live).cuda()], ref['h'][0][live], ref['h'][1][live], 'hidden')
+    assert (f64(out)[~live] == 3.0).all() and (f64(hidden)[~live] == 5.0).all()
+    dx0 = torch.full((rows, p.n_in), 3.0, dtype=TYPES[t], device='cuda:0')
+    dx, da, db = p.backward(d['x'], d['dy'], o, i, hidden=hidden if with_hidden else None, dx=dx0)
+    within(dx[torch.from_numpy(live).cuda()], ref['dx'][0][live], ref['dx'][1][live], 'dx')
+    assert (f64(dx)[~live] == 3.0).all()
+    within(da, ref['da'][0], ref['da'][1], 'da')
+    within(db, ref['db'][0], ref['db'][1], 'db')
+    again = p.backward(d['x'], d['dy'], o, i, hidden=hidden if with_hidden else None)
+    assert torch.equal(again[1], da) and torch.equal(again[2], db)                # the same bits every time
+    assert torch.equal(p.forward(d['x'], o, i)[torch.from_numpy(live).cuda()], y[torch.from_numpy(live).cuda()])
+
+
+# rows, in, out, rank, adapters, offsets, adapters of the requests
+CASES = {
+    'one row': (1, 64, 64, 16, 2, [0, 1], [1]),
+    'one of everything': (1, 1, 1, 1, 1, [0, 1], [0]),
+    'the second dense layer': (128, 555, 270, 8, 4, [0, 40, 41, 90, 128], [2, 0, 3, 1]),
+    'the first dense layer': (300, 540, 540, 8, 4, [0, 100, 200, 290], [0, 1, 0]),
+    'one token each': (33, 128, 192, 4, 5, list(range(34)), [i % 6 - 1 for i in range(33)]),
+    'odd': (70, 77, 131, 5, 3, [0, 3, 3, 64, 70], [2, 1, -1, 0]),
+    'requests end inside tiles': (700, 96, 200, 16, 3, [0, 15, 17, 127, 129, 600, 700], [0, 1, 2, 0, -1, 1]),
+    'rank above a slab': (530, 160, 96, 40, 2, [0, 200, 530], [1, 0]),
+    'largest rank': (40, 136, 72, 128, 2, [0, 20, 40], [1, 0]),
+    'rank of many rows': (600, 256, 128, 100, 2, [0, 333, 600], [1, 0]),
+    'rows behind and before the requests': (600, 64, 80, 8, 2, [20, 300, 577], [0, 1]),
+    'no request': (20, 32, 32, 4, 2, [0], []),
+    'only empty requests': (20, 32, 32, 4, 2, [7, 7, 7], [0, 1]),
+    'no adapter at all': (600, 64, 64, 4, 2, [0, 600], [-1]),
+    'numbers outside the bank': (64, 64, 64, 4, 2, [0, 20, 64], [2, -7]),
+    'more requests than a wave is wide': (1500, 72, 88, 8, 7, [15 * i for i in range(101)], [i % 8 - 1 for i in range(100)]),
+    'aligned': (1100, 512, 768, 16, 4, [0, 1, 256, 512, 1000, 1100], [0, 1, 2, 3, -1]),
+    'wide': (260, 64, 1000, 16, 2, [0, 130, 260], [0, 1]),
+}
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('case', list(CASES))
+def test_against_float64(handle, case, t):
+    rows, n_in, n_out, rank, adapters, off, ids = CASES[case]
+    check_all(handle, data(t, rows, n_in, n_out, rank, adapters, len(case) + rows, bias=rows % 2 == 0), off, ids, t, with_hidden=rows % 3 != 0)
