@@ -57,8 +57,10 @@ __device__ __forceinline__ Span span_of(const Requests& r, int q, int m0, int m1
 // contraction each, joined through LDS; operands go from global memory to the f32 matrix cores without a stop (both are contiguous along the
 // contraction: a lane's 16 or 8 bytes are its operand of four MFMAs, whose contraction indices are permuted alike on both sides).
 template <class T, int JT>
-__global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r) {
+__global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
+                                                          unsigned int* __restrict__ tickets, int n_tickets) {
     __shared__ float s_part[4][JT * 4][64];
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, kq = lane >> 4;
     const int m0 = blockIdx.x * 16, m1 = min(m0 + 16, r.rows);
@@ -109,34 +111,57 @@ __global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ 
     }
 }
 
-// Few rows: a wave per (row, direction) reads both vectors along the contraction and adds up over its lanes.
+// Few rows: a workgroup owns four directions of one row, its four waves a quarter of the contraction each (every load of the quarter of a
+// 4096-long row is in flight at once), joined through LDS.  It also clears the tickets of the projection behind it (lowrank_few.h).
+template <class T> __device__ __forceinline__ void load8f(const T* p, int left, float (&f)[8]) {
+    typename Vec4<T>::raw a, b;
+    raw_load<T>(a, p, left);
+    raw_load<T>(b, p + 4, left - 4);
+    float lo[4], hi[4];
+    unpack<T>(a, lo);
+    unpack<T>(b, hi);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
+}
 template <class T>
-__global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r) {
+__global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
+                                                          unsigned int* __restrict__ tickets, int n_tickets) {
+    __shared__ float s_part[4][4];
+    for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * gridDim.y * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int row = blockIdx.x, j = blockIdx.y * 4 + wave;
+    const int row = blockIdx.x, j0 = blockIdx.y * 4;
     const int q = first_request(r, row);
-    if (q >= r.n || j >= r.rank) return;
+    if (q >= r.n) return;
     const Span sp = span_of(r, q, row, row + 1);
     if (sp.lo >= sp.hi) return;
-    float sum = 0.f;
+    float sum[4] = {};
     if (sp.s >= 0) {
         const T* xr = x + (int64_t)row * ldx;
-        const T* pr = p + ((int64_t)sp.s * r.rank + j) * K;
-#pragma unroll 4
-        for (int k = lane * 4; k < K; k += 256) {
-            typename Vec4<T>::raw ra, rb;
-            raw_load<T>(ra, xr + k, K - k);
-            raw_load<T>(rb, pr + k, K - k);
-            float a[4], b[4];
-            unpack<T>(ra, a);
-            unpack<T>(rb, b);
+        const T* pr = p + ((int64_t)sp.s * r.rank + j0) * K;
+        const int per = (K + 2047) / 2048 * 512, k_hi = min(K, (wave + 1) * per);
+#pragma unroll 2
+        for (int k = wave * per + lane * 8; k < k_hi; k += 512) {
+            float a[8], b[4][8];
+            load8f(xr + k, K - k, a);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum = fmaf(a[i], b[i], sum);
+            for (int j = 0; j < 4; ++j) load8f(pr + (int64_t)min(j, r.rank - 1 - j0) * K + k, K - k, b[j]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sum[j] = fmaf(a[i], b[j][i], sum[j]);
         }
 #pragma unroll
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int o = 32; o; o >>= 1) sum[j] += __shfl_xor(sum[j], o);
     }
-    if (lane == 0) h[(int64_t)row * r.rank + j] = sum;
+    if (lane == 0)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s_part[wave][j] = sum[j];
+    __syncthreads();
+    const int j = j0 + (int)threadIdx.x;
+    if (threadIdx.x < 4 && j < r.rank)
+        h[(int64_t)row * r.rank + j] = (s_part[0][threadIdx.x] + s_part[1][threadIdx.x]) + (s_part[2][threadIdx.x] + s_part[3][threadIdx.x]);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ project, f32 matrix cores
@@ -299,6 +324,13 @@ __global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
     }
 }
 
+}  // namespace
+}  // namespace scs
+#include "lowrank_mfma16.h"
+#include "lowrank_few.h"
+namespace scs {
+namespace {
+
 // ------------------------------------------------------------------------------------------------------------------ wgrad
 // G_s[j][k] = scale_s sum over the rows of s of H[row][j] X[row][k], f32.  A workgroup owns 64 columns of one adapter and one slice of the
 // rows; a lane's vector of X is its operand of four MFMAs (columns 4 c + t of MFMA t), the four waves take every fourth group of four rows
@@ -392,21 +424,40 @@ int wgrad_slices(const scs_lowrank& p, int64_t F) {
     return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
 }
 
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, bytes = 0; };
+// ---- few rows (lowrank_few.h)
+struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; int tickets = 0; };      // mt 0: the tile kernels
+Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
+    Few f;
+    if (p.rows > (p.dtype == SCS_F32 ? 512 : 64)) return f;
+    f.mt = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
+    if (p.dtype == SCS_F32 && p.rows > 64) f.mt = 2;
+    f.tiles_n = (int)((N + 63) / 64);
+    f.tiles_m = (int)((p.rows + 16 * f.mt - 1) / (16 * f.mt));
+    const int64_t steps = (K + 31) / 32;
+    f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.rows <= 16 ? 512 : 256) / ((int64_t)f.tiles_n * f.tiles_m), steps / (2 * kFewWaves)));
+    if (f.splits > 1) {
+        f.part = (size_t)f.splits * f.tiles_m * 16 * f.mt * f.tiles_n * 64 * 4;
+        f.tickets = f.tiles_n * f.tiles_m;
+    }
+    return f;
+}
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t b) { const size_t o = at; at += up(b); return o; };
     l.hid = take((size_t)p.rows * p.rank * 4);
+    const Few f = backward ? few_of(p, p.out_features, p.in_features) : few_of(p, p.in_features, p.out_features);
+    size_t part = f.part;
+    l.tickets = take((size_t)f.tickets * 4);
     if (backward) {
         l.hid2 = take((size_t)p.rows * p.rank * 4);
-        size_t part = 0;
         for (const int64_t F : {p.in_features, p.out_features}) {
             const int s = wgrad_slices(p, F);
             if (s > 1) part = std::max(part, (size_t)s * p.n_adapters * p.rank * F * 4);
         }
-        l.part = take(part);
     }
+    l.part = take(part);
     l.bytes = at;
     return l;
 }
@@ -437,18 +488,36 @@ template <class F> void by_tiles(int rank, F&& f) {
     else f(std::integral_constant<int, 8>{});
 }
 
-template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st) {
+template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st, unsigned int* tickets = nullptr, int n_tickets = 0) {
     const Requests r = requests_of(p);
     if (p.rows <= kDotRows) {
-        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r);
+        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r, tickets, n_tickets);
         return;
     }
     by_tiles(p.rank, [&](auto jt) {
-        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r);
+        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r, tickets, n_tickets);
     });
 }
 
-template <class T, bool TRANS> void project(const ProjectArgs<T>& g, hipStream_t st) {
+template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const Few& f, float* part, unsigned int* tickets, hipStream_t st) {
+    const dim3 grid(f.tiles_n, f.tiles_m, f.splits);
+    if (f.mt == 1) hipLaunchKernelGGL((project_few_kernel<T, 1, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
+    else if (f.mt == 2) hipLaunchKernelGGL((project_few_kernel<T, 2, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
+    else hipLaunchKernelGGL((project_few_kernel<T, 4, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
+}
+
+template <class T, bool TRANS> void project16(const ProjectArgs<T>& g, hipStream_t st) {
+    auto tiles = [&](int b) { return (int64_t)((g.r.rows + b - 1) / b) * ((g.N + b - 1) / b); };
+    const bool aligned = g.K % 8 == 0 && g.N % 8 == 0 && g.ldx % 8 == 0 && g.ldw % 8 == 0 && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.w % 16 == 0;
+    if (tiles(256) >= 192 && aligned)
+        hipLaunchKernelGGL((project16_kernel<T, 2, 4, 8, 4, TRANS, true>), dim3((unsigned)tiles(256)), dim3(512), 0, st, g);
+    else if (aligned) hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, true>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, false>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
+}
+
+template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& f, float* part, unsigned int* tickets, hipStream_t st) {
+    if (f.mt) { project_few<T, TRANS>(g, f, part, tickets, st); return; }
+    if constexpr (sizeof(T) == 2) { project16<T, TRANS>(g, st); return; }
     // the column tile with the least padding, the widest among equals
     int best = 8, waste = 1 << 30;
     for (const int nt : {8, 6, 4}) {
@@ -477,8 +546,10 @@ template <class T>
 int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t ldy, float* hidden, unsigned char* ws, hipStream_t st) {
     const Layout l = layout_of(p, false);
     float* h = hidden ? hidden : (float*)(ws + l.hid);
-    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st);
-    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)}, st);
+    const Few f = few_of(p, p.in_features, p.out_features);
+    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st, (unsigned int*)(ws + l.tickets), f.tickets);
+    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)},
+                      f, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }
@@ -490,9 +561,11 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     float* u = (float*)(ws + l.hid);
     float* part = (float*)(ws + l.part);
     const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
-    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st);
+    const Few f = few_of(p, p.out_features, p.in_features);
+    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st, (unsigned int*)(ws + l.tickets), f.tickets);
     if (dx)
-        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)}, st);
+        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
+                         f, part, (unsigned int*)(ws + l.tickets), st);
     if (da) wgrad<T>(p, u, (const T*)x, ldx, (int)p.in_features, da, part, st);
     if (db) {
         const float* h = hidden;

@@ -127,6 +127,12 @@ CASES = {
     'more requests than a wave is wide': (1500, 72, 88, 8, 7, [15 * i for i in range(101)], [i % 8 - 1 for i in range(100)]),
     'aligned': (1100, 512, 768, 16, 4, [0, 1, 256, 512, 1000, 1100], [0, 1, 2, 3, -1]),
     'wide': (260, 64, 1000, 16, 2, [0, 130, 260], [0, 1]),
+    'one row, long contractions': (1, 4096, 1040, 16, 3, [0, 1], [2]),
+    'few rows, long contractions': (13, 2056, 1500, 33, 3, [0, 1, 5, 5, 12], [2, 0, 1, -1]),
+    'tokens, long contractions': (48, 2000, 1111, 20, 5, list(range(49)), [i % 7 - 1 for i in range(48)]),
+    'few rows above a tile': (61, 1033, 640, 8, 2, [0, 30, 60], [1, 0]),
+    'many tiles': (3100, 264, 4104, 16, 3, [0, 100, 1500, 1501, 3000, 3090], [0, 1, 2, -1, 0]),
+    'many tiles the other way': (2100, 4096, 328, 24, 3, [0, 700, 1500, 2100], [0, 1, 2]),
 }
 
 
