@@ -7,6 +7,7 @@ mini-batch, one new token), each with its own adapter or none.  The layers it st
 (nets.py:179, 217, 227); W keeps their (in, out) order.
 """
 import ctypes
+import threading
 
 from . import _hip
 
@@ -65,7 +66,12 @@ class Projection:
             if tuple(scale.shape) != (self.n_adapters,) or not scale.is_contiguous():
                 raise ValueError('scale must be a contiguous [%d]' % self.n_adapters)
         self._lib = _hip.load_library()
-        self._plan = (self._types[self.dtype], ldw, w.data_ptr(), _hip._ptr(bias), a.data_ptr(), b.data_ptr(), _hip._ptr(scale))
+        self._item = w.element_size()
+        self._plan = (self._types[self.dtype], self.rank, self.n_adapters, 0, 0, self.n_in, self.n_out, ldw, w.data_ptr(), _hip._ptr(bias), a.data_ptr(),
+                      b.data_ptr(), _hip._ptr(scale), None, None)
+        self._reads = [(t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * ldw + self.n_out if t is w else t.numel()) * t.element_size())
+                       for t in (w, a, b, bias, scale) if t is not None]
+        self._sizes, self._tls = {}, threading.local()
 
     def _own(self, t, what, dtype):
         if not self._torch.is_tensor(t) or t.dtype != dtype:
@@ -76,70 +82,88 @@ class Projection:
     @staticmethod
     def _stride(t, what):
         """Row stride of a 2-D tensor whose rows are contiguous."""
-        rows, cols = t.shape
-        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+        (rows, cols), (d0, d1) = t.shape, t.stride()
+        if (cols > 1 and d1 != 1) or (rows > 1 and d0 < cols):
             raise ValueError('the rows of %s must be contiguous and apart' % what)
-        return max(int(t.stride(0)), int(cols)) if rows > 1 else int(cols)
+        return d0 if rows > 1 and d0 > cols else cols
 
-    def _rows(self, t, cols, what, rows=None):
+    def _rows(self, t, rows, cols, what):
+        """(address, row stride, end address) of a [rows, cols] tensor of the projection's type."""
         self._own(t, what, self.dtype)
-        if t.dim() != 2 or int(t.shape[1]) != cols or (rows is not None and int(t.shape[0]) != rows):
-            raise ValueError('%s must be [%s, %d], got %r' % (what, 'rows' if rows is None else rows, cols, tuple(t.shape)))
-        return self._stride(t, what)
+        if tuple(t.shape) != (rows, cols):
+            raise ValueError('%s must be [%d, %d], got %r' % (what, rows, cols, tuple(t.shape)))
+        ld, at = self._stride(t, what), t.data_ptr()
+        return at, ld, at + (((rows - 1) * ld + cols) * self._item if rows else 0)
 
-    def _call(self, rows, offsets, adapters):
+    def _flat(self, t, shape, what):
+        """(address, 0, end address) of a contiguous float32 tensor of a shape."""
+        self._own(t, what, self._torch.float32)
+        if tuple(t.shape) != shape or not t.is_contiguous():
+            raise ValueError('%s must be a contiguous float32 %r' % (what, shape))
+        at = t.data_ptr()
+        return at, 0, at + 4 * t.numel()
+
+    @staticmethod
+    def _apart(outs, reads):
+        """No output shares memory with what the call reads or with another output."""
+        for i, (what, (at, _, end)) in enumerate(outs):
+            for a, b in reads:
+                if at < b and a < end:
+                    raise ValueError('%s shares memory with a tensor that the call reads' % what)
+            for _, (a, _, b) in outs[:i]:
+                if at < b and a < end:
+                    raise ValueError('%s shares memory with another output' % what)
+
+    def _call(self, x, rows, offsets, adapters):
+        """The call's description on this thread (one per thread: two threads may call at once)."""
         torch = self._torch
+        if x.dim() != 2:
+            raise ValueError('x must be [rows, %d], got %r' % (self.n_in, tuple(x.shape)))
         for t, what in ((offsets, 'offsets'), (adapters, 'adapters')):
             self._own(t, what, torch.int32)
             if t.dim() != 1 or not t.is_contiguous():
                 raise ValueError('%s must be 1-D and contiguous' % what)
-        if offsets.numel() != adapters.numel() + 1:
-            raise ValueError('%d offsets for %d requests (one more than requests)' % (offsets.numel(), adapters.numel()))
-        dt, ldw, w, bias, a, b, scale = self._plan
-        return _Call(dt, self.rank, self.n_adapters, adapters.numel(), rows, self.n_in, self.n_out, ldw, w, bias, a, b, scale,
-                     offsets.data_ptr(), adapters.data_ptr() if adapters.numel() else None)
+        n = adapters.numel()
+        if offsets.numel() != n + 1:
+            raise ValueError('%d offsets for %d requests (one more than requests)' % (offsets.numel(), n))
+        call = getattr(self._tls, 'call', None)
+        if call is None:
+            call = self._tls.call = _Call(*self._plan)
+            self._tls.ref = ctypes.byref(call)
+        call.rows, call.n_requests, call.offsets, call.adapters = rows, n, offsets.data_ptr(), adapters.data_ptr()
+        return self._tls.ref
 
-    def _workspace(self, call, back):
-        n = ctypes.c_size_t(0)
-        _hip._check(self._lib.scs_lowrank_workspace(self.handle.h, ctypes.byref(call), back, ctypes.byref(n)), 'scs_lowrank_workspace')
-        return self._torch.empty((max(16, n.value),), dtype=self._torch.uint8, device=self.device), n.value
-
-    def _hidden(self, hidden, rows):
-        self._own(hidden, 'hidden', self._torch.float32)
-        if tuple(hidden.shape) != (rows, self.rank) or not hidden.is_contiguous():
-            raise ValueError('hidden must be a contiguous float32 [%d, %d]' % (rows, self.rank))
-        return hidden.data_ptr()
-
-    def _apart(self, out, what, *others):
-        """An output must not share memory with what the call reads."""
-        lo, hi = self._extent(out)
-        for t in others:
-            if t is not None:
-                a, b = self._extent(t)
-                if lo < b and a < hi:
-                    raise ValueError('%s shares memory with a tensor that the call reads or writes' % what)
-
-    @staticmethod
-    def _extent(t):
-        n = t.numel() and sum((s - 1) * d for s, d in zip(t.shape, t.stride())) + 1
-        return t.data_ptr(), t.data_ptr() + n * t.element_size()
+    def _workspace(self, call, back, rows):
+        """Workspace of a call; its size hangs on the numbers of rows alone."""
+        n = self._sizes.get((back, rows))
+        if n is None:
+            size = ctypes.c_size_t(0)
+            _hip._check(self._lib.scs_lowrank_workspace(self.handle.h, call, back, ctypes.byref(size)), 'scs_lowrank_workspace')
+            if len(self._sizes) > 4096:
+                self._sizes.clear()
+            n = self._sizes[back, rows] = size.value
+        return self._torch.empty((n + 16,), dtype=self._torch.uint8, device=self.device), n
 
     def forward(self, x, offsets, adapters, out=None, hidden=None):
         """y [rows, out] for x [rows, in].  Request q owns rows [offsets[q], offsets[q + 1]) (int32 on the device, ascending) and uses adapter
         adapters[q] (int32; -1, or a number outside the bank: none).  Rows outside [offsets[0], offsets[-1]) of `out` are left as they were;
         without `out` they are zeros.  `hidden` (float32 [rows, rank]) receives x_i A_s^T for backward()."""
         torch = self._torch
-        ldx = self._rows(x, self.n_in, 'x')
-        rows = int(x.shape[0])
-        call = self._call(rows, offsets, adapters)
+        rows = x.shape[0]
+        call = self._call(x, rows, offsets, adapters)
+        px = self._rows(x, rows, self.n_in, 'x')
         if out is None:
             out = torch.zeros((rows, self.n_out), dtype=self.dtype, device=self.device)
-        ldy = self._rows(out, self.n_out, 'out', rows)
-        self._apart(out, 'out', x, self.w, self.a, self.b, self.bias, hidden)
-        hp = None if hidden is None else self._hidden(hidden, rows)
-        ws, n = self._workspace(call, 0)
-        _hip._check(self._lib.scs_lowrank_forward(self.handle.h, ctypes.byref(call), x.data_ptr(), ldx, out.data_ptr(), ldy, hp, ws.data_ptr(), n,
-                                                  torch.cuda.current_stream(self.device).cuda_stream or None), 'scs_lowrank_forward')
+        py = self._rows(out, rows, self.n_out, 'out')
+        outs = [('out', py)]
+        if hidden is not None:
+            outs.append(('hidden', self._flat(hidden, (rows, self.rank), 'hidden')))
+        self._apart(outs, [(px[0], px[2])] + self._reads)
+        ws, n = self._workspace(call, 0, rows)
+        rc = self._lib.scs_lowrank_forward(self.handle.h, call, px[0], px[1], py[0], py[1], outs[1][1][0] if hidden is not None else None,
+                                           ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
+        if rc:
+            _hip._check(rc, 'scs_lowrank_forward')
         return out
 
     def backward(self, x, dy, offsets, adapters, hidden=None, dx=None, da=None, db=None, want=('dx', 'da', 'db')):
@@ -147,41 +171,38 @@ class Projection:
         adapter's requests (zeros where there are none); None for what `want` does not name.  `hidden`: what forward() left, or None (formed
         again).  Rows of `dx` outside the requests are left as they were, without `dx` they are zeros."""
         torch = self._torch
-        ldx = self._rows(x, self.n_in, 'x')
-        rows = int(x.shape[0])
-        lddy = self._rows(dy, self.n_out, 'dy', rows)
-        call = self._call(rows, offsets, adapters)
-        for k in want:
-            if k not in ('dx', 'da', 'db'):
-                raise ValueError("want names 'dx', 'da' and 'db', got %r" % (k,))
-        if not want:
-            raise ValueError('want names nothing')
-        lddx = 0
+        rows = x.shape[0]
+        call = self._call(x, rows, offsets, adapters)
+        px, pdy = self._rows(x, rows, self.n_in, 'x'), self._rows(dy, rows, self.n_out, 'dy')
+        if not want or any(k not in ('dx', 'da', 'db') for k in want):
+            raise ValueError("want names some of 'dx', 'da' and 'db', got %r" % (want,))
+        outs = []
         if 'dx' in want:
             if dx is None:
                 dx = torch.zeros((rows, self.n_in), dtype=self.dtype, device=self.device)
-            lddx = self._rows(dx, self.n_in, 'dx', rows)
+            pdx = self._rows(dx, rows, self.n_in, 'dx')
+            outs.append(('dx', pdx))
         else:
-            dx = None
-        shapes = {'da': (self.n_adapters, self.rank, self.n_in), 'db': (self.n_adapters, self.rank, self.n_out)}
-        grads = {}
-        for k, t in (('da', da), ('db', db)):
+            dx, pdx = None, (None, 0)
+        pg = []
+        for k, t, cols in (('da', da, self.n_in), ('db', db, self.n_out)):
             if k not in want:
-                grads[k] = None
+                pg.append((None, None))
                 continue
+            shape = (self.n_adapters, self.rank, cols)
             if t is None:
-                t = torch.empty(shapes[k], dtype=torch.float32, device=self.device)
-            self._own(t, k, torch.float32)
-            if tuple(t.shape) != shapes[k] or not t.is_contiguous():
-                raise ValueError('%s must be a contiguous float32 %r' % (k, shapes[k]))
-            grads[k] = t
-        da, db = grads['da'], grads['db']
-        for t, what, more in ((dx, 'dx', (da, db)), (da, 'da', (db,)), (db, 'db', ())):
-            if t is not None:
-                self._apart(t, what, x, dy, self.w, self.a, self.b, hidden, *more)
-        hp = None if hidden is None else self._hidden(hidden, rows)
-        ws, n = self._workspace(call, 1)
-        _hip._check(self._lib.scs_lowrank_backward(self.handle.h, ctypes.byref(call), x.data_ptr(), ldx, dy.data_ptr(), lddy, hp, _hip._ptr(dx), lddx,
-                                                   _hip._ptr(da), _hip._ptr(db), ws.data_ptr(), n,
-                                                   torch.cuda.current_stream(self.device).cuda_stream or None), 'scs_lowrank_backward')
-        return dx, da, db
+                t = torch.empty(shape, dtype=torch.float32, device=self.device)
+            outs.append((k, self._flat(t, shape, k)))
+            pg.append((t, outs[-1][1][0]))
+        reads = [(px[0], px[2]), (pdy[0], pdy[2])] + self._reads
+        ph = None
+        if hidden is not None:
+            ph = self._flat(hidden, (rows, self.rank), 'hidden')
+            reads.append((ph[0], ph[2]))
+        self._apart(outs, reads)
+        ws, n = self._workspace(call, 1, rows)
+        rc = self._lib.scs_lowrank_backward(self.handle.h, call, px[0], px[1], pdy[0], pdy[1], ph and ph[0], pdx[0], pdx[1], pg[0][1], pg[1][1],
+                                            ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
+        if rc:
+            _hip._check(rc, 'scs_lowrank_backward')
+        return dx, pg[0][0], pg[1][0]

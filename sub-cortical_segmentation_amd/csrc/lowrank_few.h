@@ -15,20 +15,31 @@
 namespace scs {
 namespace {
 
-// what a coherent store has written is visible to every XCD once it is acknowledged: no cache has to be written back for it
-__device__ __forceinline__ void coherent_store(float* p, const f32x4& v) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) __hip_atomic_store(p + i, v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Partial sums travel past the L2s (one per XCD): written through to, and read from, the memory that all of them share (cache policy sc0 sc1),
+// so that no cache has to be written back or emptied around the ticket.  A store is there once it is acknowledged (vmcnt).
+constexpr int kCoherent = 1 | 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t part_buffer(float* p, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)bytes, 0x00020000);
 }
-__device__ __forceinline__ f32x4 coherent_load(const float* p) {
+__device__ __forceinline__ void coherent_store(__amdgpu_buffer_rsrc_t b, int at, const f32x4& v) {
+    u32x4 u;
+    __builtin_memcpy(&u, &v, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(u, b, at * 4, 0, kCoherent);
+}
+__device__ __forceinline__ f32x4 coherent_load(__amdgpu_buffer_rsrc_t b, int at) {
+    const u32x4 u = __builtin_amdgcn_raw_buffer_load_b128(b, at * 4, 0, kCoherent);
     f32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = __hip_atomic_load(p + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __builtin_memcpy(&v, &u, 16);
     return v;
 }
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 constexpr int kFewWaves = 8;
+
+template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
+template <class T> __device__ __forceinline__ u32x4 at8(const T* p) { return reinterpret_cast<const Loose<u32x4>*>(p)->v; }
+// where four columns from n on can be read from any row but W's last one (from the last one as well where N % 4 == 0)
+__device__ __forceinline__ int few_column(int n, int N) { return min(n, N % 4 ? N - 1 : N - 4); }
 
 // one step of the contraction: 32 (16-bit) or 16 (f32) values, four products of sixteen columns
 template <class T, int MT, bool TRANS> struct FewStep;
@@ -38,8 +49,22 @@ template <class T, int MT, bool TRANS> struct FewStep16 {
     u32x4 x[MT];
     u32x2 w[TRANS ? 1 : 8];
     u32x4 wt[TRANS ? 4 : 1];
-    __device__ __forceinline__ void load(const ProjectArgs<T>& g, int m0, int n, int k0, int lr, int kq) {
+    // rows and columns beyond the matrices are read as their last ones (nobody keeps what comes of them); only the last step looks at every element
+    __device__ __forceinline__ void load(const ProjectArgs<T>& g, int m0, int n, int k0, int lr, int kq, bool inside) {
         const int k = k0 + 8 * kq;
+        if (inside) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] = at8(g.x + (int64_t)min(m0 + 16 * i + lr, g.r.rows - 1) * g.ldx + k);
+            if constexpr (TRANS) {
+#pragma unroll
+                for (int t = 0; t < 4; ++t) wt[t] = at8(g.w + (int64_t)min(n + t, g.N - 1) * g.ldw + k);
+            } else {
+                const T* p = g.w + (int64_t)k * g.ldw + few_column(n, g.N);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = at4(p + i * g.ldw);
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const int m = m0 + 16 * i + lr;
@@ -77,8 +102,16 @@ template <int MT, bool TRANS> struct FewStep<_Float16, MT, TRANS> : FewStep16<_F
 template <int MT, bool TRANS> struct FewStep<float, MT, TRANS> {
     static constexpr int K = 16;
     f32x4 x[MT], w[4];
-    __device__ __forceinline__ void load(const ProjectArgs<float>& g, int m0, int n, int k0, int lr, int kq) {
+    __device__ __forceinline__ void load(const ProjectArgs<float>& g, int m0, int n, int k0, int lr, int kq, bool inside) {
         const int k = k0 + 4 * kq;
+        if (inside) {
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] = at4(g.x + (int64_t)min(m0 + 16 * i + lr, g.r.rows - 1) * g.ldx + k);
+            const float* p = TRANS ? g.w + k : g.w + (int64_t)k * g.ldw + few_column(n, g.N);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = at4(TRANS ? p + (int64_t)min(n + i, g.N - 1) * g.ldw : p + i * g.ldw);
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const int m = m0 + 16 * i + lr;
@@ -100,25 +133,38 @@ template <int MT, bool TRANS> struct FewStep<float, MT, TRANS> {
     }
 };
 
+// sixteen consecutive elements (zeros behind `left`)
+template <class T> struct Cols16 {
+    u32x4 v[sizeof(T)];
+    __device__ __forceinline__ void load(const T* p, int left) {
+        constexpr int PER = 16 / sizeof(T);
+        if (left >= 16) {
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T); ++i) v[i] = reinterpret_cast<const Loose<u32x4>*>(p + i * PER)->v;
+            return;
+        }
+        T e[16] = {};
+#pragma unroll
+        for (int i = 0; i < 15; ++i) if (i < left) e[i] = p[i];
+        __builtin_memcpy(v, e, sizeof(v));
+    }
+    __device__ __forceinline__ void four(int q, float (&f)[4]) const {
+        T e[16];
+        __builtin_memcpy(e, v, sizeof(v));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = to_f32(e[4 * q + i]);
+    }
+};
+
 template <class T, int MT, bool TRANS>
-__global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs<T> g, int splits, float* part, unsigned int* tickets) {
+__global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs<T> g, const int* __restrict__ row_adapter, int splits, float* part, unsigned int* tickets) {
     typedef FewStep<T, MT, TRANS> Step;
-    __shared__ f32x4 s_part[kFewWaves][MT * 4][64];
-    __shared__ int s_adapter[MT * 16];
+    __shared__ f32x4 s_part[kFewWaves][MT * 16][17];             // [row][16 columns' quarters + 1]: neither side of the join meets a bank twice
     __shared__ bool s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, kq = lane >> 4;
     const int n0 = blockIdx.x * 64, m0 = blockIdx.y * MT * 16, split = blockIdx.z;
     const Requests& r = g.r;
-
-    // the rows' adapters: -2 behind or before the requests, -1 none
-    if (tid < MT * 16) s_adapter[tid] = -2;
-    __syncthreads();
-    const int m1 = min(m0 + MT * 16, r.rows);
-    for (int q = first_request(r, m0) + tid; q < r.n && r.offsets[q] < m1; q += 64 * kFewWaves) {
-        const Span sp = span_of(r, q, m0, m1);
-        for (int m = sp.lo; m < sp.hi; ++m) s_adapter[m - m0] = sp.s;
-    }
 
     f32x4 acc[MT][4];
 #pragma unroll
@@ -128,52 +174,62 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
 
     const int steps = (g.K + Step::K - 1) / Step::K, shares = splits * kFewWaves, share = split * kFewWaves + wave;
     const int s0 = (int)((int64_t)steps * share / shares), s1 = (int)((int64_t)steps * (share + 1) / shares);
-    {
-        constexpr int AHEAD = MT <= 2 ? 2 : 1;
-        Step st[AHEAD + 1];
+    // (columns beyond N in W's last but one row run into its last one, which a stride of four and more covers)
+    const int inside = TRANS ? g.K : g.ldw < 4 || g.N < 4 ? 0 : g.N % 4 ? g.K - 1 : g.K;
+    constexpr int AHEAD = 3;
+    Step st[AHEAD + 1];
+    int adapter[MT];                                       // of row lr: -2 outside the requests, -1 none
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) if (s0 + i < s1) st[i].load(g, m0, n0 + 4 * lr, (s0 + i) * Step::K, lr, kq);
-        for (int s = s0; s < s1; s += AHEAD + 1) {
+    for (int i = 0; i < AHEAD; ++i) if (s0 + i < s1) st[i].load(g, m0, n0 + 4 * lr, (s0 + i) * Step::K, lr, kq, (s0 + i + 1) * Step::K <= inside);
 #pragma unroll
-            for (int i = 0; i <= AHEAD; ++i) {
-                if (s + i + AHEAD < s1) st[(i + AHEAD) % (AHEAD + 1)].load(g, m0, n0 + 4 * lr, (s + i + AHEAD) * Step::K, lr, kq);
-                if (s + i < s1) st[i].run(acc);
+    for (int i = 0; i < MT; ++i) adapter[i] = m0 + 16 * i + lr < r.rows ? row_adapter[m0 + 16 * i + lr] : -2;
+    // adapters: this wave's directions, one or two at a time, each row under its own adapter (the loads of all rows in flight together)
+    constexpr int U = sizeof(T) == 4 || MT == 4 ? 1 : 2;               // (two of these would not fit the registers)
+    for (int j0 = share; j0 < r.rank; j0 += U * shares) {
+        float h[U][MT];
+        Cols16<T> p[U][MT];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const int j = j0 + u * shares, m = min(m0 + 16 * i + lr, r.rows - 1);
+                const bool on = adapter[i] >= 0 && j < r.rank;
+                const int s = on ? adapter[i] : 0;
+                h[u][i] = on ? (r.scale ? r.scale[s] : 1.f) * g.h[(int64_t)m * r.rank + j] : 0.f;
+                p[u][i].load(g.low + ((int64_t)s * r.rank + (on ? j : 0)) * g.N + n0 + 16 * kq, on ? g.N - (n0 + 16 * kq) : 0);
             }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float f[4];
+                    p[u][i].four(e, f);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) acc[i][t][e] = fmaf(h[u][i], f[t], acc[i][t][e]);          // (0 x 0 where a row takes no part)
+                }
+    }
+
+    for (int s = s0; s < s1; s += AHEAD + 1) {
+#pragma unroll
+        for (int i = 0; i <= AHEAD; ++i) {
+            const int next = s + i + AHEAD;
+            if (next < s1) st[(i + AHEAD) % (AHEAD + 1)].load(g, m0, n0 + 4 * lr, next * Step::K, lr, kq, (next + 1) * Step::K <= inside);
+            if (s + i < s1) st[i].run(acc);
         }
     }
 
-    // adapters: this wave's directions
-    __syncthreads();
-    for (int j = share; j < r.rank; j += shares) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int m = m0 + 16 * i + lr, s = s_adapter[16 * i + lr];
-            if (s < 0) continue;
-            const float h = (r.scale ? r.scale[s] : 1.f) * g.h[(int64_t)m * r.rank + j];
-            const T* p = g.low + ((int64_t)s * r.rank + j) * g.N + n0 + 16 * kq;
-            const int left = g.N - (n0 + 16 * kq);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                typename Vec4<T>::raw rp;
-                raw_load<T>(rp, p + 4 * e, left - 4 * e);
-                float f[4];
-                unpack<T>(rp, f);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[i][t][e] = fmaf(h, f[t], acc[i][t][e]);
-            }
-        }
-    }
-
-    // row lr, columns 16 kq + 4 e + t of this lane
+    // this lane holds row lr, columns 16 kq + 4 e + t; behind the join a lane holds four columns of a row and sixteen lanes 64 of them, so that
+    // stores are whole lines (as the sums lie in the registers they would be 16-byte pieces: 26 us a call instead of 14 at 48 rows, 2048 x 8192, f16)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_part[wave][i * 4 + e][lane] = f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+        for (int e = 0; e < 4; ++e) s_part[wave][i * 16 + lr][4 * kq + e] = f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
     __syncthreads();
-    const int64_t plane = (int64_t)gridDim.y * MT * 16 * gridDim.x * 64;             // partial sums of one split, whole tiles
-    const int ldp = gridDim.x * 64;
-    auto finish = [&](f32x4 v, int m, int n, int s) {
-        if (s == -2 || m >= r.rows || n >= g.N) return;
+    const int ldp = gridDim.x * 64, plane = gridDim.y * MT * 16 * ldp;               // partial sums of one split, whole tiles
+    const __amdgpu_buffer_rsrc_t pb = part_buffer(part, (int64_t)splits * plane * 4);
+    auto finish = [&](f32x4 v, int m, int n) {
         float b[4] = {};
         if (g.bias) {
             typename Vec4<T>::raw rb;
@@ -183,13 +239,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
         const float f[4] = {v[0] + b[0], v[1] + b[1], v[2] + b[2], v[3] + b[3]};
         raw_store<T>(pack<T>(f), g.y + (int64_t)m * g.ldy + n, g.N - n);
     };
-    for (int e = wave; e < MT * 4; e += kFewWaves) {
-        f32x4 v = s_part[0][e][lane];
+    const int c4 = tid & 15, n = n0 + 4 * c4;
+    for (int row = tid >> 4; row < MT * 16; row += 4 * kFewWaves) {
+        const int m = m0 + row;
+        if (m >= r.rows || n >= g.N || row_adapter[m] == -2) continue;
+        f32x4 v = s_part[0][row][c4];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; ++w) v += s_part[w][e][lane];
-        const int mi = (e >> 2) * 16 + lr, n = n0 + 16 * kq + 4 * (e & 3);
-        if (splits == 1) finish(v, m0 + mi, n, s_adapter[mi]);
-        else coherent_store(part + split * plane + (int64_t)(m0 + mi) * ldp + n, v);
+        for (int w = 1; w < kFewWaves; ++w) v += s_part[w][row][c4];
+        if (splits == 1) finish(v, m, n);
+        else coherent_store(pb, split * plane + m * ldp + n, v);
     }
     if (splits == 1) return;
     stores_done();
@@ -198,14 +256,13 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
         s_last = __hip_atomic_fetch_add(&tickets[blockIdx.y * gridDim.x + blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned int)splits - 1;
     __syncthreads();
     if (!s_last) return;
-    for (int e = wave; e < MT * 4; e += kFewWaves) {
-        const int mi = (e >> 2) * 16 + lr, n = n0 + 16 * kq + 4 * (e & 3);
-        if (s_adapter[mi] == -2) continue;
-        const float* p = part + (int64_t)(m0 + mi) * ldp + n;
-        f32x4 v = coherent_load(p);
-#pragma unroll 4
-        for (int s = 1; s < splits; ++s) v += coherent_load(p + s * plane);
-        finish(v, m0 + mi, n, s_adapter[mi]);
+    for (int row = tid >> 4; row < MT * 16; row += 4 * kFewWaves) {
+        const int m = m0 + row;
+        if (m >= r.rows || n >= g.N || row_adapter[m] == -2) continue;
+        f32x4 v = coherent_load(pb, m * ldp + n);
+#pragma unroll 8
+        for (int i = 1; i < splits; ++i) v += coherent_load(pb, i * plane + m * ldp + n);
+        finish(v, m, n);
     }
 }
 

@@ -58,7 +58,7 @@ __device__ __forceinline__ Span span_of(const Requests& r, int q, int m0, int m1
 // contraction: a lane's 16 or 8 bytes are its operand of four MFMAs, whose contraction indices are permuted alike on both sides).
 template <class T, int JT>
 __global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
-                                                          unsigned int* __restrict__ tickets, int n_tickets) {
+                                                          int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
     __shared__ float s_part[4][JT * 4][64];
     for (int i = blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -68,10 +68,12 @@ __global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ 
     const int k_lo = wave * per * 16, k_hi = min(K, (wave + 1) * per * 16);
     const int row = min(m0 + lr, r.rows - 1);
     const T* xr = x + (int64_t)row * ldx;
+    int mine = -2;
     for (int q = first_request(r, m0); q < r.n; ++q) {
         const Span sp = span_of(r, q, m0, m1);
         if (r.offsets[q] >= m1) break;
         if (sp.lo >= sp.hi) continue;
+        if (m0 + (int)threadIdx.x >= sp.lo && m0 + (int)threadIdx.x < sp.hi) mine = sp.s;
         f32x4 acc[JT];
 #pragma unroll
         for (int t = 0; t < JT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -109,10 +111,12 @@ __global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ 
             if (m >= sp.lo && m < sp.hi && j < r.rank) h[(int64_t)m * r.rank + j] = v;
         }
     }
+    if (threadIdx.x < 16 && m0 + (int)threadIdx.x < r.rows) row_adapter[m0 + threadIdx.x] = mine;
 }
 
 // Few rows: a workgroup owns four directions of one row, its four waves a quarter of the contraction each (every load of the quarter of a
-// 4096-long row is in flight at once), joined through LDS.  It also clears the tickets of the projection behind it (lowrank_few.h).
+// 4096-long row is in flight at once), joined through LDS.  It also clears the
+// tickets of the projection behind it (lowrank_few.h); both shrink kernels leave every row's adapter (-2 outside the requests, -1 none).
 template <class T> __device__ __forceinline__ void load8f(const T* p, int left, float (&f)[8]) {
     typename Vec4<T>::raw a, b;
     raw_load<T>(a, p, left);
@@ -125,14 +129,15 @@ template <class T> __device__ __forceinline__ void load8f(const T* p, int left, 
 }
 template <class T>
 __global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
-                                                          unsigned int* __restrict__ tickets, int n_tickets) {
+                                                          int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
     __shared__ float s_part[4][4];
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * gridDim.y * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x, j0 = blockIdx.y * 4;
     const int q = first_request(r, row);
-    if (q >= r.n) return;
-    const Span sp = span_of(r, q, row, row + 1);
+    Span sp{0, 0, -1, 1.f};
+    if (q < r.n) sp = span_of(r, q, row, row + 1);
+    if (threadIdx.x == 0 && blockIdx.y == 0) row_adapter[row] = sp.lo < sp.hi ? sp.s : -2;
     if (sp.lo >= sp.hi) return;
     float sum[4] = {};
     if (sp.s >= 0) {
@@ -429,19 +434,18 @@ struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; 
 Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     Few f;
     if (p.rows > (p.dtype == SCS_F32 ? 512 : 64)) return f;
-    f.mt = p.rows <= 16 ? 1 : p.rows <= 32 ? 2 : 4;
-    if (p.dtype == SCS_F32 && p.rows > 64) f.mt = 2;
+    f.mt = p.dtype == SCS_F32 ? 1 : (int)(p.rows + 15) / 16;
     f.tiles_n = (int)((N + 63) / 64);
     f.tiles_m = (int)((p.rows + 16 * f.mt - 1) / (16 * f.mt));
     const int64_t steps = (K + 31) / 32;
-    f.splits = (int)std::max<int64_t>(1, std::min<int64_t>((p.rows <= 16 ? 512 : 256) / ((int64_t)f.tiles_n * f.tiles_m), steps / (2 * kFewWaves)));
+    f.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)f.tiles_n * f.tiles_m), steps / (2 * kFewWaves)));
     if (f.splits > 1) {
         f.part = (size_t)f.splits * f.tiles_m * 16 * f.mt * f.tiles_n * 64 * 4;
         f.tickets = f.tiles_n * f.tiles_m;
     }
     return f;
 }
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, bytes = 0; };
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward) {
     Layout l;
     size_t at = 0;
@@ -450,6 +454,7 @@ Layout layout_of(const scs_lowrank& p, bool backward) {
     const Few f = backward ? few_of(p, p.out_features, p.in_features) : few_of(p, p.in_features, p.out_features);
     size_t part = f.part;
     l.tickets = take((size_t)f.tickets * 4);
+    l.rows = take((size_t)p.rows * 4);
     if (backward) {
         l.hid2 = take((size_t)p.rows * p.rank * 4);
         for (const int64_t F : {p.in_features, p.out_features}) {
@@ -488,22 +493,26 @@ template <class F> void by_tiles(int rank, F&& f) {
     else f(std::integral_constant<int, 8>{});
 }
 
-template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st, unsigned int* tickets = nullptr, int n_tickets = 0) {
+template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st, int* row_adapter, unsigned int* tickets = nullptr, int n_tickets = 0) {
     const Requests r = requests_of(p);
     if (p.rows <= kDotRows) {
-        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r, tickets, n_tickets);
+        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r, row_adapter, tickets, n_tickets);
         return;
     }
     by_tiles(p.rank, [&](auto jt) {
-        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r, tickets, n_tickets);
+        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r, row_adapter, tickets, n_tickets);
     });
 }
 
-template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const Few& f, float* part, unsigned int* tickets, hipStream_t st) {
+template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
     const dim3 grid(f.tiles_n, f.tiles_m, f.splits);
-    if (f.mt == 1) hipLaunchKernelGGL((project_few_kernel<T, 1, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
-    else if (f.mt == 2) hipLaunchKernelGGL((project_few_kernel<T, 2, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
-    else hipLaunchKernelGGL((project_few_kernel<T, 4, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, f.splits, part, tickets);
+    auto go = [&](auto mt) { hipLaunchKernelGGL((project_few_kernel<T, mt.value, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, rows, f.splits, part, tickets); };
+    if (sizeof(T) == 4 || f.mt == 1) go(std::integral_constant<int, 1>{});
+    else if constexpr (sizeof(T) == 2) {
+        if (f.mt == 2) go(std::integral_constant<int, 2>{});
+        else if (f.mt == 3) go(std::integral_constant<int, 3>{});
+        else go(std::integral_constant<int, 4>{});
+    }
 }
 
 template <class T, bool TRANS> void project16(const ProjectArgs<T>& g, hipStream_t st) {
@@ -515,8 +524,8 @@ template <class T, bool TRANS> void project16(const ProjectArgs<T>& g, hipStream
     else hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, false>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
 }
 
-template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& f, float* part, unsigned int* tickets, hipStream_t st) {
-    if (f.mt) { project_few<T, TRANS>(g, f, part, tickets, st); return; }
+template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
+    if (f.mt) { project_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
     if constexpr (sizeof(T) == 2) { project16<T, TRANS>(g, st); return; }
     // the column tile with the least padding, the widest among equals
     int best = 8, waste = 1 << 30;
@@ -547,9 +556,10 @@ int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t l
     const Layout l = layout_of(p, false);
     float* h = hidden ? hidden : (float*)(ws + l.hid);
     const Few f = few_of(p, p.in_features, p.out_features);
-    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st, (unsigned int*)(ws + l.tickets), f.tickets);
+    int* rows = (int*)(ws + l.rows);
+    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)},
-                      f, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
+                      f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }
@@ -562,16 +572,17 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     float* part = (float*)(ws + l.part);
     const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
     const Few f = few_of(p, p.out_features, p.in_features);
-    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st, (unsigned int*)(ws + l.tickets), f.tickets);
+    int* rows = (int*)(ws + l.rows);
+    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     if (dx)
         project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
-                         f, part, (unsigned int*)(ws + l.tickets), st);
+                         f, rows, part, (unsigned int*)(ws + l.tickets), st);
     if (da) wgrad<T>(p, u, (const T*)x, ldx, (int)p.in_features, da, part, st);
     if (db) {
         const float* h = hidden;
         if (!h) {
             h = (float*)(ws + l.hid2);
-            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), st);
+            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), st, rows);
         }
         wgrad<T>(p, h, (const T*)dy, lddy, (int)p.out_features, db, part, st);
     }
