@@ -332,6 +332,7 @@ __global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
 }  // namespace
 }  // namespace scs
 #include "lowrank_mfma16.h"
+#include "lowrank_tiles.h"
 #include "lowrank_few.h"
 namespace scs {
 namespace {
@@ -518,8 +519,9 @@ template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const F
 template <class T, bool TRANS> void project16(const ProjectArgs<T>& g, hipStream_t st) {
     auto tiles = [&](int b) { return (int64_t)((g.r.rows + b - 1) / b) * ((g.N + b - 1) / b); };
     const bool aligned = g.K % 8 == 0 && g.N % 8 == 0 && g.ldx % 8 == 0 && g.ldw % 8 == 0 && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.w % 16 == 0;
-    if (tiles(256) >= 192 && aligned)
-        hipLaunchKernelGGL((project16_kernel<T, 2, 4, 8, 4, TRANS, true>), dim3((unsigned)tiles(256)), dim3(512), 0, st, g);
+    const bool piped = aligned && g.K % 64 == 0 && g.ldx <= (1 << 21) && g.ldw <= (1 << 21);
+    if (piped && tiles(256) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 4, 8, 4, TRANS>), dim3((unsigned)tiles(256)), dim3(512), 0, st, g);
+    else if (piped) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
     else if (aligned) hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, true>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
     else hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, false>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
 }
