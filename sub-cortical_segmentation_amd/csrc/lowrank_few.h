@@ -36,8 +36,6 @@ __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)
 
 constexpr int kFewWaves = 8;
 
-template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
-template <class T> __device__ __forceinline__ u32x4 at8(const T* p) { return reinterpret_cast<const Loose<u32x4>*>(p)->v; }
 // where four columns from n on can be read from any row but W's last one (from the last one as well where N % 4 == 0)
 __device__ __forceinline__ int few_column(int n, int N) { return min(n, N % 4 ? N - 1 : N - 4); }
 
@@ -54,10 +52,10 @@ template <class T, int MT, bool TRANS> struct FewStep16 {
         const int k = k0 + 8 * kq;
         if (inside) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) x[i] = at8(g.x + (int64_t)min(m0 + 16 * i + lr, g.r.rows - 1) * g.ldx + k);
+            for (int i = 0; i < MT; ++i) x[i] = at16(g.x + (int64_t)min(m0 + 16 * i + lr, g.r.rows - 1) * g.ldx + k);
             if constexpr (TRANS) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) wt[t] = at8(g.w + (int64_t)min(n + t, g.N - 1) * g.ldw + k);
+                for (int t = 0; t < 4; ++t) wt[t] = at16(g.w + (int64_t)min(n + t, g.N - 1) * g.ldw + k);
             } else {
                 const T* p = g.w + (int64_t)k * g.ldw + few_column(n, g.N);
 #pragma unroll

@@ -13,14 +13,6 @@
 namespace scs {
 namespace {
 
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-template <class T> struct Frag;
-template <> struct Frag<__bf16> { typedef __bf16 v8 __attribute__((ext_vector_type(8))); };
-template <> struct Frag<_Float16> { typedef _Float16 v8 __attribute__((ext_vector_type(8))); };
-__device__ __forceinline__ f32x4 mfma16(Frag<__bf16>::v8 a, Frag<__bf16>::v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mfma16(Frag<_Float16>::v8 a, Frag<_Float16>::v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
 __device__ const u32x4 kZeroPiece = {0, 0, 0, 0};            // what lies behind the end of the contraction
 
 // eight elements at any element alignment, zeros behind `left`

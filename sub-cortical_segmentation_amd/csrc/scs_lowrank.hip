@@ -53,65 +53,115 @@ __device__ __forceinline__ Span span_of(const Requests& r, int q, int m0, int m1
 }
 
 // ------------------------------------------------------------------------------------------------------------------ shrink
-// H[row][j] = sum_k X[row][k] P_s[j][k] (0 without an adapter).  Many rows: a workgroup owns 16 rows, its four waves a quarter of the
-// contraction each, joined through LDS; operands go from global memory to the f32 matrix cores without a stop (both are contiguous along the
-// contraction: a lane's 16 or 8 bytes are its operand of four MFMAs, whose contraction indices are permuted alike on both sides).
-template <class T, int JT>
-__global__ __launch_bounds__(256) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
-                                                          int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
-    __shared__ float s_part[4][JT * 4][64];
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * 256) tickets[i] = 0;
+// H[row][j] = sum_k X[row][k] P_s[j][k] (0 without an adapter).  Many rows: reading X once is the work.  A workgroup of eight waves owns 16 MT
+// rows, each wave an eighth of the contraction, joined through LDS; operands go from global memory to the matrix cores without a stop (both are
+// contiguous along the contraction: a lane's 16 bytes are its operand of one 16-bit product or of four f32 ones, whose contraction
+// indices are permuted alike on both sides), four steps' loads in flight.
+template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
+template <class T> __device__ __forceinline__ u32x4 at16(const T* p) { return reinterpret_cast<const Loose<u32x4>*>(p)->v; }
+// 16 bytes of elements at any element alignment, zeros behind `left`
+template <class T> __device__ __forceinline__ u32x4 load16(const T* p, int64_t left) {
+    constexpr int N = 16 / sizeof(T);
+    if (left >= N) return at16(p);
+    T e[N] = {};
+    for (int i = 0; i < N - 1; ++i) if (i < left) e[i] = p[i];
+    u32x4 r;
+    __builtin_memcpy(&r, e, 16);
+    return r;
+}
+template <class T> __device__ __forceinline__ f32x4 product16(const u32x4& a, const u32x4& b, f32x4 c) {
+    if constexpr (sizeof(T) == 4) {
+        f32x4 x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[i], y[i], c, 0, 0, 0);
+        return c;
+    } else {
+        typename Frag<T>::v8 x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+        return mfma16(x, y, c);
+    }
+}
+
+constexpr int kShrinkWaves = 8;
+template <class T, int JT, int MT>
+__global__ __launch_bounds__(64 * kShrinkWaves) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
+                                                                        int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
+    constexpr int STEP = 64 / sizeof(T), PER = 16 / sizeof(T), UNROLL = JT <= 2 ? 4 : 2;      // contraction values of a step, of a lane
+    __shared__ float s_part[kShrinkWaves][MT * JT * 4][64];
+    for (int i = blockIdx.x * 64 * kShrinkWaves + threadIdx.x; i < n_tickets; i += gridDim.x * 64 * kShrinkWaves) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, kq = lane >> 4;
-    const int m0 = blockIdx.x * 16, m1 = min(m0 + 16, r.rows);
-    const int slab = (K + 15) / 16, per = (slab + 3) / 4;
-    const int k_lo = wave * per * 16, k_hi = min(K, (wave + 1) * per * 16);
-    const int row = min(m0 + lr, r.rows - 1);
-    const T* xr = x + (int64_t)row * ldx;
+    const int m0 = blockIdx.x * 16 * MT, m1 = min(m0 + 16 * MT, r.rows);
+    const int steps = (K + STEP - 1) / STEP;
+    const int s_lo = steps * wave / kShrinkWaves, s_hi = steps * (wave + 1) / kShrinkWaves;
+    const T* xr[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(m0 + 16 * i + lr, r.rows - 1) * ldx + kq * PER;
     int mine = -2;
     for (int q = first_request(r, m0); q < r.n; ++q) {
         const Span sp = span_of(r, q, m0, m1);
         if (r.offsets[q] >= m1) break;
         if (sp.lo >= sp.hi) continue;
         if (m0 + (int)threadIdx.x >= sp.lo && m0 + (int)threadIdx.x < sp.hi) mine = sp.s;
-        f32x4 acc[JT];
+        f32x4 acc[MT][JT];
 #pragma unroll
-        for (int t = 0; t < JT; ++t) acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int t = 0; t < JT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
         if (sp.s >= 0) {
-            const T* ps = p + (int64_t)sp.s * r.rank * K;
-            for (int k0 = k_lo; k0 < k_hi; k0 += 16) {
-                const int k = k0 + 4 * kq, left = K - k;
-                typename Vec4<T>::raw ra, rb[JT];
-                raw_load<T>(ra, xr + k, left);
+            const T* pr[JT];
 #pragma unroll
-                for (int t = 0; t < JT; ++t) {
-                    const int j = min(t * 16 + lr, r.rank - 1);
-                    raw_load<T>(rb[t], ps + (int64_t)j * K + k, left);
+            for (int t = 0; t < JT; ++t) pr[t] = p + ((int64_t)sp.s * r.rank + min(t * 16 + lr, r.rank - 1)) * K + kq * PER;
+            int s = s_lo;
+            for (; s + UNROLL <= s_hi && (s + UNROLL) * STEP <= K; s += UNROLL) {
+                u32x4 a[UNROLL][MT], b[UNROLL][JT];
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) a[u][i] = at16(xr[i] + (s + u) * STEP);
+#pragma unroll
+                    for (int t = 0; t < JT; ++t) b[u][t] = at16(pr[t] + (s + u) * STEP);
                 }
-                float a[4];
-                unpack<T>(ra, a);
+#pragma unroll
+                for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int t = 0; t < JT; ++t) acc[i][t] = product16<T>(a[u][i], b[u][t], acc[i][t]);
+            }
+            for (; s < s_hi; ++s) {
+                const int left = K - s * STEP - kq * PER;
+                u32x4 a[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) a[i] = load16(xr[i] + s * STEP, left);
 #pragma unroll
                 for (int t = 0; t < JT; ++t) {
-                    float b[4];
-                    unpack<T>(rb[t], b);
+                    const u32x4 b = load16(pr[t] + s * STEP, left);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], acc[t], 0, 0, 0);
+                    for (int i = 0; i < MT; ++i) acc[i][t] = product16<T>(a[i], b, acc[i][t]);
                 }
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int t = 0; t < JT; ++t)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s_part[wave][t * 4 + i][lane] = acc[t][i];
+            for (int t = 0; t < JT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s_part[wave][(i * JT + t) * 4 + e][lane] = acc[i][t][e];
         __syncthreads();
-        for (int e = wave; e < JT * 4; e += 4) {
-            const float v = (s_part[0][e][lane] + s_part[1][e][lane]) + (s_part[2][e][lane] + s_part[3][e][lane]);
-            const int m = m0 + 4 * kq + (e & 3), j = (e >> 2) * 16 + lr;
+        for (int e = wave; e < MT * JT * 4; e += kShrinkWaves) {
+            float v = s_part[0][e][lane];
+#pragma unroll
+            for (int w = 1; w < kShrinkWaves; ++w) v += s_part[w][e][lane];
+            const int i = e / (4 * JT), t = (e >> 2) % JT, m = m0 + 16 * i + 4 * kq + (e & 3), j = t * 16 + lr;
             if (m >= sp.lo && m < sp.hi && j < r.rank) h[(int64_t)m * r.rank + j] = v;
         }
     }
-    if (threadIdx.x < 16 && m0 + (int)threadIdx.x < r.rows) row_adapter[m0 + threadIdx.x] = mine;
+    if (threadIdx.x < 16 * MT && m0 + (int)threadIdx.x < r.rows) row_adapter[m0 + threadIdx.x] = mine;
 }
 
 // Few rows: a workgroup owns four directions of one row, its four waves a quarter of the contraction each (every load of the quarter of a
@@ -338,51 +388,49 @@ namespace scs {
 namespace {
 
 // ------------------------------------------------------------------------------------------------------------------ wgrad
-// G_s[j][k] = scale_s sum over the rows of s of H[row][j] X[row][k], f32.  A workgroup owns 64 columns of one adapter and one slice of the
-// rows; a lane's vector of X is its operand of four MFMAs (columns 4 c + t of MFMA t), the four waves take every fourth group of four rows
-// and are joined through LDS in a fixed order.  Slices: [slice][adapter][rank][F] partial sums, added up by wgrad_join_kernel.
-template <class T, int JT>
-__global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ h, const T* __restrict__ x, int64_t ldx, int F, int slices,
-                                                    float* __restrict__ out, Requests r) {
-    __shared__ float s_part[3][JT * 16][64];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int lr = lane & 15, kq = lane >> 4;
-    const int c0 = blockIdx.x * 64, s = blockIdx.y, slice = blockIdx.z;
-    const int per = (int)(((int64_t)r.rows + slices - 1) / slices);
-    const int m0 = min((int64_t)slice * per, (int64_t)r.rows), m1 = min((int64_t)m0 + per, (int64_t)r.rows);
-    f32x4 acc[JT][4];
-#pragma unroll
-    for (int t = 0; t < JT; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const int col = c0 + 4 * lr, left = F - col;
+// G_s[j][k] = scale_s sum over the rows of s of H[row][j] X[row][k], f32: reading X once is the work.  A workgroup owns 64 columns; a lane's
+// vector of X (four columns of a row) is its operand of four f32 products (columns 4 c + t of product t), its four waves take every fourth
+// group of sixteen rows and are joined through LDS in a fixed order.  dA and dB are one launch.
+//   by blocks: a workgroup owns a block of rows as well and leaves one partial sum for each request in it, in slot request + block (along the
+//              rows one of the two grows from each partial sum to the next: no slot is met twice); wgrad_join_kernel adds an adapter's slots up
+//   direct:    a workgroup owns one adapter and walks its requests (few rows, or requests so many that their slots would outweigh X)
+template <class T> struct WgradProblem { const float* h; const T* x; int64_t ldx; float* out; float* part; int32_t F; };
+template <class T> struct WgradArgs { WgradProblem<T> p[2]; int32_t block_rows; Requests r; };
 
-    for (int q0 = first_request(r, m0); q0 < r.n; q0 += 64) {
-        // the requests of this adapter among 64
-        const int q = q0 + lane;
-        bool mine = false;
-        if (q < r.n) mine = r.adapters[q] == s && r.offsets[q] < m1 && r.offsets[q + 1] > m0;
-        unsigned long long todo = __ballot(mine);
-        while (todo) {
-            const Span sp = span_of(r, q0 + __builtin_ctzll(todo), m0, m1);
-            todo &= todo - 1;
-            for (int b = sp.lo + wave * 4; b < sp.hi; b += 16) {
-                const int row = b + kq;
-                const bool in = row < sp.hi;
-                typename Vec4<T>::raw rx;
-                raw_load<T>(rx, x + (int64_t)row * ldx + col, in ? left : 0);
-                float f[4];
-                unpack<T>(rx, f);
+// rows [lo, hi) of one request into the accumulators
+template <class T, int JT> __device__ __forceinline__ void wgrad_rows(const WgradProblem<T>& w, const Requests& r, int col, int lo, int hi, int wave, f32x4 (&acc)[JT][4]) {
+    constexpr int UNROLL = JT <= 2 ? 4 : 2;
+    const int lane = threadIdx.x & 63, lr = lane & 15, kq = lane >> 4, left = w.F - col;
+    for (int b = lo + wave * 4 * UNROLL; b < hi; b += 16 * UNROLL) {
+        typename Vec4<T>::raw rx[UNROLL];
+        float a[UNROLL][JT];
 #pragma unroll
-                for (int t = 0; t < JT; ++t) {
-                    const int j = t * 16 + lr;
-                    const float a = in && j < r.rank ? h[(int64_t)row * r.rank + j] : 0.f;
+        for (int u = 0; u < UNROLL; ++u) {
+            const int row = b + 4 * u + kq, at = min(row, hi - 1);
+            raw_load<T>(rx[u], w.x + (int64_t)at * w.ldx + col, left);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(a, f[i], acc[t][i], 0, 0, 0);
-                }
+            for (int t = 0; t < JT; ++t) a[u][t] = w.h[(int64_t)at * r.rank + min(t * 16 + lr, r.rank - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const bool in = b + 4 * u + kq < hi;                  // (a row of another request takes no part, whatever it holds)
+            float f[4];
+            unpack<T>(rx[u], f);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) f[i] = in ? f[i] : 0.f;
+#pragma unroll
+            for (int t = 0; t < JT; ++t) {
+                const float h = in && t * 16 + lr < r.rank ? a[u][t] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(h, f[i], acc[t][i], 0, 0, 0);
             }
         }
     }
+}
+// the four waves' sums, in their order, times sc, to out [rank][F]
+template <int JT> __device__ __forceinline__ void wgrad_store(float (&s_part)[3][JT * 16][64], const f32x4 (&acc)[JT][4], int wave, int rank, int F, int col, float sc, float* out) {
+    const int lane = threadIdx.x & 63, kq = lane >> 4, left = F - col;
+    __syncthreads();
     if (wave) {
 #pragma unroll
         for (int t = 0; t < JT; ++t)
@@ -393,8 +441,6 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ h,
     }
     __syncthreads();
     if (wave) return;
-    const float sc = r.scale ? r.scale[s] : 1.f;
-    float* o = out + ((int64_t)slice * r.n_adapters + s) * r.rank * F;
 #pragma unroll
     for (int t = 0; t < JT; ++t)
 #pragma unroll
@@ -406,16 +452,83 @@ __global__ __launch_bounds__(256) void wgrad_kernel(const float* __restrict__ h,
                 const int at = t * 16 + i * 4 + e;
                 v[i] = sc * (((acc[t][i][e] + s_part[0][at][lane]) + s_part[1][at][lane]) + s_part[2][at][lane]);
             }
-            if (j < r.rank) raw_store<float>(v, o + (int64_t)j * F + col, left);
+            if (j < rank) raw_store<float>(v, out + (int64_t)j * F + col, left);
         }
 }
+template <int JT> __device__ __forceinline__ void wgrad_clear(f32x4 (&acc)[JT][4]) {
+#pragma unroll
+    for (int t = 0; t < JT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
 
-__global__ __launch_bounds__(256) void wgrad_join_kernel(const float* __restrict__ part, int slices, int64_t n, float* __restrict__ out) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        float v = part[i];
-        for (int s = 1; s < slices; ++s) v += part[s * n + i];
-        out[i] = v;
+template <class T, int JT>
+__global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
+    __shared__ float s_part[3][JT * 16][64];
+    const WgradProblem<T>& w = g.p[blockIdx.z];
+    const Requests& r = g.r;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.x * 64, col = c0 + 4 * (threadIdx.x & 15);
+    if (c0 >= w.F) return;
+    const int m0 = blockIdx.y * g.block_rows, m1 = min(m0 + g.block_rows, r.rows);
+    for (int q = first_request(r, m0); q < r.n; ++q) {
+        if (r.offsets[q] >= m1) break;
+        const Span sp = span_of(r, q, m0, m1);
+        if (sp.lo >= sp.hi || sp.s < 0) continue;
+        f32x4 acc[JT][4];
+        wgrad_clear<JT>(acc);
+        wgrad_rows<T, JT>(w, r, col, sp.lo, sp.hi, wave, acc);
+        wgrad_store<JT>(s_part, acc, wave, r.rank, w.F, col, 1.f, w.part + (int64_t)(q + blockIdx.y) * r.rank * w.F);
     }
+}
+
+template <class T, int JT>
+__global__ __launch_bounds__(256) void wgrad_direct_kernel(WgradArgs<T> g) {
+    __shared__ float s_part[3][JT * 16][64];
+    const WgradProblem<T>& w = g.p[blockIdx.z];
+    const Requests& r = g.r;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.x * 64, col = c0 + 4 * (lane & 15), s = blockIdx.y;
+    if (c0 >= w.F) return;
+    f32x4 acc[JT][4];
+    wgrad_clear<JT>(acc);
+    for (int q0 = 0; q0 < r.n; q0 += 64) {
+        const int q = q0 + lane;
+        unsigned long long todo = __ballot(q < r.n && r.adapters[q] == s);
+        while (todo) {
+            const Span sp = span_of(r, q0 + __builtin_ctzll(todo), 0, r.rows);
+            todo &= todo - 1;
+            wgrad_rows<T, JT>(w, r, col, sp.lo, sp.hi, wave, acc);
+        }
+    }
+    wgrad_store<JT>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
+}
+
+// an adapter's gradient from its requests' slots, in the order of the rows
+template <class T>
+__global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs<T> g) {
+    const WgradProblem<T>& w = g.p[blockIdx.z];
+    const Requests& r = g.r;
+    const int s = blockIdx.y, lane = threadIdx.x & 63;
+    const int64_t n = (int64_t)r.rank * w.F, i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if ((int64_t)blockIdx.x * 1024 >= n) return;
+    const int left = (int)min(n - i, (int64_t)4);
+    f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int q0 = 0; q0 < r.n; q0 += 64) {
+        const int ql = q0 + lane;
+        unsigned long long todo = __ballot(ql < r.n && r.adapters[ql] == s);
+        while (todo) {
+            const int q = q0 + __builtin_ctzll(todo);
+            todo &= todo - 1;
+            const int lo = clamp_row(r.offsets[q], r.rows), hi = clamp_row(r.offsets[q + 1], r.rows);
+            if (lo >= hi || left <= 0) continue;
+#pragma unroll 4
+            for (int b = lo / g.block_rows; b <= (hi - 1) / g.block_rows; ++b) {
+                f32x4 v;
+                raw_load<float>(v, w.part + (int64_t)(q + b) * n + i, left);
+                sum += v;
+            }
+        }
+    }
+    if (left > 0) raw_store<float>(sum * (r.scale ? r.scale[s] : 1.f), w.out + (int64_t)s * n + i, left);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ host side
@@ -423,11 +536,14 @@ constexpr int kDotRows = 512;               // up to so many rows the shrink is 
 
 size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-int wgrad_slices(const scs_lowrank& p, int64_t F) {
-    // workgroups: 64 columns x adapters x slices; more slices until there are enough for the card, none under 256 rows
-    const int64_t tiles = (F + 63) / 64 * p.n_adapters;
-    const int64_t s = std::min<int64_t>(1024 / std::max<int64_t>(tiles, 1), p.rows / 256);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows; direct where that
+// is one block, or where the slots (requests + blocks, rank f32 values a column each) would outweigh X's own rows.
+int wgrad_block_rows(const scs_lowrank& p) {
+    const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
+    const int64_t rows = std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64));
+    const int64_t blocks = (p.rows + rows - 1) / rows;
+    if (blocks <= 1 || blocks > 65535 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
+    return (int)rows;
 }
 
 // ---- few rows (lowrank_few.h)
@@ -446,7 +562,7 @@ Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     }
     return f;
 }
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, bytes = 0; };
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward) {
     Layout l;
     size_t at = 0;
@@ -458,10 +574,7 @@ Layout layout_of(const scs_lowrank& p, bool backward) {
     l.rows = take((size_t)p.rows * 4);
     if (backward) {
         l.hid2 = take((size_t)p.rows * p.rank * 4);
-        for (const int64_t F : {p.in_features, p.out_features}) {
-            const int s = wgrad_slices(p, F);
-            if (s > 1) part = std::max(part, (size_t)s * p.n_adapters * p.rank * F * 4);
-        }
+        if (const int b = wgrad_block_rows(p)) l.slots = take((size_t)(p.n_requests + (p.rows + b - 1) / b) * p.rank * (p.in_features + p.out_features) * 4);
     }
     l.part = take(part);
     l.bytes = at;
@@ -501,7 +614,9 @@ template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, co
         return;
     }
     by_tiles(p.rank, [&](auto jt) {
-        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value>), dim3((unsigned)((p.rows + 15) / 16)), dim3(256), 0, st, x, ldx, low, K, h, r, row_adapter, tickets, n_tickets);
+        constexpr int MT = jt.value <= 4 ? 2 : 1;                // (the join's LDS)
+        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, MT>), dim3((unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(64 * kShrinkWaves), 0, st, x, ldx, low, K, h, r,
+                           row_adapter, tickets, n_tickets);
     });
 }
 
@@ -541,16 +656,18 @@ template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& 
     else hipLaunchKernelGGL((project_f32_kernel<T, 4, TRANS>), grid, dim3(256), 0, st, g);
 }
 
-template <class T> void wgrad(const scs_lowrank& p, const float* h, const T* x, int64_t ldx, int F, float* out, float* part, hipStream_t st) {
-    const Requests r = requests_of(p);
-    const int s = wgrad_slices(p, F);
-    by_tiles(p.rank, [&](auto jt) {
-        hipLaunchKernelGGL((wgrad_kernel<T, jt.value>), dim3((F + 63) / 64, p.n_adapters, s), dim3(256), 0, st, h, x, ldx, F, s, s > 1 ? part : out, r);
-    });
-    if (s > 1) {
-        const int64_t n = (int64_t)p.n_adapters * p.rank * F;
-        hipLaunchKernelGGL(wgrad_join_kernel, dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096)), dim3(256), 0, st, part, s, n, out);
+template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&problems)[2], int n, float* slots, hipStream_t st) {
+    WgradArgs<T> g{{problems[0], problems[1]}, wgrad_block_rows(p), requests_of(p)};
+    const int F = std::max(problems[0].F, n > 1 ? problems[1].F : 0), tiles = (F + 63) / 64;
+    if (!g.block_rows) {
+        by_tiles(p.rank, [&](auto jt) { hipLaunchKernelGGL((wgrad_direct_kernel<T, jt.value>), dim3(tiles, p.n_adapters, n), dim3(256), 0, st, g); });
+        return;
     }
+    const int64_t blocks = (p.rows + g.block_rows - 1) / g.block_rows;
+    g.p[0].part = slots;
+    g.p[1].part = slots + (p.n_requests + blocks) * p.rank * problems[0].F;
+    by_tiles(p.rank, [&](auto jt) { hipLaunchKernelGGL((wgrad_blocks_kernel<T, jt.value>), dim3(tiles, (unsigned)blocks, n), dim3(256), 0, st, g); });
+    hipLaunchKernelGGL(wgrad_join_kernel<T>, dim3((unsigned)(((int64_t)p.rank * F + 1023) / 1024), p.n_adapters, n), dim3(256), 0, st, g);
 }
 
 template <class T>
@@ -579,15 +696,18 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     if (dx)
         project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
                          f, rows, part, (unsigned int*)(ws + l.tickets), st);
-    if (da) wgrad<T>(p, u, (const T*)x, ldx, (int)p.in_features, da, part, st);
+    WgradProblem<T> w[2]{};
+    int n = 0;
+    if (da) w[n++] = WgradProblem<T>{u, (const T*)x, ldx, da, nullptr, (int)p.in_features};
     if (db) {
         const float* h = hidden;
         if (!h) {
             h = (float*)(ws + l.hid2);
             if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), st, rows);
         }
-        wgrad<T>(p, h, (const T*)dy, lddy, (int)p.out_features, db, part, st);
+        w[n++] = WgradProblem<T>{h, (const T*)dy, lddy, db, nullptr, (int)p.out_features};
     }
+    if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }

@@ -55,6 +55,15 @@ template <class T> __device__ __forceinline__ typename Vec4<T>::raw pack(const f
     return r;
 }
 
+// ---- operands of the 16-bit matrix cores
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+template <class T> struct Frag;
+template <> struct Frag<__bf16> { typedef __bf16 v8 __attribute__((ext_vector_type(8))); };
+template <> struct Frag<_Float16> { typedef _Float16 v8 __attribute__((ext_vector_type(8))); };
+__device__ __forceinline__ f32x4 mfma16(Frag<__bf16>::v8 a, Frag<__bf16>::v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma16(Frag<_Float16>::v8 a, Frag<_Float16>::v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
 int handle_device(scs_handle h);          // (scs_api.hip)
 
 // The handle's device is current inside a call and the caller's again behind it.
