@@ -147,29 +147,18 @@ __global__ __launch_bounds__(64 * WM * WN) void project16_kernel(ProjectArgs<T> 
     // the adapters: 32 directions a pass, scale_s H as two 16-bit pieces side by side along the contraction ([16 upper | 16 lower] twice, P's
     // rows repeated to match), each request under the mask of its rows
     const int m1 = min(m0 + BM, r.rows), mw = m0 + wm * MT * 16, mw1 = min(mw + MT * 16, r.rows);
-    for (int q = first_request(r, m0); q < r.n; ++q) {
-        if (r.offsets[q] >= m1) break;
-        const Span sp = span_of(r, q, m0, m1);
-        if (sp.lo >= sp.hi || sp.s < 0) continue;
+    Walk walk(r, m0, m1);
+    int q;
+    Span sp;
+    while (walk.next(q, sp)) {
+        if (sp.s < 0) continue;
         const T* ps = g.low + (int64_t)sp.s * r.rank * g.N;
         for (int j0 = 0; j0 < r.rank; j0 += 32) {
-            for (int e = tid; e < BM * 4; e += THREADS) {
-                const int m = e >> 2, jg = e & 3, row = m0 + m;
-                T hi[8], lo[8];
-                u32x4 vh, vl;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = j0 + jg * 8 + i;
-                    const float v = row >= sp.lo && row < sp.hi && j < r.rank ? sp.scale * g.h[(int64_t)row * r.rank + j] : 0.f;
-                    hi[i] = from_f32<T>(v);
-                    const float up = to_f32(hi[i]);
-                    lo[i] = from_f32<T>(fabsf(up) <= 3.4e38f ? v - up : 0.f);
-                }
-                const int c = (jg >> 1) * 4 + (jg & 1);
-                __builtin_memcpy(&vh, hi, 16);
-                __builtin_memcpy(&vl, lo, 16);
-                *(u32x4*)&s_a[0][m * BK + ((c ^ (m & 7)) * 8)] = vh;
-                *(u32x4*)&s_a[0][m * BK + (((c + 2) ^ (m & 7)) * 8)] = vl;
+            for (int e = tid; e < BM * 8; e += THREADS) {
+                const int m = e >> 3, c = e & 7, row = m0 + m, group = j0 / 16 + (c >> 2), groups = (r.rank + 15) / 16;
+                u32x4 v = u32x4{0, 0, 0, 0};
+                if (row >= sp.lo && row < sp.hi && group < groups) v = *((const u32x4*)(g.pieces + ((int64_t)row * groups + group) * 32) + (c & 3));
+                *(u32x4*)&s_a[0][m * BK + ((c ^ (m & 7)) * 8)] = v;
             }
             for (int e = tid; e < 32 * NP; e += THREADS) {
                 const int jj = e / NP, c = e % NP, k = (jj >> 4) * 32 + (jj & 15), j = j0 + jj;

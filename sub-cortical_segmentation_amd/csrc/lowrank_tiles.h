@@ -127,55 +127,6 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
         }
         __builtin_amdgcn_sched_group_barrier(0x008, MT * NT - EACH * READS, 0);
     };
-    // the adapters: 16 directions a pass, scale_s H as its upper and lower 16-bit piece side by side along the contraction, P's rows repeated
-    const int m1 = min(m0 + BM, r.rows), mw = m0 + wm * MT * 16, mw1 = min(mw + MT * 16, r.rows);
-    for (int q = first_request(r, m0); q < r.n; ++q) {
-        if (r.offsets[q] >= m1) break;
-        const Span sp = span_of(r, q, m0, m1);
-        if (sp.lo >= sp.hi || sp.s < 0) continue;
-        const T* ps = g.low + (int64_t)sp.s * r.rank * g.N;
-        for (int j0 = 0; j0 < r.rank; j0 += 16) {
-            for (int e = tid; e < BM * 2; e += THREADS) {
-                const int m = e >> 1, jg = e & 1, row = m0 + m;
-                T hi[8], lo[8];
-                u32x4 vh, vl;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = j0 + jg * 8 + i;
-                    const float v = row >= sp.lo && row < sp.hi && j < r.rank ? sp.scale * g.h[(int64_t)row * r.rank + j] : 0.f;
-                    hi[i] = from_f32<T>(v);
-                    const float up = to_f32(hi[i]);
-                    lo[i] = from_f32<T>(fabsf(up) <= 3.4e38f ? v - up : 0.f);
-                }
-                __builtin_memcpy(&vh, hi, 16);
-                __builtin_memcpy(&vl, lo, 16);
-                *(u32x4*)&s_a[0][m * BK + ((jg ^ ((m >> 2) & 3)) * 8)] = vh;
-                *(u32x4*)&s_a[0][m * BK + (((jg + 2) ^ ((m >> 2) & 3)) * 8)] = vl;
-            }
-            for (int e = tid; e < 16 * NP; e += THREADS) {
-                const int k = e / NP, c = e % NP, j = j0 + k;
-                const u32x4 v = load8(ps + (int64_t)j * g.N + n0 + c * 8, j < r.rank ? g.N - (n0 + c * 8) : 0);
-                const int f = (k & 3) | ((k >> 3) & 1) << 2, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
-                *(u32x4*)&s_b[0][k * BN + at] = v;
-                *(u32x4*)&s_b[0][(k + 16) * BN + at] = v;
-            }
-            __syncthreads();
-            if (sp.lo < mw1 && sp.hi > mw) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const v8 w = frag_n(0, wn * NT + j);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        const f32x4 part = mfma16(w, frag_x(0, i), f32x4{0.f, 0.f, 0.f, 0.f});
-                        const int row = mw + i * 16 + lr;
-                        if (row >= sp.lo && row < sp.hi) acc[i][j] += part;
-                    }
-                }
-            }
-            __syncthreads();
-        }
-    }
-
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) fetch(s);
     copies_but<(STAGES - 1) * LOADS>();
@@ -195,22 +146,84 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
         multiply(x1, w1);
         spread();
     }
-    copies_but<0>();                                                     // (none may land in LDS that is another workgroup's by then)
+    copies_but<0>();                                                     // (none may land in LDS that holds something else by then)
+    workgroup_barrier();
+
+    // the adapters: 16 directions a pass, scale_s H as its upper and lower 16-bit piece side by side along the contraction, P's rows repeated
+    const int m1 = min(m0 + BM, r.rows), mw = m0 + wm * MT * 16;
+    auto frag_x_at = [&](int lr, int kq, int tile) { return *(const v8*)&s_a[0][(tile * 16 + lr) * BK + ((kq ^ (lr >> 2)) * 8)]; };
+    auto frag_n_at = [&](int lr, int kq, int tile) {
+        const T* at = &s_b[0][(8 * kq + (lr >> 2)) * BN + ((tile ^ ((lr >> 2) | (kq & 1) << 2)) << 4) + (lr & 3) * 4];
+        const s16x4 lo = lds_transposed(at), hi = lds_transposed(at + 4 * BN);
+        v8 v;
+        __builtin_memcpy(&v, &lo, 8);
+        __builtin_memcpy((char*)&v + 8, &hi, 8);
+        return v;
+    };
+    Walk walk(r, m0, m1);
+    int q;
+    Span sp;
+    while (walk.next(q, sp)) {
+        const T* ps = g.low + (int64_t)max(sp.s, 0) * r.rank * g.N;
+#pragma unroll 1
+        for (int j0 = sp.s < 0 ? r.rank : 0; j0 < r.rank; j0 += 16) {
+            // (opaque copies: addresses formed from them are formed here, not kept in registers beside the sums from the kernel's start on)
+            int tid = threadIdx.x, lr = tid & 15, kq = (tid >> 4) & 3;
+            asm volatile("" : "+v"(tid), "+v"(lr), "+v"(kq));
+            for (int e = tid; e < BM * 4; e += THREADS) {
+                const int m = e >> 2, c = e & 3, row = m0 + m;
+                const u32x4* at = (const u32x4*)(g.pieces + ((int64_t)min(row, r.rows - 1) * ((r.rank + 15) / 16) + j0 / 16) * 32) + c;
+                const u32x4 v = *at;
+                const bool in = row >= sp.lo && row < sp.hi;
+                *(u32x4*)&s_a[0][m * BK + ((c ^ ((m >> 2) & 3)) * 8)] = in ? v : u32x4{0, 0, 0, 0};
+            }
+            for (int e = tid; e < 16 * NP; e += THREADS) {
+                const int k = e / NP, c = e % NP, j = j0 + k;
+                const u32x4 v = at16(ps + (int64_t)min(j, r.rank - 1) * g.N + min(n0 + c * 8, g.N - 8));
+                const u32x4 w = j < r.rank ? v : u32x4{0, 0, 0, 0};
+                const int f = (k & 3) | ((k >> 3) & 1) << 2, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
+                *(u32x4*)&s_b[0][k * BN + at] = w;
+                *(u32x4*)&s_b[0][(k + 16) * BN + at] = w;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const v8 w = frag_n_at(lr, kq, wn * NT + j);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    const f32x4 part = mfma16(w, frag_x_at(lr, kq, wm * MT + i), f32x4{0.f, 0.f, 0.f, 0.f});
+                    const int row = mw + i * 16 + lr;
+                    const bool in = row >= sp.lo && row < sp.hi;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] += in ? part[e] : 0.f;
+                }
+                __builtin_amdgcn_sched_barrier(0);                      // (all columns' partial products at once do not fit beside the sums)
+            }
+            __syncthreads();
+        }
+    }
 
     const int live_lo = clamp_row(r.offsets[0], r.rows), live_hi = clamp_row(r.offsets[r.n], r.rows);
+    int el = threadIdx.x & 63;
+    asm volatile("" : "+v"(el));
+    const int col = n0 + wn * NT * 16 + 4 * (el >> 4);                    // (N is a multiple of 8: four columns or none)
+    float bias[NT][4] = {};
+    if (g.bias) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-        const int col = n0 + (wn * NT + j) * 16 + 4 * kq;                // (N is a multiple of 8: four columns or none)
-        if (col >= g.N) continue;
-        float bias[4] = {};
-        if (g.bias) unpack<T>(reinterpret_cast<const Loose<u32x2>*>(g.bias + col)->v, bias);
+        for (int j = 0; j < NT; ++j) unpack<T>(at4(g.bias + min(col + j * 16, g.N - 4)), bias[j]);
+    }
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            const int row = mw + i * 16 + lr;
-            if (row < live_lo || row >= live_hi) continue;
-            const float v[4] = {acc[i][j][0] + bias[0], acc[i][j][1] + bias[1], acc[i][j][2] + bias[2], acc[i][j][3] + bias[3]};
-            reinterpret_cast<Loose<u32x2>*>(g.y + (int64_t)row * g.ldy + col)->v = pack<T>(v);
+    for (int i = 0; i < MT; ++i) {
+        const int row = mw + i * 16 + (el & 15);
+        if (row >= live_lo && row < live_hi) {
+            T* y = g.y + (int64_t)row * g.ldy + col;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const float v[4] = {acc[i][j][0] + bias[j][0], acc[i][j][1] + bias[j][1], acc[i][j][2] + bias[j][2], acc[i][j][3] + bias[j][3]};
+                if (col + j * 16 < g.N) reinterpret_cast<Loose<u32x2>*>(y + j * 16)->v = pack<T>(v);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 

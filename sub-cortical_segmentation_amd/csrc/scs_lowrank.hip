@@ -28,33 +28,55 @@ struct Requests {
 
 __device__ __forceinline__ int clamp_row(int o, int rows) { return o < 0 ? 0 : o > rows ? rows : o; }
 
-// smallest q with offsets[q + 1] > row (n if there is none): binary search down to one wave's width, then one load a lane
-__device__ __forceinline__ int first_request(const Requests& r, int row) {
-    int lo = 0, hi = r.n;
-    while (hi - lo > 64) {
-        const int mid = (lo + hi) >> 1;
-        if (r.offsets[mid + 1] <= row) lo = mid + 1; else hi = mid;
-    }
-    const int q = lo + (int)(threadIdx.x & 63);
-    const unsigned long long below = __ballot(q < hi && r.offsets[q + 1] <= row);
-    const int add = ~below == 0ull ? 64 : __builtin_ctzll(~below);
-    return min(lo + add, hi);
-}
+struct Span { int lo, hi, s; };           // rows of a request inside [m0, m1) and its adapter (-1: none)
 
-struct Span { int lo, hi, s; float scale; };           // rows of request q inside [m0, m1) and its adapter (-1: none)
-__device__ __forceinline__ Span span_of(const Requests& r, int q, int m0, int m1) {
-    Span p;
-    p.lo = max(m0, clamp_row(r.offsets[q], r.rows));
-    p.hi = min(m1, clamp_row(r.offsets[q + 1], r.rows));
-    const int s = r.adapters[q];
-    p.s = (unsigned)s < (unsigned)r.n_adapters ? s : -1;
-    p.scale = p.s >= 0 && r.scale ? r.scale[p.s] : 1.f;
-    return p;
-}
+// The requests that own rows of [m0, m1), one after the other.  A wave holds 64 requests in its lanes - three loads at once, whatever
+// comes of them - and deals them out by lane reads; where there are more, a binary search finds the first window.  Whole waves call.
+struct Walk {
+    const Requests& r;
+    int m0, m1, base, at;
+    int lo, hi, ad;                                    // of request base + lane
+    __device__ __forceinline__ Walk(const Requests& req, int from, int to) : r(req), m0(from), m1(to), base(0), at(0) {
+        int end = r.n;
+        while (end - base > 64) {
+            const int mid = (base + end) >> 1;
+            if (r.offsets[mid + 1] <= m0) base = mid + 1; else end = mid;
+        }
+        window();
+    }
+    __device__ __forceinline__ void window() {
+        const int q = base + (int)(threadIdx.x & 63), c = max(min(q, r.n - 1), 0);
+        lo = r.offsets[c];
+        hi = q < r.n ? r.offsets[c + 1] : 0x7fffffff;
+        ad = r.n ? r.adapters[c] : -1;
+        at = -1;
+    }
+    // the next request with rows inside (its number in q), false behind the last one
+    __device__ __forceinline__ bool next(int& q, Span& p) {
+        for (;;) {
+            if (at < 0) {                              // skip what ends before m0
+                const unsigned long long below = __ballot(hi <= m0);
+                at = ~below == 0ull ? 64 : __builtin_ctzll(~below);
+            }
+            if (base + at >= r.n) return false;
+            if (at >= 64) { base += 64; window(); continue; }
+            q = base + at;
+            const int a = __builtin_amdgcn_readlane(lo, at), b = __builtin_amdgcn_readlane(hi, at), s = __builtin_amdgcn_readlane(ad, at);
+            ++at;
+            if (a >= m1) return false;
+            p.lo = max(m0, clamp_row(a, r.rows));
+            p.hi = min(m1, clamp_row(b, r.rows));
+            if (p.lo >= p.hi) continue;
+            p.s = (unsigned)s < (unsigned)r.n_adapters ? s : -1;
+            return true;
+        }
+    }
+    __device__ __forceinline__ float scale(const Span& p) const { return p.s >= 0 && r.scale ? r.scale[p.s] : 1.f; }
+};
 
 // ------------------------------------------------------------------------------------------------------------------ shrink
-// H[row][j] = sum_k X[row][k] P_s[j][k] (0 without an adapter).  Many rows: reading X once is the work.  A workgroup of eight waves owns 16 MT
-// rows, each wave an eighth of the contraction, joined through LDS; operands go from global memory to the matrix cores without a stop (both are
+// H[row][j] = sum_k X[row][k] P_s[j][k] (0 without an adapter).  Many rows: reading X once is the work.  A workgroup of W waves owns 16 MT
+// rows, each wave a share of the contraction, joined through LDS; operands go from global memory to the matrix cores without a stop (both are
 // contiguous along the contraction: a lane's 16 bytes are its operand of one 16-bit product or of four f32 ones, whose contraction
 // indices are permuted alike on both sides), four steps' loads in flight.
 template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
@@ -85,27 +107,48 @@ template <class T> __device__ __forceinline__ f32x4 product16(const u32x4& a, co
     }
 }
 
-constexpr int kShrinkWaves = 8;
-template <class T, int JT, int MT>
-__global__ __launch_bounds__(64 * kShrinkWaves) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
-                                                                        int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
-    constexpr int STEP = 64 / sizeof(T), PER = 16 / sizeof(T), UNROLL = JT <= 2 ? 4 : 2;      // contraction values of a step, of a lane
-    __shared__ float s_part[kShrinkWaves][MT * JT * 4][64];
-    for (int i = blockIdx.x * 64 * kShrinkWaves + threadIdx.x; i < n_tickets; i += gridDim.x * 64 * kShrinkWaves) tickets[i] = 0;
+// a value as the nearest 16-bit one and what is left of it (bf16: 2^-17 of the value is lost, f16: 2^-23 down to its smallest steps).  Beyond f16's
+// range the upper piece is infinite, as the value is in f16
+template <class T> __device__ __forceinline__ void write_pieces(T* pieces, int64_t row, int j, int rank, float v) {
+    if constexpr (sizeof(T) == 2) {
+        T* at = pieces + (row * ((rank + 15) / 16) + j / 16) * 32 + j % 16;
+        const T hi = from_f32<T>(v);
+        const float up = to_f32(hi);
+        at[0] = hi;
+        at[16] = from_f32<T>(fabsf(up) <= 3.4e38f ? v - up : 0.f);
+    }
+}
+
+template <class T, int JT, int MT, int W>
+__global__ __launch_bounds__(64 * W) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, T* __restrict__ pieces, Requests r,
+                                                             int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
+    constexpr int STEP = 64 / sizeof(T), PER = 16 / sizeof(T), UNROLL = JT <= 2 ? 4 : 2, UNIT = UNROLL * STEP;      // contraction values
+    __shared__ float s_part[W][MT * JT * 4][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, kq = lane >> 4;
     const int m0 = blockIdx.x * 16 * MT, m1 = min(m0 + 16 * MT, r.rows);
-    const int steps = (K + STEP - 1) / STEP;
-    const int s_lo = steps * wave / kShrinkWaves, s_hi = steps * (wave + 1) / kShrinkWaves;
+    // the contraction in units of 256 bytes of a row, dealt to the waves in turn and from another start in each workgroup: rows lie at the
+    // same L2 channel where their stride is a multiple of 4 KB, and neighbouring units at neighbouring channels
+    const int units = (K + UNIT - 1) / UNIT;
+    auto start = [&](int v) { return (int)((v + blockIdx.x) % (unsigned)units) * UNIT; };
+    Walk walk(r, m0, m1);
     const T* xr[MT];
+    u32x4 first[UNROLL][MT];                            // X of this wave's first unit, on its way while the requests are looked up
+    const int k_first = start(wave);
 #pragma unroll
     for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(m0 + 16 * i + lr, r.rows - 1) * ldx + kq * PER;
-    int mine = -2;
-    for (int q = first_request(r, m0); q < r.n; ++q) {
-        const Span sp = span_of(r, q, m0, m1);
-        if (r.offsets[q] >= m1) break;
-        if (sp.lo >= sp.hi) continue;
+    if (wave < units && k_first + UNIT <= K) {
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < MT; ++i) first[u][i] = at16(xr[i] + k_first + u * STEP);
+    }
+    for (int i = blockIdx.x * 64 * W + threadIdx.x; i < n_tickets; i += gridDim.x * 64 * W) tickets[i] = 0;
+    int mine = -2, q;
+    Span sp;
+    while (walk.next(q, sp)) {
         if (m0 + (int)threadIdx.x >= sp.lo && m0 + (int)threadIdx.x < sp.hi) mine = sp.s;
+        const float scale = walk.scale(sp);
         f32x4 acc[MT][JT];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -115,33 +158,36 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_rows_kernel(const T*
             const T* pr[JT];
 #pragma unroll
             for (int t = 0; t < JT; ++t) pr[t] = p + ((int64_t)sp.s * r.rank + min(t * 16 + lr, r.rank - 1)) * K + kq * PER;
-            int s = s_lo;
-            for (; s + UNROLL <= s_hi && (s + UNROLL) * STEP <= K; s += UNROLL) {
-                u32x4 a[UNROLL][MT], b[UNROLL][JT];
+            for (int v = wave; v < units; v += W) {
+                const int k0 = start(v);
+                if (k0 + UNIT <= K) {
+                    u32x4 a[UNROLL][MT], b[UNROLL][JT];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u) {
+                    for (int u = 0; u < UNROLL; ++u) {
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) a[u][i] = at16(xr[i] + (s + u) * STEP);
+                        for (int t = 0; t < JT; ++t) b[u][t] = at16(pr[t] + k0 + u * STEP);
 #pragma unroll
-                    for (int t = 0; t < JT; ++t) b[u][t] = at16(pr[t] + (s + u) * STEP);
+                        for (int i = 0; i < MT; ++i) a[u][i] = v == wave ? first[u][i] : at16(xr[i] + k0 + u * STEP);
+                    }
+#pragma unroll
+                    for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+#pragma unroll
+                            for (int t = 0; t < JT; ++t) acc[i][t] = product16<T>(a[u][i], b[u][t], acc[i][t]);
+                    continue;
                 }
+                for (int k = k0; k < K; k += STEP) {
+                    const int left = K - k - kq * PER;
+                    u32x4 a[MT];
 #pragma unroll
-                for (int u = 0; u < UNROLL; ++u)
+                    for (int i = 0; i < MT; ++i) a[i] = load16(xr[i] + k, left);
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
+                    for (int t = 0; t < JT; ++t) {
+                        const u32x4 b = load16(pr[t] + k, left);
 #pragma unroll
-                        for (int t = 0; t < JT; ++t) acc[i][t] = product16<T>(a[u][i], b[u][t], acc[i][t]);
-            }
-            for (; s < s_hi; ++s) {
-                const int left = K - s * STEP - kq * PER;
-                u32x4 a[MT];
-#pragma unroll
-                for (int i = 0; i < MT; ++i) a[i] = load16(xr[i] + s * STEP, left);
-#pragma unroll
-                for (int t = 0; t < JT; ++t) {
-                    const u32x4 b = load16(pr[t] + s * STEP, left);
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) acc[i][t] = product16<T>(a[i], b, acc[i][t]);
+                        for (int i = 0; i < MT; ++i) acc[i][t] = product16<T>(a[i], b, acc[i][t]);
+                    }
                 }
             }
         }
@@ -153,12 +199,14 @@ __global__ __launch_bounds__(64 * kShrinkWaves) void shrink_rows_kernel(const T*
 #pragma unroll
                 for (int e = 0; e < 4; ++e) s_part[wave][(i * JT + t) * 4 + e][lane] = acc[i][t][e];
         __syncthreads();
-        for (int e = wave; e < MT * JT * 4; e += kShrinkWaves) {
+        for (int e = wave; e < MT * JT * 4; e += W) {
             float v = s_part[0][e][lane];
 #pragma unroll
-            for (int w = 1; w < kShrinkWaves; ++w) v += s_part[w][e][lane];
+            for (int w = 1; w < W; ++w) v += s_part[w][e][lane];
             const int i = e / (4 * JT), t = (e >> 2) % JT, m = m0 + 16 * i + 4 * kq + (e & 3), j = t * 16 + lr;
-            if (m >= sp.lo && m < sp.hi && j < r.rank) h[(int64_t)m * r.rank + j] = v;
+            if (m < sp.lo || m >= sp.hi) continue;
+            if (j < r.rank) h[(int64_t)m * r.rank + j] = v;
+            if (pieces && t < (r.rank + 15) / 16) write_pieces<T>(pieces, m, j, r.rank, j < r.rank ? scale * v : 0.f);
         }
     }
     if (threadIdx.x < 16 * MT && m0 + (int)threadIdx.x < r.rows) row_adapter[m0 + threadIdx.x] = mine;
@@ -178,17 +226,18 @@ template <class T> __device__ __forceinline__ void load8f(const T* p, int left, 
     for (int i = 0; i < 4; ++i) { f[i] = lo[i]; f[4 + i] = hi[i]; }
 }
 template <class T>
-__global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, Requests r,
+__global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, T* __restrict__ pieces, Requests r,
                                                           int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
     __shared__ float s_part[4][4];
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * gridDim.y * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x, j0 = blockIdx.y * 4;
-    const int q = first_request(r, row);
-    Span sp{0, 0, -1, 1.f};
-    if (q < r.n) sp = span_of(r, q, row, row + 1);
-    if (threadIdx.x == 0 && blockIdx.y == 0) row_adapter[row] = sp.lo < sp.hi ? sp.s : -2;
-    if (sp.lo >= sp.hi) return;
+    Walk walk(r, row, row + 1);
+    int q;
+    Span sp;
+    const bool owned = walk.next(q, sp);
+    if (threadIdx.x == 0 && blockIdx.y == 0) row_adapter[row] = owned ? sp.s : -2;
+    if (!owned) return;
     float sum[4] = {};
     if (sp.s >= 0) {
         const T* xr = x + (int64_t)row * ldx;
@@ -215,8 +264,12 @@ __global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ 
         for (int j = 0; j < 4; ++j) s_part[wave][j] = sum[j];
     __syncthreads();
     const int j = j0 + (int)threadIdx.x;
-    if (threadIdx.x < 4 && j < r.rank)
-        h[(int64_t)row * r.rank + j] = (s_part[0][threadIdx.x] + s_part[1][threadIdx.x]) + (s_part[2][threadIdx.x] + s_part[3][threadIdx.x]);
+    const int all = (r.rank + 15) / 16 * 16, last = blockIdx.y == gridDim.y - 1 ? all - j0 : 4;       // (the last one fills its 16 pieces up with zeros)
+    if ((int)threadIdx.x < last) {
+        const float v = j < r.rank ? (s_part[0][threadIdx.x & 3] + s_part[1][threadIdx.x & 3]) + (s_part[2][threadIdx.x & 3] + s_part[3][threadIdx.x & 3]) : 0.f;
+        if (j < r.rank) h[(int64_t)row * r.rank + j] = v;
+        if (pieces) write_pieces<T>(pieces, row, j, r.rank, walk.scale(sp) * v);
+    }
 }
 
 // ------------------------------------------------------------------------------------------------------------------ project, f32 matrix cores
@@ -229,6 +282,7 @@ struct ProjectArgs {
     const T* bias;
     const T* low;                     // P: [n_adapters][rank][N]
     const float* h;                   // [rows][rank]
+    const T* pieces;                  // 16-bit types, many rows: scale_s h as two 16-bit pieces, [rows][ceil(rank / 16)][16 upper | 16 lower]
     T* y; int64_t ldy;
     int32_t K, N;
     Requests r;
@@ -325,16 +379,18 @@ __global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
 
     // the adapters' products, request by request, each under the mask of its rows
     const int m1 = min(m0 + kPBM, r.rows);
-    for (int q = first_request(r, m0); q < r.n; ++q) {
-        const Span sp = span_of(r, q, m0, m1);
-        if (r.offsets[q] >= m1) break;
-        if (sp.lo >= sp.hi || sp.s < 0) continue;
+    Walk walk(r, m0, m1);
+    int q;
+    Span sp;
+    while (walk.next(q, sp)) {
+        if (sp.s < 0) continue;
+        const float scale = walk.scale(sp);
         const T* ps = g.low + (int64_t)sp.s * r.rank * g.N;
         for (int j0 = 0; j0 < r.rank; j0 += kPBK) {
             for (int e = tid; e < kPBM * kPBK; e += 256) {
                 const int m = e / kPBK, j = e % kPBK, row = m0 + m;
                 const bool in = row >= sp.lo && row < sp.hi && j0 + j < r.rank;
-                s_a[0][m * kPAS + j] = in ? sp.scale * g.h[(int64_t)row * r.rank + j0 + j] : 0.f;
+                s_a[0][m * kPAS + j] = in ? scale * g.h[(int64_t)row * r.rank + j0 + j] : 0.f;
             }
             for (int e = tid; e < kPBK * BN; e += 256) {
                 const int j = e / BN, c = e % BN;
@@ -470,10 +526,11 @@ __global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.x * 64, col = c0 + 4 * (threadIdx.x & 15);
     if (c0 >= w.F) return;
     const int m0 = blockIdx.y * g.block_rows, m1 = min(m0 + g.block_rows, r.rows);
-    for (int q = first_request(r, m0); q < r.n; ++q) {
-        if (r.offsets[q] >= m1) break;
-        const Span sp = span_of(r, q, m0, m1);
-        if (sp.lo >= sp.hi || sp.s < 0) continue;
+    Walk walk(r, m0, m1);
+    int q;
+    Span sp;
+    while (walk.next(q, sp)) {
+        if (sp.s < 0) continue;
         f32x4 acc[JT][4];
         wgrad_clear<JT>(acc);
         wgrad_rows<T, JT>(w, r, col, sp.lo, sp.hi, wave, acc);
@@ -491,12 +548,12 @@ __global__ __launch_bounds__(256) void wgrad_direct_kernel(WgradArgs<T> g) {
     f32x4 acc[JT][4];
     wgrad_clear<JT>(acc);
     for (int q0 = 0; q0 < r.n; q0 += 64) {
-        const int q = q0 + lane;
-        unsigned long long todo = __ballot(q < r.n && r.adapters[q] == s);
-        while (todo) {
-            const Span sp = span_of(r, q0 + __builtin_ctzll(todo), 0, r.rows);
-            todo &= todo - 1;
-            wgrad_rows<T, JT>(w, r, col, sp.lo, sp.hi, wave, acc);
+        const int q = q0 + lane, c = min(q, r.n - 1);
+        const int lo = clamp_row(r.offsets[c], r.rows), hi = clamp_row(r.offsets[c + 1], r.rows);
+        unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
+        for (; todo; todo &= todo - 1) {
+            const int at = __builtin_ctzll(todo);
+            wgrad_rows<T, JT>(w, r, col, __builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(hi, at), wave, acc);
         }
     }
     wgrad_store<JT>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
@@ -513,17 +570,16 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs<T> g) {
     const int left = (int)min(n - i, (int64_t)4);
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int q0 = 0; q0 < r.n; q0 += 64) {
-        const int ql = q0 + lane;
-        unsigned long long todo = __ballot(ql < r.n && r.adapters[ql] == s);
-        while (todo) {
-            const int q = q0 + __builtin_ctzll(todo);
-            todo &= todo - 1;
-            const int lo = clamp_row(r.offsets[q], r.rows), hi = clamp_row(r.offsets[q + 1], r.rows);
-            if (lo >= hi || left <= 0) continue;
+        const int q = q0 + lane, c = min(q, r.n - 1);
+        const int lo = clamp_row(r.offsets[c], r.rows), hi = clamp_row(r.offsets[c + 1], r.rows);
+        unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
+        for (; todo; todo &= todo - 1) {
+            const int at = __builtin_ctzll(todo);
+            const int b_lo = __builtin_amdgcn_readlane(lo, at) / g.block_rows, b_hi = (__builtin_amdgcn_readlane(hi, at) - 1) / g.block_rows;
 #pragma unroll 4
-            for (int b = lo / g.block_rows; b <= (hi - 1) / g.block_rows; ++b) {
+            for (int b = b_lo; b <= b_hi; ++b) {
                 f32x4 v;
-                raw_load<float>(v, w.part + (int64_t)(q + b) * n + i, left);
+                raw_load<float>(v, w.part + (int64_t)(q0 + at + b) * n + i, left);
                 sum += v;
             }
         }
@@ -562,7 +618,7 @@ Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     }
     return f;
 }
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, bytes = 0; };
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, pieces = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward) {
     Layout l;
     size_t at = 0;
@@ -572,6 +628,7 @@ Layout layout_of(const scs_lowrank& p, bool backward) {
     size_t part = f.part;
     l.tickets = take((size_t)f.tickets * 4);
     l.rows = take((size_t)p.rows * 4);
+    if (p.dtype != SCS_F32 && !f.mt) l.pieces = take((size_t)p.rows * ((p.rank + 15) / 16) * 64);
     if (backward) {
         l.hid2 = take((size_t)p.rows * p.rank * 4);
         if (const int b = wgrad_block_rows(p)) l.slots = take((size_t)(p.n_requests + (p.rows + b - 1) / b) * p.rank * (p.in_features + p.out_features) * 4);
@@ -607,16 +664,28 @@ template <class F> void by_tiles(int rank, F&& f) {
     else f(std::integral_constant<int, 8>{});
 }
 
-template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, hipStream_t st, int* row_adapter, unsigned int* tickets = nullptr, int n_tickets = 0) {
+template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, T* pieces, hipStream_t st, int* row_adapter, unsigned int* tickets = nullptr, int n_tickets = 0) {
     const Requests r = requests_of(p);
     if (p.rows <= kDotRows) {
-        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, r, row_adapter, tickets, n_tickets);
+        hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets);
         return;
     }
     by_tiles(p.rank, [&](auto jt) {
-        constexpr int MT = jt.value <= 4 ? 2 : 1;                // (the join's LDS)
-        hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, MT>), dim3((unsigned)((p.rows + 16 * MT - 1) / (16 * MT))), dim3(64 * kShrinkWaves), 0, st, x, ldx, low, K, h, r,
-                           row_adapter, tickets, n_tickets);
+        // about two units a wave; two row tiles a wave (P read half as often) where workgroups abound
+        constexpr int UNIT = (jt.value <= 2 ? 4 : 2) * 64 / (int)sizeof(T);
+        const int units = (K + UNIT - 1) / UNIT;
+        auto go = [&](auto mt, auto w) {
+            hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, mt.value, w.value>), dim3((unsigned)((p.rows + 16 * mt.value - 1) / (16 * mt.value))), dim3(64 * w.value), 0, st,
+                               x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets);
+        };
+        constexpr int MT = jt.value <= 2 ? 2 : 1, MOST = jt.value <= 2 ? 16 : 8;             // (registers)
+        typedef std::integral_constant<int, 1> One;
+        if (p.rows >= 16384) {
+            if (units >= 16) go(std::integral_constant<int, MT>{}, std::integral_constant<int, 8>{});
+            else go(std::integral_constant<int, MT>{}, std::integral_constant<int, 4>{});
+        } else if (units >= 32) go(One{}, std::integral_constant<int, MOST>{});
+        else if (units >= 16) go(One{}, std::integral_constant<int, 8>{});
+        else go(One{}, std::integral_constant<int, 4>{});
     });
 }
 
@@ -676,8 +745,9 @@ int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t l
     float* h = hidden ? hidden : (float*)(ws + l.hid);
     const Few f = few_of(p, p.in_features, p.out_features);
     int* rows = (int*)(ws + l.rows);
-    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
-    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)},
+    T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
+    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
+    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)},
                       f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
@@ -692,9 +762,10 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
     const Few f = few_of(p, p.out_features, p.in_features);
     int* rows = (int*)(ws + l.rows);
-    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
+    T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
+    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     if (dx)
-        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
+        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
                          f, rows, part, (unsigned int*)(ws + l.tickets), st);
     WgradProblem<T> w[2]{};
     int n = 0;
@@ -703,7 +774,7 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         const float* h = hidden;
         if (!h) {
             h = (float*)(ws + l.hid2);
-            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), st, rows);
+            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), (T*)nullptr, st, rows);
         }
         w[n++] = WgradProblem<T>{h, (const T*)dy, lddy, db, nullptr, (int)p.out_features};
     }
