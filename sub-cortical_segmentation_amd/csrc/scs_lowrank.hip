@@ -439,6 +439,7 @@ __global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
 }  // namespace scs
 #include "lowrank_mfma16.h"
 #include "lowrank_tiles.h"
+#include "lowrank_tiles32.h"
 #include "lowrank_few.h"
 namespace scs {
 namespace {
@@ -714,11 +715,29 @@ template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& 
     if (f.mt) { project_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
     if constexpr (sizeof(T) == 2) { project16<T, TRANS>(g, st); return; }
     // the column tile with the least padding, the widest among equals
-    int best = 8, waste = 1 << 30;
-    for (const int nt : {8, 6, 4}) {
-        const int w = (g.N + 16 * nt - 1) / (16 * nt) * 16 * nt;
-        if (w < waste) { waste = w; best = nt; }
+    auto least = [&](std::initializer_list<int> nts) {
+        int best = 0, waste = 1 << 30;
+        for (const int nt : nts) {
+            const int w = (g.N + 16 * nt - 1) / (16 * nt) * 16 * nt;
+            if (w < waste) { waste = w; best = nt; }
+        }
+        return best;
+    };
+    if constexpr (sizeof(T) == 4) {
+        const bool aligned = g.K % 4 == 0 && g.N % 4 == 0 && g.ldx % 4 == 0 && g.ldw % 4 == 0 && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.w % 16 == 0;
+        if (aligned && g.ldx <= (1 << 21) && g.ldw <= (1 << 21)) {
+            const int nt = least({8, 7, 6, 5, 4});
+            const dim3 grid((unsigned)((g.r.rows + 127) / 128 * ((g.N + 16 * nt - 1) / (16 * nt))));
+            auto go = [&](auto n) { hipLaunchKernelGGL((project_tiles32_kernel<n.value, TRANS>), grid, dim3(256), 0, st, g); };
+            if (nt == 8) go(std::integral_constant<int, 8>{});
+            else if (nt == 7) go(std::integral_constant<int, 7>{});
+            else if (nt == 6) go(std::integral_constant<int, 6>{});
+            else if (nt == 5) go(std::integral_constant<int, 5>{});
+            else go(std::integral_constant<int, 4>{});
+            return;
+        }
     }
+    const int best = least({8, 6, 4});
     const dim3 grid((unsigned)((g.r.rows + kPBM - 1) / kPBM), (unsigned)((g.N + 16 * best - 1) / (16 * best)));
     if (best == 8) hipLaunchKernelGGL((project_f32_kernel<T, 8, TRANS>), grid, dim3(256), 0, st, g);
     else if (best == 6) hipLaunchKernelGGL((project_f32_kernel<T, 6, TRANS>), grid, dim3(256), 0, st, g);
