@@ -354,8 +354,10 @@ typedef struct {
     const int32_t* adapters;       /* [n_requests] */
 } scs_lowrank;
 
-/* Bytes of workspace that a call needs (device memory, aligned to 16 bytes; it may be shared by calls that run one after the other). */
-int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward, size_t* bytes);
+/* Bytes of workspace that a call needs (device memory, aligned to 16 bytes; it may be shared by calls that run one after the other).
+ * rows_dev, ld: x and ldx of the forward call, dy and lddy of the backward call (only their alignment counts: operands that do not lie at
+ * multiples of 16 bytes are laid out anew in the workspace). */
+int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward, const void* rows_dev, int64_t ld, size_t* bytes);
 
 /* x [rows][in] with row stride ldx >= in (elements), y [rows][out] with ldy >= out; y must not overlap the inputs.
  * hidden: f32 [rows][rank] or NULL; receives x_i A_s^T (0 where a row has no adapter) for the backward call. */

@@ -61,7 +61,7 @@ SIGNATURES = {
     'scs_set_fused_adam': (_c.c_int, [_vp, _c.c_int, _c.c_float, _c.c_float, _c.c_float, _c.c_float]),
     'scs_eval_batch': (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _c.c_int64, _c.POINTER(_c.c_double),
                                   _c.POINTER(_c.c_int64), _vp]),
-    'scs_lowrank_workspace': (_c.c_int, [_vp, _vp, _c.c_int, _c.POINTER(_c.c_size_t)]),
+    'scs_lowrank_workspace': (_c.c_int, [_vp, _vp, _c.c_int, _vp, _c.c_int64, _c.POINTER(_c.c_size_t)]),
     'scs_lowrank_forward': (_c.c_int, [_vp, _vp, _vp, _c.c_int64, _vp, _c.c_int64, _vp, _vp, _c.c_size_t, _vp]),
     'scs_lowrank_backward': (_c.c_int, [_vp, _vp, _vp, _c.c_int64, _vp, _c.c_int64, _vp, _vp, _c.c_int64, _vp, _vp, _vp, _c.c_size_t, _vp]),
     'scs_adamw_create': (_c.c_int, [_vp, _vp, _c.c_int32, _c.c_int, _vp, _vp, _vp, _vp, _c.c_int64, _c.POINTER(_vp)]),

@@ -133,15 +133,16 @@ class Projection:
         call.rows, call.n_requests, call.offsets, call.adapters = rows, n, offsets.data_ptr(), adapters.data_ptr()
         return self._tls.ref
 
-    def _workspace(self, call, back, rows, requests):
-        """Workspace of a call; its size hangs on the numbers of rows and requests alone."""
-        n = self._sizes.get((back, rows, requests))
+    def _workspace(self, call, back, rows, requests, at, ld):
+        """Workspace of a call; its size hangs on the numbers of rows and requests and on whether the rows lie at multiples of 16 bytes."""
+        key = (back, rows, requests, at % 16, ld)
+        n = self._sizes.get(key)
         if n is None:
             size = ctypes.c_size_t(0)
-            _hip._check(self._lib.scs_lowrank_workspace(self.handle.h, call, back, ctypes.byref(size)), 'scs_lowrank_workspace')
+            _hip._check(self._lib.scs_lowrank_workspace(self.handle.h, call, back, at, ld, ctypes.byref(size)), 'scs_lowrank_workspace')
             if len(self._sizes) > 4096:
                 self._sizes.clear()
-            n = self._sizes[back, rows, requests] = size.value
+            n = self._sizes[key] = size.value
         return self._torch.empty((n + 16,), dtype=self._torch.uint8, device=self.device), n
 
     def forward(self, x, offsets, adapters, out=None, hidden=None):
@@ -159,7 +160,7 @@ class Projection:
         if hidden is not None:
             outs.append(('hidden', self._flat(hidden, (rows, self.rank), 'hidden')))
         self._apart(outs, [(px[0], px[2])] + self._reads)
-        ws, n = self._workspace(call, 0, rows, adapters.numel())
+        ws, n = self._workspace(call, 0, rows, adapters.numel(), px[0], px[1])
         rc = self._lib.scs_lowrank_forward(self.handle.h, call, px[0], px[1], py[0], py[1], outs[1][1][0] if hidden is not None else None,
                                            ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
         if rc:
@@ -200,7 +201,7 @@ class Projection:
             ph = self._flat(hidden, (rows, self.rank), 'hidden')
             reads.append((ph[0], ph[2]))
         self._apart(outs, reads)
-        ws, n = self._workspace(call, 1, rows, adapters.numel())
+        ws, n = self._workspace(call, 1, rows, adapters.numel(), pdy[0], pdy[1])
         rc = self._lib.scs_lowrank_backward(self.handle.h, call, px[0], px[1], pdy[0], pdy[1], ph and ph[0], pdx[0], pdx[1], pg[0][1], pg[1][1],
                                             ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
         if rc:

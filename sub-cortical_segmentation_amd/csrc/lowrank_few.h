@@ -10,7 +10,7 @@
 // up in their order, so the result does not depend on which one that is.
 #pragma once
 #include "scs_ops.h"
-#include "lowrank_mfma16.h"
+#include "lowrank_tiles.h"
 
 namespace scs {
 namespace {

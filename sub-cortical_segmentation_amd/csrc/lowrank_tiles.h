@@ -1,19 +1,42 @@
-// The shared projection on the 16-bit matrix cores for many rows and 16-byte-aligned operands (scs_lowrank.hip): a pipelined form of
-// lowrank_mfma16.h (same transposed product, same two LDS images).
+// The shared projection on the 16-bit matrix cores for many rows (scs_lowrank.hip): Y = X W' + scale_s H P_s for bf16 and f16.
 //
-// What bounds it: LDS.  A slab of 32 along the contraction costs a workgroup (BM + BN) 64 bytes of copies into LDS, and every wave reads its
-// own (16 MT + 16 NT) 64 bytes back; at 256 x 256 with four waves of 128 x 128 that is 6 bytes a cycle and matrix core of the 128 the LDS has,
-// against 1024 cycles of MFMA (eight waves of 128 x 64 read 1.5 times as much).  So the wave tile is as large as the accumulators allow (256
-// AGPRs), one wave per SIMD, and what hides latency is the pipeline alone: four slabs of LDS, three in flight while one is read, a slab's
-// fragments read into registers while the slab before is multiplied, one barrier a slab that no copy has to be drained for.
+// D is formed transposed (A operand = weights, B operand = rows of X: v_mfma_f32_16x16x32), so that a lane holds four consecutive columns of
+// one row.  A workgroup owns BM x BN of Y; both operands pass through LDS in slabs of 32 along the contraction, copied global -> LDS in 16-byte
+// pieces without a register between.  LDS images, swizzled so that a fragment's lanes meet no bank twice:
+//   K-major [row][32]: 16-byte piece c of a row lies at c ^ (row >> 2 & 3).  X always; W' where it is W^T (backward: W's rows run along the contraction)
+//   N-major [32][BN]:  32-byte unit u of row k lies at u ^ f(k), f = (k & 3) | (k >> 3 & 1) << 2 (as many of its bits as there are units).  W (forward) and the adapters' P: the transposing
+//            LDS read (ds_read_b64_tr_b16) turns four rows of sixteen columns into each column's four contraction values
+//
+// What bounds it: LDS and the matrix cores alike.  A slab costs a 256 x 256 tile 32 KB of copies into LDS and eight waves of 128 x 64 96 KB of
+// fragment reads, 1024 cycles of the LDS's 128 bytes a cycle against 1024 of MFMA.  Four waves of 128 x 128 would read a third less, but
+// their 256 sums leave the compiler too few registers: 530 us instead of 260 at 8192 x 4096 x 4096.  What hides latency is the pipeline: four slabs
+// of LDS, three in flight while one is read, a slab's fragments read into registers while the slab before is multiplied, one barrier a slab
+// that no copy has to be drained for (drained at every slab: 350 us).  8192 x 4096 x 4096, bf16: about 230 us, 1200 TFLOP/s.
 //
 // The copies are issued from inline assembly because the compiler, which tracks them, waits for every one of them before the next LDS read; the
 // waits are written out instead (copies return in order: vmcnt(n) leaves the n youngest in flight).
 #pragma once
-#include "lowrank_mfma16.h"
+#include "scs_ops.h"
 
 namespace scs {
 namespace {
+
+__device__ const u32x4 kZeroPiece = {0, 0, 0, 0};            // what lies behind the end of the contraction
+
+// eight elements at any element alignment, zeros behind `left`
+template <class T> __device__ __forceinline__ u32x4 load8(const T* p, int64_t left) {
+    if (left >= 8) return reinterpret_cast<const Loose<u32x4>*>(p)->v;
+    T e[8] = {};
+    for (int i = 0; i < 7; ++i) if (i < left) e[i] = p[i];
+    u32x4 r;
+    __builtin_memcpy(&r, e, 16);
+    return r;
+}
+
+// four contraction values of this lane's column out of the transposing read
+__device__ __forceinline__ s16x4 lds_transposed(const void* p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+}
 
 // 16 bytes a lane from base + offset (bytes) to LDS byte `lds` + 16 lane; no register is written, so none can be overtaken
 __device__ __forceinline__ void copy_to_lds(const void* base, unsigned int offset, unsigned int lds) {
@@ -26,10 +49,12 @@ __device__ __forceinline__ void workgroup_barrier() {
     asm volatile("" : : : "memory");
 }
 
-template <class T, int WN, int MT, int NT, bool TRANS>
+// EVEN: N is a multiple of 8 (outputs, bias and P are read and written four and eight columns at a time)
+template <class T, int WN, int MT, int NT, bool TRANS, bool EVEN>
 __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<T> g) {
     typedef typename Frag<T>::v8 v8;
     constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * WN * NT, BK = 32, STAGES = 4, NP = BN / 8;
+    constexpr int UNITS = BN / 16 < 8 ? BN / 16 - 1 : 7;               // bits of f(k) that a row has units for
     constexpr int A_IT = BM * 4 / THREADS, B_IT = BN * 4 / THREADS, LOADS = A_IT + B_IT;
     __shared__ __attribute__((aligned(16))) T s_a[STAGES][BM * BK];
     __shared__ __attribute__((aligned(16))) T s_b[STAGES][BN * BK];
@@ -37,7 +62,8 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     const int lr = lane & 15, kq = lane >> 4, wm = wave / WN, wn = wave % WN;
     const Requests& r = g.r;
 
-    // (the order of lowrank_mfma16.h: a run of neighbouring tiles, eight row tiles high, for each XCD)
+    // workgroups are dealt to the eight XCDs in turn: give each XCD a run of neighbouring tiles, eight row tiles high, so that its L2
+    // serves W's columns and X's rows again
     int m0, n0;
     {
         const int tm = (r.rows + BM - 1) / BM, tn = (g.N + BN - 1) / BN, total = tm * tn, pid = blockIdx.x;
@@ -48,7 +74,6 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
         n0 = in / high * BN;
     }
 
-    // K-major image [row][32]: piece c of a row at c ^ (row >> 2 & 3); N-major image [32][BN]: unit u of row k at u ^ f(k), as before.
     // Addresses are a uniform base, which moves along the contraction, and a lane's 32-bit offset inside the tile (rows and columns beyond
     // the matrices read as their last ones)
     const int pa = (tid & 3) ^ ((tid >> 4) & 3);
@@ -62,13 +87,13 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     for (int i = 0; i < B_IT; ++i) {
         if constexpr (TRANS) ob[i] = (unsigned int)(min((tid >> 2) + i * (THREADS / 4), g.N - 1 - n0) * (int)g.ldw + pa * 8) * 2u;
         else {
-            const int k = tid / NP + i * (THREADS / NP), f = (k & 3) | ((k >> 3) & 1) << 2, piece = ((((tid % NP) >> 1) ^ f) << 1) | (tid & 1);
-            ob[i] = (unsigned int)(k * (int)g.ldw + min(piece * 8, g.N - 8 - n0)) * 2u;
+            const int k = tid / NP + i * (THREADS / NP), f = ((k & 3) | ((k >> 3) & 1) << 2) & UNITS, piece = ((((tid % NP) >> 1) ^ f) << 1) | (tid & 1);
+            ob[i] = (unsigned int)(k * (int)g.ldw + min(piece * 8, g.nw - 8 - n0)) * 2u;
         }
     }
     const unsigned int lds_a = (unsigned int)(uintptr_t)(__attribute__((address_space(3))) void*)&s_a[0][0] + wave * 1024;
     const unsigned int lds_b = (unsigned int)(uintptr_t)(__attribute__((address_space(3))) void*)&s_b[0][0] + wave * 1024;
-    const int slabs = g.K / BK;                              // (K is a multiple of 2 BK)
+    const int slabs = g.K / BK;                              // (K is a multiple of 64)
     // slab s into its stage; those beyond the last one are copied for the count's sake alone (the last one again, which nobody reads)
     auto fetch = [&](int s) {
         const int from = min(s, slabs - 1);
@@ -83,7 +108,7 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
 
     const int ka = (wm * MT * 16 + lr) * BK + ((kq ^ (lr >> 2)) * 8);                                  // (row >> 2 & 3 is lr >> 2: tiles are 16 rows)
     const int kt = (wn * NT * 16 + lr) * BK + ((kq ^ (lr >> 2)) * 8);
-    const int fr = (lr >> 2) | (kq & 1) << 2, nb = (8 * kq + (lr >> 2)) * BN + (lr & 3) * 4;
+    const int fr = ((lr >> 2) | (kq & 1) << 2) & UNITS, nb = (8 * kq + (lr >> 2)) * BN + (lr & 3) * 4;
     auto frag_x = [&](int st, int i) { return *(const v8*)&s_a[st][ka + i * 16 * BK]; };
     auto frag_n = [&](int st, int tile) {
         const T* at = &s_b[st][nb + ((tile ^ fr) << 4)];
@@ -153,7 +178,7 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     const int m1 = min(m0 + BM, r.rows), mw = m0 + wm * MT * 16;
     auto frag_x_at = [&](int lr, int kq, int tile) { return *(const v8*)&s_a[0][(tile * 16 + lr) * BK + ((kq ^ (lr >> 2)) * 8)]; };
     auto frag_n_at = [&](int lr, int kq, int tile) {
-        const T* at = &s_b[0][(8 * kq + (lr >> 2)) * BN + ((tile ^ ((lr >> 2) | (kq & 1) << 2)) << 4) + (lr & 3) * 4];
+        const T* at = &s_b[0][(8 * kq + (lr >> 2)) * BN + ((tile ^ (((lr >> 2) | (kq & 1) << 2) & UNITS)) << 4) + (lr & 3) * 4];
         const s16x4 lo = lds_transposed(at), hi = lds_transposed(at + 4 * BN);
         v8 v;
         __builtin_memcpy(&v, &lo, 8);
@@ -179,9 +204,10 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
             }
             for (int e = tid; e < 16 * NP; e += THREADS) {
                 const int k = e / NP, c = e % NP, j = j0 + k;
-                const u32x4 v = at16(ps + (int64_t)min(j, r.rank - 1) * g.N + min(n0 + c * 8, g.N - 8));
+                const T* at_p = ps + (int64_t)min(j, r.rank - 1) * g.N;
+                const u32x4 v = EVEN ? at16(at_p + min(n0 + c * 8, g.N - 8)) : load8(at_p + n0 + c * 8, g.N - (n0 + c * 8));
                 const u32x4 w = j < r.rank ? v : u32x4{0, 0, 0, 0};
-                const int f = (k & 3) | ((k >> 3) & 1) << 2, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
+                const int f = ((k & 3) | ((k >> 3) & 1) << 2) & UNITS, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
                 *(u32x4*)&s_b[0][k * BN + at] = w;
                 *(u32x4*)&s_b[0][(k + 16) * BN + at] = w;
             }
@@ -206,11 +232,16 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     const int live_lo = clamp_row(r.offsets[0], r.rows), live_hi = clamp_row(r.offsets[r.n], r.rows);
     int el = threadIdx.x & 63;
     asm volatile("" : "+v"(el));
-    const int col = n0 + wn * NT * 16 + 4 * (el >> 4);                    // (N is a multiple of 8: four columns or none)
+    const int col = n0 + wn * NT * 16 + 4 * (el >> 4);
     float bias[NT][4] = {};
     if (g.bias) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) unpack<T>(at4(g.bias + min(col + j * 16, g.N - 4)), bias[j]);
+        for (int j = 0; j < NT; ++j) {
+            typename Vec4<T>::raw b = {};
+            if constexpr (EVEN) b = at4(g.bias + min(col + j * 16, g.N - 4));
+            else raw_load<T>(b, g.bias + col + j * 16, g.N - (col + j * 16));
+            unpack<T>(b, bias[j]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -220,7 +251,9 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
                 const float v[4] = {acc[i][j][0] + bias[j][0], acc[i][j][1] + bias[j][1], acc[i][j][2] + bias[j][2], acc[i][j][3] + bias[j][3]};
-                if (col + j * 16 < g.N) reinterpret_cast<Loose<u32x2>*>(y + j * 16)->v = pack<T>(v);
+                if constexpr (EVEN) {
+                    if (col + j * 16 < g.N) reinterpret_cast<Loose<u32x2>*>(y + j * 16)->v = pack<T>(v);
+                } else raw_store<T>(pack<T>(v), y + j * 16, g.N - (col + j * 16));
             }
         }
         __builtin_amdgcn_sched_barrier(0);

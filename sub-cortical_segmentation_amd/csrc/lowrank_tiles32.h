@@ -1,4 +1,4 @@
-// The shared projection on the f32 matrix cores for many rows and 16-byte-aligned operands (scs_lowrank.hip): the pipeline of lowrank_tiles.h
+// The shared projection on the f32 matrix cores for many rows (scs_lowrank.hip): the pipeline of lowrank_tiles.h
 // (four slabs of LDS, copies in flight across barriers, the next slab's fragments read while this one is multiplied) with exact f32 products.
 //
 // What bounds it: v_mfma_f32_16x16x4_f32, 32 cycles each on the vector ALUs, which every other vector instruction takes time from: so the copies
@@ -17,7 +17,8 @@ __device__ __forceinline__ void copy_to_lds(const void* src, unsigned int lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
 }
 
-template <int NT, bool TRANS>
+// EVEN: N is a multiple of 4
+template <int NT, bool TRANS, bool EVEN>
 __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<float> g) {
     constexpr int BM = 128, BN = 16 * NT, BK = 16, STAGES = 4, NP = BN / 4, LOADS = 4;
     __shared__ __attribute__((aligned(16))) float s_a[STAGES][BM * BK];
@@ -26,7 +27,7 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
     const int lr = lane & 15, kq = lane >> 4;
     const Requests& r = g.r;
 
-    // (a run of neighbouring tiles, eight row tiles high, for each XCD: lowrank_mfma16.h)
+    // (a run of neighbouring tiles, eight row tiles high, for each XCD: lowrank_tiles.h)
     int m0, n0;
     {
         const int tm = (r.rows + BM - 1) / BM, tn = (g.N + BN - 1) / BN, total = tm * tn, pid = blockIdx.x;
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
         } else {
             const int l = tid + i * 256, k = min(l / NP, BK - 1), at = l - l / NP * NP, piece = (at + NP - 4 * (k >> 2) % NP) % NP;
             kb[i] = k;
-            ob[i] = (unsigned int)(k * (int)g.ldw + min(piece * 4, g.N - 4 - n0)) * 4u;
+            ob[i] = (unsigned int)(k * (int)g.ldw + min(piece * 4, g.nw - 4 - n0)) * 4u;
         }
     }
     const unsigned int lds_a = (unsigned int)(uintptr_t)(__attribute__((address_space(3))) void*)&s_a[0][0] + wave * 1024;
@@ -158,7 +159,10 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
             }
             for (int e = tid; e < BK * NP; e += 256) {
                 const int k = e / NP, c = e - k * NP;
-                const f32x4 v = at4(ps + (int64_t)min(j0 + k, r.rank - 1) * g.N + min(n0 + c * 4, g.N - 4));
+                const float* at = ps + (int64_t)min(j0 + k, r.rank - 1) * g.N;
+                f32x4 v;
+                if constexpr (EVEN) v = at4(at + min(n0 + c * 4, g.N - 4));
+                else raw_load<float>(v, at + n0 + c * 4, g.N - (n0 + c * 4));
                 const f32x4 z = f32x4{0.f, 0.f, 0.f, 0.f};
                 *(f32x4*)&s_b[0][k * BN + (c + 4 * (k >> 2)) % NP * 4] = j0 + k < r.rank ? v : z;
             }
@@ -193,11 +197,17 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
         if (row < live_lo || row >= live_hi) continue;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int col = n0 + t * 16 + 4 * kq;            // (N is a multiple of 4: four columns or none)
+            const int col = n0 + t * 16 + 4 * kq;
             if (col >= g.N) continue;
             f32x4 v = acc[i][t];
-            if (g.bias) v += at4(g.bias + col);
-            reinterpret_cast<Loose<f32x4>*>(g.y + (int64_t)row * g.ldy + col)->v = v;
+            if constexpr (EVEN) {
+                if (g.bias) v += at4(g.bias + col);
+                reinterpret_cast<Loose<f32x4>*>(g.y + (int64_t)row * g.ldy + col)->v = v;
+            } else {
+                f32x4 b = f32x4{0.f, 0.f, 0.f, 0.f};
+                if (g.bias) raw_load<float>(b, g.bias + col, g.N - col);
+                raw_store<float>(v + b, g.y + (int64_t)row * g.ldy + col, g.N - col);
+            }
         }
     }
 }

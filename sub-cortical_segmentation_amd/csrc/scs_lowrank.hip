@@ -272,9 +272,7 @@ __global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ 
     }
 }
 
-// ------------------------------------------------------------------------------------------------------------------ project, f32 matrix cores
-// Any type, any size, any stride: 128 rows x 16 NT columns a workgroup of four waves (32 rows each), the contraction in slabs of 32 staged
-// through LDS as f32 (registers hold the next slab while this one is multiplied).
+// ------------------------------------------------------------------------------------------------------------------ project
 template <class T>
 struct ProjectArgs {
     const T* x; int64_t ldx;
@@ -285,159 +283,29 @@ struct ProjectArgs {
     const T* pieces;                  // 16-bit types, many rows: scale_s h as two 16-bit pieces, [rows][ceil(rank / 16)][16 upper | 16 lower]
     T* y; int64_t ldy;
     int32_t K, N;
+    int32_t nw;                       // columns of W's rows that can be read (N-major W: N, or more where it was laid out anew)
     Requests r;
 };
 
-constexpr int kPBM = 128, kPBK = 32, kPAS = 36;
-
-template <class T, int NT, bool TRANS>
-__global__ __launch_bounds__(256, 2) void project_f32_kernel(ProjectArgs<T> g) {
-    constexpr int BN = 16 * NT, BS = BN + 4;                 // (4 BS % 64 == 16: the four k-rows of a fragment lie on disjoint banks)
-    constexpr int B_FLOATS = TRANS ? (BN * kPAS > kPBK * BS ? BN * kPAS : kPBK * BS) : kPBK * BS;
-    __shared__ __attribute__((aligned(16))) float s_a[2][kPBM * kPAS];
-    __shared__ __attribute__((aligned(16))) float s_b[2][B_FLOATS];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int lr = lane & 15, kq = lane >> 4;
-    const int m0 = blockIdx.x * kPBM, n0 = blockIdx.y * BN;
-    const Requests& r = g.r;
-
-    constexpr int A_PER = kPBM * kPBK / 1024, B_PER = (BN * kPBK / 4 + 255) / 256;
-    typename Vec4<T>::raw ra[A_PER], rb[B_PER];
-    auto load_slab = [&](int k0) {
-#pragma unroll
-        for (int i = 0; i < A_PER; ++i) {                    // 8 vectors a row, 32 rows at a time
-            const int row = m0 + (tid >> 3) + 32 * i, k = k0 + (tid & 7) * 4;
-            raw_load<T>(ra[i], g.x + (int64_t)row * g.ldx + k, row < r.rows ? g.K - k : 0);
-        }
-#pragma unroll
-        for (int i = 0; i < B_PER; ++i) {
-            const int e = tid + 256 * i;
-            if constexpr (TRANS) {
-                const int n = n0 + (e >> 3), k = k0 + (e & 7) * 4;
-                raw_load<T>(rb[i], g.w + (int64_t)n * g.ldw + k, (e >> 3) < BN && n < g.N ? g.K - k : 0);
-            } else {
-                const int kr = e / (BN / 4), n = n0 + (e - kr * (BN / 4)) * 4, k = k0 + kr;
-                raw_load<T>(rb[i], g.w + (int64_t)k * g.ldw + n, kr < kPBK && k < g.K ? g.N - n : 0);
-            }
-        }
-    };
-    auto store_slab = [&](int buf) {
-#pragma unroll
-        for (int i = 0; i < A_PER; ++i) {
-            float f[4];
-            unpack<T>(ra[i], f);
-            *(f32x4*)&s_a[buf][((tid >> 3) + 32 * i) * kPAS + (tid & 7) * 4] = f32x4{f[0], f[1], f[2], f[3]};
-        }
-#pragma unroll
-        for (int i = 0; i < B_PER; ++i) {
-            const int e = tid + 256 * i;
-            float f[4];
-            unpack<T>(rb[i], f);
-            if constexpr (TRANS) {
-                if ((e >> 3) < BN) *(f32x4*)&s_b[buf][(e >> 3) * kPAS + (e & 7) * 4] = f32x4{f[0], f[1], f[2], f[3]};
-            } else {
-                const int kr = e / (BN / 4), c = (e - kr * (BN / 4)) * 4;
-                if (kr < kPBK) *(f32x4*)&s_b[buf][kr * BS + c] = f32x4{f[0], f[1], f[2], f[3]};
-            }
-        }
-    };
-
-    f32x4 acc[2][NT];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const int slabs = (g.K + kPBK - 1) / kPBK;
-    load_slab(0);
-    store_slab(0);
-    __syncthreads();
-    for (int s = 0; s < slabs; ++s) {
-        if (s + 1 < slabs) load_slab((s + 1) * kPBK);
-        const float* sa = s_a[s & 1] + (wave * 32 + lr) * kPAS + 4 * kq;
-        const float* sb = s_b[s & 1];
-#pragma unroll
-        for (int ks = 0; ks < kPBK; ks += 16) {
-            const f32x4 a0 = *(const f32x4*)(sa + ks), a1 = *(const f32x4*)(sa + 16 * kPAS + ks);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                f32x4 b;
-                if constexpr (TRANS) b = *(const f32x4*)(sb + (t * 16 + lr) * kPAS + ks + 4 * kq);
-                else
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b[j] = sb[(ks + 4 * kq + j) * BS + t * 16 + lr];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc[0][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[j], b[j], acc[0][t], 0, 0, 0);
-                    acc[1][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[j], b[j], acc[1][t], 0, 0, 0);
-                }
-            }
-        }
-        if (s + 1 < slabs) store_slab((s + 1) & 1);
-        __syncthreads();
-    }
-
-    // the adapters' products, request by request, each under the mask of its rows
-    const int m1 = min(m0 + kPBM, r.rows);
-    Walk walk(r, m0, m1);
-    int q;
-    Span sp;
-    while (walk.next(q, sp)) {
-        if (sp.s < 0) continue;
-        const float scale = walk.scale(sp);
-        const T* ps = g.low + (int64_t)sp.s * r.rank * g.N;
-        for (int j0 = 0; j0 < r.rank; j0 += kPBK) {
-            for (int e = tid; e < kPBM * kPBK; e += 256) {
-                const int m = e / kPBK, j = e % kPBK, row = m0 + m;
-                const bool in = row >= sp.lo && row < sp.hi && j0 + j < r.rank;
-                s_a[0][m * kPAS + j] = in ? scale * g.h[(int64_t)row * r.rank + j0 + j] : 0.f;
-            }
-            for (int e = tid; e < kPBK * BN; e += 256) {
-                const int j = e / BN, c = e % BN;
-                s_b[0][j * BS + c] = j0 + j < r.rank && n0 + c < g.N ? to_f32(ps[(int64_t)(j0 + j) * g.N + n0 + c]) : 0.f;
-            }
-            __syncthreads();
-            const float* sa = s_a[0] + (wave * 32 + lr) * kPAS + 4 * kq;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
-                    for (int ks = 0; ks < kPBK && j0 + ks < r.rank; ks += 16) {
-                        const f32x4 a = *(const f32x4*)(sa + i * 16 * kPAS + ks);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            part = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], s_b[0][(ks + 4 * kq + j) * BS + t * 16 + lr], part, 0, 0, 0);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = m0 + wave * 32 + i * 16 + 4 * kq + e;
-                        if (row >= sp.lo && row < sp.hi) acc[i][t][e] += part[e];
-                    }
-                }
-            __syncthreads();
-        }
-    }
-
-    const int live_lo = r.n ? clamp_row(r.offsets[0], r.rows) : 0, live_hi = r.n ? clamp_row(r.offsets[r.n], r.rows) : 0;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int col = n0 + t * 16 + lr;
-        if (col >= g.N) continue;
-        const float bv = g.bias ? to_f32(g.bias[col]) : 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int row = m0 + wave * 32 + i * 16 + 4 * kq + e;
-                if (row >= live_lo && row < live_hi) g.y[(int64_t)row * g.ldy + col] = from_f32<T>(acc[i][t][e] + bv);
-            }
+// The tile kernels copy 16-byte pieces: rows that start at any element, or sizes that end inside a piece, are first laid out anew with zeros
+// behind their ends (up to two matrices in one launch; their bytes once read and once written).
+struct PackMatrix { const void* src; void* dst; int64_t ld; int32_t rows, cols, rows_out, cols_out; };
+struct PackArgs { PackMatrix m[2]; };
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs g) {
+    constexpr int PER = 16 / sizeof(T);
+    const PackMatrix& m = g.m[blockIdx.y];
+    const int pieces = m.cols_out / PER;
+    const int64_t n = (int64_t)m.rows_out * pieces;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / pieces;
+        const int col = (int)(i - row * pieces) * PER;
+        ((u32x4*)m.dst)[i] = load16((const T*)m.src + row * m.ld + col, row < m.rows ? m.cols - col : 0);
     }
 }
 
 }  // namespace
 }  // namespace scs
-#include "lowrank_mfma16.h"
 #include "lowrank_tiles.h"
 #include "lowrank_tiles32.h"
 #include "lowrank_few.h"
@@ -619,8 +487,27 @@ Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     }
     return f;
 }
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, pieces = 0, bytes = 0; };
-Layout layout_of(const scs_lowrank& p, bool backward) {
+// What of a projection's operands has to be laid out anew for the tile kernels: K up to a multiple of 64 (16-bit) or 4 (f32), rows at multiples
+// of 16 bytes.  `K`, `N`: of this direction; `x`, `ldx`: X as the call gets it.
+struct Pack { bool x = false, w = false; int64_t K = 0, nw = 0, w_rows = 0, w_cols = 0; size_t x_bytes = 0, w_bytes = 0; };
+Pack pack_of(const scs_lowrank& p, int64_t K, int64_t N, bool trans, const void* x, int64_t ldx) {
+    Pack k;
+    const int e = p.dtype == SCS_F32 ? 4 : 2, per = 16 / e, unit = p.dtype == SCS_F32 ? 4 : 64;
+    auto whole = [](int64_t v, int64_t u) { return (v + u - 1) / u * u; };
+    k.K = whole(K, unit);
+    // (2^21: the tile kernels' offsets inside a tile have 32 bits)
+    k.x = k.K != K || ldx % per || (uintptr_t)x % 16 || ldx > (1 << 21);
+    k.w = k.K != K || p.ldw % per || (uintptr_t)p.w % 16 || (!trans && N % per) || p.ldw > (1 << 21);
+    k.nw = trans ? N : whole(N, per);
+    k.w_rows = trans ? N : k.K;
+    k.w_cols = trans ? k.K : k.nw;
+    if (k.x) k.x_bytes = (size_t)p.rows * k.K * e;
+    if (k.w) k.w_bytes = (size_t)k.w_rows * k.w_cols * e;
+    return k;
+}
+
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, pieces = 0, pack_x = 0, pack_w = 0, bytes = 0; };
+Layout layout_of(const scs_lowrank& p, bool backward, const void* x, int64_t ldx) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t b) { const size_t o = at; at += up(b); return o; };
@@ -635,6 +522,11 @@ Layout layout_of(const scs_lowrank& p, bool backward) {
         if (const int b = wgrad_block_rows(p)) l.slots = take((size_t)(p.n_requests + (p.rows + b - 1) / b) * p.rank * (p.in_features + p.out_features) * 4);
     }
     l.part = take(part);
+    if (!f.mt) {
+        const Pack k = backward ? pack_of(p, p.out_features, p.in_features, true, x, ldx) : pack_of(p, p.in_features, p.out_features, false, x, ldx);
+        l.pack_x = take(k.x_bytes);
+        l.pack_w = take(k.w_bytes);
+    }
     l.bytes = at;
     return l;
 }
@@ -701,47 +593,54 @@ template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const F
     }
 }
 
-template <class T, bool TRANS> void project16(const ProjectArgs<T>& g, hipStream_t st) {
-    auto tiles = [&](int b) { return (int64_t)((g.r.rows + b - 1) / b) * ((g.N + b - 1) / b); };
-    const bool aligned = g.K % 8 == 0 && g.N % 8 == 0 && g.ldx % 8 == 0 && g.ldw % 8 == 0 && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.w % 16 == 0;
-    const bool piped = aligned && g.K % 64 == 0 && g.ldx <= (1 << 21) && g.ldw <= (1 << 21);
-    if (piped && tiles(256) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 4, 8, 4, TRANS>), dim3((unsigned)tiles(256)), dim3(512), 0, st, g);
-    else if (piped) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
-    else if (aligned) hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, true>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((project16_kernel<T, 2, 2, 4, 4, TRANS, false>), dim3((unsigned)tiles(128)), dim3(256), 0, st, g);
+template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T>& g, hipStream_t st) {
+    auto tiles = [&](int64_t bm, int64_t bn) { return (g.r.rows + bm - 1) / bm * ((g.N + bn - 1) / bn); };
+    if constexpr (sizeof(T) == 2) {
+        // the largest tile that still gives most of the 256 CUs one
+        if (tiles(256, 256) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 4, 8, 4, TRANS, EVEN>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, st, g);
+        else if (tiles(128, 128) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS, EVEN>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, g);
+        else hipLaunchKernelGGL((project_tiles_kernel<T, 2, 2, 2, TRANS, EVEN>), dim3((unsigned)tiles(64, 64)), dim3(256), 0, st, g);
+    } else {
+        // the column tile with the least padding, the widest among equals
+        int nt = 0, waste = 1 << 30;
+        for (const int n : {8, 7, 6, 5, 4}) {
+            const int w = (g.N + 16 * n - 1) / (16 * n) * 16 * n;
+            if (w < waste) { waste = w; nt = n; }
+        }
+        auto go = [&](auto n) { hipLaunchKernelGGL((project_tiles32_kernel<n.value, TRANS, EVEN>), dim3((unsigned)tiles(128, 16 * n.value)), dim3(256), 0, st, g); };
+        if (nt == 8) go(std::integral_constant<int, 8>{});
+        else if (nt == 7) go(std::integral_constant<int, 7>{});
+        else if (nt == 6) go(std::integral_constant<int, 6>{});
+        else if (nt == 5) go(std::integral_constant<int, 5>{});
+        else go(std::integral_constant<int, 4>{});
+    }
 }
 
-template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
+template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T> g, const Few& f, const int* rows, float* part, unsigned int* tickets, T* pack_x, T* pack_w,
+                                            hipStream_t st) {
+    g.nw = g.N;
     if (f.mt) { project_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
-    if constexpr (sizeof(T) == 2) { project16<T, TRANS>(g, st); return; }
-    // the column tile with the least padding, the widest among equals
-    auto least = [&](std::initializer_list<int> nts) {
-        int best = 0, waste = 1 << 30;
-        for (const int nt : nts) {
-            const int w = (g.N + 16 * nt - 1) / (16 * nt) * 16 * nt;
-            if (w < waste) { waste = w; best = nt; }
-        }
-        return best;
-    };
-    if constexpr (sizeof(T) == 4) {
-        const bool aligned = g.K % 4 == 0 && g.N % 4 == 0 && g.ldx % 4 == 0 && g.ldw % 4 == 0 && (uintptr_t)g.x % 16 == 0 && (uintptr_t)g.w % 16 == 0;
-        if (aligned && g.ldx <= (1 << 21) && g.ldw <= (1 << 21)) {
-            const int nt = least({8, 7, 6, 5, 4});
-            const dim3 grid((unsigned)((g.r.rows + 127) / 128 * ((g.N + 16 * nt - 1) / (16 * nt))));
-            auto go = [&](auto n) { hipLaunchKernelGGL((project_tiles32_kernel<n.value, TRANS>), grid, dim3(256), 0, st, g); };
-            if (nt == 8) go(std::integral_constant<int, 8>{});
-            else if (nt == 7) go(std::integral_constant<int, 7>{});
-            else if (nt == 6) go(std::integral_constant<int, 6>{});
-            else if (nt == 5) go(std::integral_constant<int, 5>{});
-            else go(std::integral_constant<int, 4>{});
-            return;
-        }
+    const Pack k = pack_of(p, g.K, g.N, TRANS, g.x, g.ldx);
+    PackArgs pa{};
+    int n = 0;
+    if (k.x) {
+        pa.m[n++] = PackMatrix{g.x, pack_x, g.ldx, g.r.rows, g.K, g.r.rows, (int)k.K};
+        g.x = pack_x;
+        g.ldx = k.K;
     }
-    const int best = least({8, 6, 4});
-    const dim3 grid((unsigned)((g.r.rows + kPBM - 1) / kPBM), (unsigned)((g.N + 16 * best - 1) / (16 * best)));
-    if (best == 8) hipLaunchKernelGGL((project_f32_kernel<T, 8, TRANS>), grid, dim3(256), 0, st, g);
-    else if (best == 6) hipLaunchKernelGGL((project_f32_kernel<T, 6, TRANS>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((project_f32_kernel<T, 4, TRANS>), grid, dim3(256), 0, st, g);
+    if (k.w) {
+        pa.m[n++] = PackMatrix{g.w, pack_w, g.ldw, TRANS ? g.N : g.K, TRANS ? g.K : g.N, (int)k.w_rows, (int)k.w_cols};
+        g.w = pack_w;
+        g.ldw = k.w_cols;
+        g.nw = (int)k.nw;
+    }
+    if (n) {
+        const int64_t most = std::max(k.x_bytes, k.w_bytes) / 16;
+        hipLaunchKernelGGL(pack_kernel<T>, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8192), n), dim3(256), 0, st, pa);
+    }
+    g.K = (int)k.K;
+    if (g.N % (sizeof(T) == 2 ? 8 : 4) == 0) project_tiles<T, TRANS, true>(g, st);
+    else project_tiles<T, TRANS, false>(g, st);
 }
 
 template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&problems)[2], int n, float* slots, hipStream_t st) {
@@ -760,14 +659,14 @@ template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&prob
 
 template <class T>
 int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t ldy, float* hidden, unsigned char* ws, hipStream_t st) {
-    const Layout l = layout_of(p, false);
+    const Layout l = layout_of(p, false, x, ldx);
     float* h = hidden ? hidden : (float*)(ws + l.hid);
     const Few f = few_of(p, p.in_features, p.out_features);
     int* rows = (int*)(ws + l.rows);
     T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
     shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
-    project<T, false>(ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, requests_of(p)},
-                      f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
+    project<T, false>(p, ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, 0, requests_of(p)},
+                      f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }
@@ -775,7 +674,7 @@ int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t l
 template <class T>
 int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, int64_t lddy, const float* hidden, void* dx, int64_t lddx, float* da, float* db,
              unsigned char* ws, hipStream_t st) {
-    const Layout l = layout_of(p, true);
+    const Layout l = layout_of(p, true, dy, lddy);
     float* u = (float*)(ws + l.hid);
     float* part = (float*)(ws + l.part);
     const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
@@ -784,8 +683,8 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
     if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     if (dx)
-        project<T, true>(ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, requests_of(p)},
-                         f, rows, part, (unsigned int*)(ws + l.tickets), st);
+        project<T, true>(p, ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, 0, requests_of(p)},
+                         f, rows, part, (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
     WgradProblem<T> w[2]{};
     int n = 0;
     if (da) w[n++] = WgradProblem<T>{u, (const T*)x, ldx, da, nullptr, (int)p.in_features};
@@ -809,11 +708,11 @@ using namespace scs;
 
 extern "C" {
 
-int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward_call, size_t* bytes) {
+int scs_lowrank_workspace(scs_handle h, const scs_lowrank* p, int backward_call, const void* rows_dev, int64_t ld, size_t* bytes) {
     SCS_ARG(h && bytes, "null handle or output");
     const int rc = check(p);
     if (rc != SCS_OK) return rc;
-    *bytes = layout_of(*p, backward_call != 0).bytes;
+    *bytes = layout_of(*p, backward_call != 0, rows_dev, ld).bytes;
     return SCS_OK;
 }
 
@@ -827,7 +726,7 @@ int scs_lowrank_forward(scs_handle h, const scs_lowrank* p, const void* x_dev, i
     SCS_ARG(x_dev && y_dev, "x or y is NULL");
     SCS_ARG(ldx >= p->in_features && ldy >= p->out_features, "a row stride is below the row's length");
     SCS_ARG((uintptr_t)x_dev % e == 0 && (uintptr_t)y_dev % e == 0 && (uintptr_t)hidden_dev % 4 == 0, "a matrix is not aligned to its elements");
-    const size_t need = layout_of(*p, false).bytes;
+    const size_t need = layout_of(*p, false, x_dev, ldx).bytes;
     SCS_ARG(workspace_bytes >= need && workspace_dev && (uintptr_t)workspace_dev % 16 == 0, "the workspace is too small, NULL or not aligned to 16 bytes (scs_lowrank_workspace)");
     DeviceGuard dev(handle_device(h));
     if (dev.rc != SCS_OK) return dev.rc;
@@ -852,7 +751,7 @@ int scs_lowrank_backward(scs_handle h, const scs_lowrank* p, const void* x_dev, 
     SCS_ARG(none || !dx_dev || lddx >= p->in_features, "the row stride of dx is below the row's length");
     SCS_ARG((uintptr_t)x_dev % e == 0 && (uintptr_t)dy_dev % e == 0 && (uintptr_t)dx_dev % e == 0 && (uintptr_t)hidden_dev % 4 == 0 &&
             (uintptr_t)da_dev % 4 == 0 && (uintptr_t)db_dev % 4 == 0, "a matrix is not aligned to its elements");
-    const size_t need = layout_of(*p, true).bytes;
+    const size_t need = layout_of(*p, true, dy_dev, lddy).bytes;
     SCS_ARG(need == 0 || (workspace_bytes >= need && workspace_dev && (uintptr_t)workspace_dev % 16 == 0),
             "the workspace is too small, NULL or not aligned to 16 bytes (scs_lowrank_workspace)");
     DeviceGuard dev(handle_device(h));

@@ -132,6 +132,9 @@ CASES = {
     'tokens, long contractions': (48, 2000, 1111, 20, 5, list(range(49)), [i % 7 - 1 for i in range(48)]),
     'few rows above a tile': (61, 1033, 640, 8, 2, [0, 30, 60], [1, 0]),
     'many tiles': (3100, 264, 4104, 16, 3, [0, 100, 1500, 1501, 3000, 3090], [0, 1, 2, -1, 0]),
+    'medium tiles': (1500, 192, 2056, 16, 3, [0, 100, 900, 1500], [0, 1, 2]),
+    'medium tiles, odd': (1600, 197, 2051, 9, 3, [0, 100, 900, 1600], [0, 1, 2]),
+    'many tiles, odd': (3333, 131, 4099, 17, 3, [0, 1000, 2222, 3333], [2, 1, 0]),
     'many tiles the other way': (2100, 4096, 328, 24, 3, [0, 700, 1500, 2100], [0, 1, 2]),
 }
 
