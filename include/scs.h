@@ -130,7 +130,12 @@ int scs_probe_f32_mfma_clock(scs_handle h, double* tflops, double* shader_ghz);
 int scs_forward(scs_handle h, const float* ax_dev, const float* co_dev, const float* sa_dev,
                 const float* atlas_dev, int64_t n, float* probs_dev, int32_t* labels_dev, void* stream);
 
-/* Same, host pointers: uploads chunk by chunk, synchronises before returning. */
+/* The dense head's input of the same forward pass: features_dev float32 [n][540], the three towers' d1 outputs side by side (nets.py:179, 215) -
+ * what site adapters of FC1, fc_2 and out_layer are trained and evaluated on.  Always the exact-f32 kernels. */
+int scs_forward_features(scs_handle h, const float* ax_dev, const float* co_dev, const float* sa_dev, const float* atlas_dev, int64_t n,
+                         float* features_dev, void* stream);
+
+/* scs_forward on host pointers: uploads chunk by chunk, synchronises before returning. */
 int scs_forward_host(scs_handle h, const float* ax, const float* co, const float* sa, const float* atlas,
                      int64_t n, float* probs, int32_t* labels);
 

@@ -34,6 +34,7 @@ SIGNATURES = {
     'scs_probe_f32_mfma': (_c.c_int, [_vp, _c.POINTER(_c.c_double)]),
     'scs_probe_f32_mfma_clock': (_c.c_int, [_vp, _c.POINTER(_c.c_double), _c.POINTER(_c.c_double)]),
     'scs_forward': (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _c.c_int64, _vp, _vp, _vp]),
+    'scs_forward_features': (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _c.c_int64, _vp, _vp]),
     'scs_forward_host': (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _c.c_int64, _vp, _vp]),
     'scs_forward_volume': (_c.c_int, [_vp, _vp, _c.c_int, _c.c_int, _c.c_int, _vp, _vp, _c.c_int64, _vp, _vp, _vp]),
     'scs_forward_volume_rows': (_c.c_int, [_vp, _vp, _c.c_int, _c.c_int, _c.c_int, _vp, _vp, _c.c_int64, _vp, _vp, _vp]),
@@ -308,6 +309,13 @@ class Handle:
         self._check_inputs(ax, co, sa, atlas, n, probs=probs, labels=labels)
         _check(self.lib.scs_forward(self.h, _ptr(ax), _ptr(co), _ptr(sa), _ptr(atlas), int(n), _ptr(probs),
                                     _ptr(labels), stream or None), 'scs_forward')
+
+    def forward_features(self, ax, co, sa, atlas, n, features, stream=0):
+        """features float32 [n, 540]: the dense head's input of the forward pass (scs_forward_features)."""
+        self._check_inputs(ax, co, sa, atlas, n)
+        _need(features, 540 * n, 'features')
+        _check(self.lib.scs_forward_features(self.h, _ptr(ax), _ptr(co), _ptr(sa), _ptr(atlas), int(n), _ptr(features), stream or None),
+               'scs_forward_features')
 
     def forward_host(self, ax, co, sa, atlas, n, probs=None, labels=None):
         self._check_inputs(ax, co, sa, atlas, n, probs=probs, labels=labels)

@@ -9,9 +9,11 @@ mini-batch, one new token), each with its own adapter or none.  The layers it st
 import ctypes
 import threading
 
+import numpy as np
+
 from . import _hip
 
-__all__ = ['Projection']
+__all__ = ['Projection', 'SiteAdapters', 'group_rows']
 
 
 class _Call(ctypes.Structure):
@@ -207,3 +209,86 @@ class Projection:
         if rc:
             _hip._check(rc, 'scs_lowrank_backward')
         return dx, pg[0][0], pg[1][0]
+
+
+def group_rows(sites):
+    """(order, offsets, adapters) of rows by site: `order` sorts them (stable), request q of the sorted rows is
+    [offsets[q], offsets[q + 1]) and uses adapters[q]."""
+    sites = np.asarray(sites, dtype=np.int64).ravel()
+    order = np.argsort(sites, kind='stable')
+    s = sites[order]
+    starts = np.flatnonzero(np.concatenate([[True], s[1:] != s[:-1]])) if s.size else np.zeros((0,), np.int64)
+    return order, np.concatenate([starts, [s.size]]).astype(np.int32), s[starts].astype(np.int32)
+
+
+class SiteAdapters:
+    """Low-rank adapters of the dense head (FC1, fc_2, out_layer: nets.py:217, 227, 231) for a number of sites, beside the weights of a Net.
+
+      params  parameter dict of the Net (the shared weights are copied to the device)
+      state   None - A ~ N(0, 1 / in), B = 0: every site predicts what the shared weights predict - or the arrays of state_dict()
+
+    The head's rectifiers sit between the layers as in the net (PReLU behind ReLU is the identity); dropout is off."""
+
+    LAYERS = ('FC1', 'fc_2', 'out_layer')
+
+    def __init__(self, handle, params, sites, rank=8, scale=1.0, seed=0, state=None):
+        import torch
+        self._torch = torch
+        self.device = torch.device('cuda', handle.device)
+        self.sites, self.rank = int(sites), int(rank)
+        up = lambda a: torch.from_numpy(np.array(a, dtype=np.float32, order='C')).to(self.device)
+        rng = np.random.default_rng(seed)
+        self.layers, self.tensors, self.names = [], [], []
+        self.scale = up(np.full((self.sites,), scale, np.float32) if state is None else state['scale'])
+        for name in self.LAYERS:
+            w, b = params[name]
+            n_in, n_out = w.shape
+            shapes = {'a': (self.sites, self.rank, n_in), 'b': (self.sites, self.rank, n_out)}
+            if state is None:
+                first = {'a': rng.normal(0.0, n_in ** -0.5, shapes['a']), 'b': np.zeros(shapes['b'])}
+            else:
+                first = {k: state['%s.%s' % (name, k)] for k in shapes}
+                for k, sh in shapes.items():
+                    if tuple(first[k].shape) != sh:
+                        raise ValueError('adapter array %s.%s has shape %r, expected %r' % (name, k, first[k].shape, sh))
+            a, d = up(first['a']), up(first['b'])
+            self.layers.append(Projection(handle, up(w), a, d, bias=up(b), scale=self.scale))
+            self.tensors += [a, d]
+            self.names += [name + '.a', name + '.b']
+
+    def state_dict(self):
+        """Host arrays: scale, <layer>.a, <layer>.b."""
+        d = {n: t.cpu().numpy() for n, t in zip(self.names, self.tensors)}
+        d['scale'] = self.scale.cpu().numpy()
+        return d
+
+    def _forward(self, features, atlas, offsets, sites, keep):
+        torch = self._torch
+        rows = features.shape[0]
+        hidden = [torch.zeros((rows, self.rank), device=self.device) for _ in self.layers] if keep else [None] * 3
+        x1 = features
+        y1 = torch.relu_(self.layers[0].forward(x1, offsets, sites, hidden=hidden[0]))
+        x2 = torch.cat([y1, atlas], 1)
+        y2 = torch.relu_(self.layers[1].forward(x2, offsets, sites, hidden=hidden[1]))
+        z = self.layers[2].forward(y2, offsets, sites, hidden=hidden[2])
+        return z, (x1, y1, x2, y2, hidden)
+
+    def logits(self, features, atlas, offsets, sites):
+        """[rows, 15] for features [rows, 540] (Net.features) and prior rows [rows, 15]; requests as in Projection.forward."""
+        return self._forward(features, atlas, offsets, sites, False)[0]
+
+    def loss_and_gradients(self, features, atlas, y, offsets, sites, grads=None):
+        """(mean cross-entropy as a device scalar, gradients in the order of self.tensors) for labels y int64 [rows]."""
+        torch = self._torch
+        z, (x1, y1, x2, y2, hidden) = self._forward(features, atlas, offsets, sites, True)
+        logp = torch.log_softmax(z, 1)
+        loss = -logp.gather(1, y[:, None]).mean()
+        dz = logp.exp()
+        dz.scatter_add_(1, y[:, None], torch.full_like(y, -1, dtype=torch.float32)[:, None])
+        dz /= max(1, z.shape[0])
+        g = grads if grads is not None else [torch.empty_like(t) for t in self.tensors]
+        dy2 = self.layers[2].backward(y2, dz, offsets, sites, hidden=hidden[2], da=g[4], db=g[5])[0].mul_(y2 > 0)
+        dx2 = self.layers[1].backward(x2, dy2, offsets, sites, hidden=hidden[1], da=g[2], db=g[3])[0]
+        dy1 = dx2[:, :y1.shape[1]] * (y1 > 0)
+        self.layers[0].backward(x1, dy1, offsets, sites, hidden=hidden[0], da=g[0], db=g[1], want=('da', 'db'))
+        return loss, g

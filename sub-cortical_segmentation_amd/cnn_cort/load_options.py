@@ -53,6 +53,13 @@ def load_options(user_config):
         options['fwd_split'] = user_config.get('model', 'fwd_split').strip()      # 'True': inference on the split kernels (nets.py)
     if user_config.has_option('model', 'fit_split'):
         options['fit_split'] = user_config.get('model', 'fit_split').strip()      # 'True': fit()'s forward conv1 + conv2 block on the split kernels
+    if user_config.has_option('model', 'optimizer'):
+        options['optimizer'] = user_config.get('model', 'optimizer').strip()      # 'adam' (the reference's) or 'adamw'
+    for key in ('weight_decay', 'max_norm'):
+        if user_config.has_option('model', key):
+            options[key] = user_config.getfloat('model', key)
+    if user_config.has_option('model', 'optimizer_bits'):
+        options['optimizer_bits'] = user_config.getint('model', 'optimizer_bits')
     return options
 
 

@@ -114,7 +114,8 @@ class Net:
 
     def __init__(self, weights_file=None, history_file=None, max_epochs=100, patience=20, eval_size=0.25,
                  batch_size=128, verbose=0, device=None, update_learning_rate=0.001, seed=0, augment=False,
-                 fit_slice=16384, fit_resident_bytes=2 << 30, fwd_split=False, fit_split=False):
+                 fit_slice=16384, fit_resident_bytes=2 << 30, fwd_split=False, fit_split=False, optimizer='adam',
+                 weight_decay=0.01, optimizer_bits=32, max_norm=None):
         self.augment = bool(augment)
         # inference (predict / predict_proba / test_scan's patch entries) on the split kernels: convolutions on the f16 matrix cores
         # with every f32 operand as two f16 pieces, f32-grade results at ~2x the rate (csrc/conv_split.h; option fwd_split of libscs)
@@ -132,6 +133,13 @@ class Net:
         self.batch_size = int(batch_size)
         self.verbose = int(verbose)
         self.update_learning_rate = float(update_learning_rate)
+        # optimizer 'adam': lasagne.updates.adam (nets.py:236-237); 'adamw': decoupled weight decay on the weight matrices, moments in 32 or
+        # 8 bits, gradients clipped at max_norm (cnn_cort/optim.py)
+        if optimizer not in ('adam', 'adamw'):
+            raise ValueError("optimizer must be 'adam' or 'adamw', got %r" % (optimizer,))
+        self.optimizer, self.weight_decay = optimizer, float(weight_decay)
+        self.optimizer_bits, self.max_norm = int(optimizer_bits), None if max_norm is None else float(max_norm)
+        self.adapters = None         # SiteAdapters (fit_adapters, load_adapters_from)
         self.seed = int(seed)
         self.device = device
         self.train_history_ = []
@@ -322,13 +330,153 @@ class Net:
             probs[lo:hi] = d_probs.cpu().numpy()
         labels[lo:hi] = d_lab.cpu().numpy()
 
-    def predict_proba(self, X):
-        """float32 [N,15] softmax outputs (deterministic forward) - base.py:435-438."""
-        return self._forward(X, True)[0]
+    def predict_proba(self, X, sites=None):
+        """float32 [N,15] softmax outputs (deterministic forward) - base.py:435-438.  sites: None, or the site of every sample (one
+        integer, or [N]; -1 = the shared weights alone) whose adapters the dense head takes (fit_adapters)."""
+        return self._forward(X, True)[0] if sites is None else self._forward_sites(X, sites)[0]
 
-    def predict(self, X):
+    def predict(self, X, sites=None):
         """int64 [N] = argmax(predict_proba) - base.py:425-428 (nolearn, use_label_encoder=False)."""
-        return self._forward(X, False)[1]
+        return self._forward(X, False)[1] if sites is None else self._forward_sites(X, sites)[1]
+
+    # ------------------------------------------------------------------ site adapters
+    def features(self, X):
+        """float32 [N,540] on the device: the dense head's input (the towers' d1 outputs side by side, nets.py:215)."""
+        torch = self._torch()
+        n = self._check_X(X)
+        h = self._ensure_handle()
+        out = torch.empty((n, 540), dtype=torch.float32, device='cuda:%d' % self._dev())
+        stream = torch.cuda.current_stream(self._dev()).cuda_stream
+        for lo, hi, (ax, co, sa, at) in self._device_slices(X, n):
+            h.forward_features(ax, co, sa, at, hi - lo, out[lo:hi], stream)
+        return out
+
+    @staticmethod
+    def _check_sites(sites, n, count):
+        sites = np.asarray(sites)
+        if sites.dtype.kind not in 'iu':
+            raise ValueError('sites must be integers')
+        sites = np.full((n,), int(sites), np.int64) if sites.ndim == 0 else sites.astype(np.int64)
+        if sites.shape != (n,):
+            raise ValueError('sites has shape %r for %d samples' % (sites.shape, n))
+        if n and (sites.min() < -1 or sites.max() >= count):
+            raise ValueError('sites must lie in -1..%d' % (count - 1))
+        return sites
+
+    def _atlas_rows(self, X):
+        torch = self._torch()
+        a = X['in4']
+        t = torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)) if isinstance(a, np.ndarray) else a
+        return t.to(device='cuda:%d' % self._dev(), dtype=torch.float32).contiguous()
+
+    def _forward_sites(self, X, sites):
+        from .adapters import group_rows
+        torch = self._torch()
+        if self.adapters is None:
+            raise RuntimeError('no site adapters: fit_adapters or load_adapters_from first')
+        n = self._check_X(X)
+        sites = self._check_sites(sites, n, self.adapters.sites)
+        order, offsets, ids = group_rows(sites)
+        dev = self.adapters.device
+        back = torch.from_numpy(order).to(dev)
+        feat, atlas = self.features(X)[back], self._atlas_rows(X)[back]
+        z = self.adapters.logits(feat, atlas, torch.from_numpy(offsets).to(dev), torch.from_numpy(ids).to(dev))
+        probs = torch.empty_like(z)
+        probs[back] = torch.softmax(z, 1)
+        return probs.cpu().numpy(), probs.argmax(1).cpu().numpy().astype(np.int64)
+
+    def fit_adapters(self, X, y, sites, n_sites=None, rank=8, scale=1.0, epochs=None, learning_rate=None):
+        """Train low-rank adapters of the dense head (FC1, fc_2, out_layer) for every site, the shared weights and the towers fixed: what
+        a net that is trained once needs to follow several scanners.  sites: int [N], the site of every sample (0..n_sites-1; -1 = trains
+        no adapter).  The training loop is fit's (stratified hold-out of eval_size, consecutive mini-batches of batch_size, early stopping
+        after `patience` epochs, the best epoch's adapters are kept); the optimiser is AdamW with the Net's weight_decay, optimizer_bits
+        and max_norm.  One process.  Returns the history (epoch, train_loss, valid_loss); predict(X, sites=...) uses the adapters."""
+        from . import dist
+        from .adapters import SiteAdapters, group_rows
+        from .optim import AdamW
+        torch = self._torch()
+        if dist.is_dist() and dist.world_size() > 1:
+            raise RuntimeError('fit_adapters runs in one process')
+        n = self._check_X(X)
+        y = np.asarray(y).astype(np.int64)
+        if y.shape != (n,) or (n and (y.min() < 0 or y.max() > 14)):
+            raise ValueError('y must be %d labels in 0..14' % n)
+        sites_in = np.asarray(sites)
+        count = int(n_sites) if n_sites is not None else int(sites_in.max()) + 1 if sites_in.size else 0
+        if count < 1:
+            raise ValueError('fit_adapters needs at least one site')
+        sites = self._check_sites(sites_in, n, count)
+        h = self._ensure_handle()
+        self._sync_host()
+        ad = SiteAdapters(h, self._params, count, rank=rank, scale=scale, seed=self.seed)
+        dev = ad.device
+        feat, atlas, labels = self.features(X), self._atlas_rows(X), torch.from_numpy(y).to(dev)
+        if self.eval_size and self.eval_size > 0:
+            tr, va = stratified_first_fold(y, int(round(1.0 / self.eval_size)))
+        else:
+            tr, va = np.arange(n), np.arange(0)
+
+        def batches(rows):
+            out = []
+            for lo in range(0, len(rows), self.batch_size):
+                b = rows[lo:lo + self.batch_size]
+                order, offsets, ids = group_rows(sites[b])               # a mini-batch is a sum: its rows may come site by site
+                out.append((torch.from_numpy(b[order]).to(dev), torch.from_numpy(offsets).to(dev), torch.from_numpy(ids).to(dev)))
+            return out
+
+        train, valid = batches(tr), batches(va)
+        opt = AdamW(h, ad.tensors, lr=self.update_learning_rate if learning_rate is None else learning_rate, weight_decay=self.weight_decay,
+                    state_bits=self.optimizer_bits, max_norm=self.max_norm)
+        grads = [torch.empty_like(t) for t in ad.tensors]
+        opt.bind(grads)
+        history, best, best_epoch, best_state = [], np.inf, 0, None
+        for epoch in range(1, (epochs or self.max_epochs) + 1):
+            total = torch.zeros((), device=dev)
+            for rows, offsets, ids in train:
+                loss, _ = ad.loss_and_gradients(feat[rows], atlas[rows], labels[rows], offsets, ids, grads)
+                opt.step()
+                total += loss * rows.numel()
+            held = torch.zeros((), device=dev)
+            for rows, offsets, ids in valid:
+                logp = torch.log_softmax(ad.logits(feat[rows], atlas[rows], offsets, ids), 1)
+                held -= logp.gather(1, labels[rows][:, None]).sum()
+            info = {'epoch': epoch, 'train_loss': float(total) / max(1, len(tr)), 'valid_loss': float(held) / len(va) if len(va) else 0.0}
+            history.append(info)
+            if self.verbose:
+                print('{:>7}  {:>10.5f}  {:>10.5f}'.format(epoch, info['train_loss'], info['valid_loss']))
+            watched = info['valid_loss'] if len(va) else info['train_loss']
+            if watched < best:
+                best, best_epoch, best_state = watched, epoch, [t.clone() for t in ad.tensors]
+            elif epoch - best_epoch >= self.patience:
+                break
+        if best_state is not None:
+            for t, b in zip(ad.tensors, best_state):
+                t.copy_(b)
+        opt.close()
+        self.adapters = ad
+        return history
+
+    def save_adapters_to(self, path):
+        """The site adapters as an .npz of plain arrays."""
+        if self.adapters is None:
+            raise RuntimeError('no site adapters to save')
+        with open(path, 'wb') as f:
+            np.savez(f, **self.adapters.state_dict())
+        return path
+
+    def load_adapters_from(self, path):
+        """Site adapters saved by save_adapters_to, beside this Net's weights."""
+        from .adapters import SiteAdapters
+        with np.load(path, allow_pickle=False) as d:
+            state = {k: d[k] for k in d.files}
+        want = {'scale'} | {'%s.%s' % (l, k) for l in SiteAdapters.LAYERS for k in 'ab'}
+        if set(state) != want:
+            raise ValueError('%s is not a file of site adapters' % (path,))
+        h = self._ensure_handle()
+        self._sync_host()
+        sites, rank = state['FC1.a'].shape[:2]
+        self.adapters = SiteAdapters(h, self._params, sites, rank=rank, state=state)
+        return self
 
     def _wait(self, stream=None):
         """Sleep (not spin) until the work queued on `stream` (default: the current one) is done: the event is polled between
@@ -763,7 +911,8 @@ class Net:
             print('-------  ----------  ----------  ---------  -----------  -----')
         # one rank: nothing sits between a step's gradients and their update, so the step applies lasagne.updates.adam itself,
         # group by group as the gradients become final (scs_set_fused_adam: same arithmetic, no launch behind the step)
-        fused = not dist.is_dist()
+        adamw = self._adamw(h) if self.optimizer == 'adamw' else None
+        fused = adamw is None and not dist.is_dist()
         h.set_fused_adam(fused, lr=self.update_learning_rate)
         try:
             for ep in range(epochs or self.max_epochs):
@@ -785,7 +934,11 @@ class Net:
                         sizes.append(nb)
                     if not fused:
                         scale = dist.allreduce_grads(h, active, stream, n_active=dist.active_ranks(len(starts), step, world))
-                        h.adam_apply(lr=self.update_learning_rate, grad_scale=scale, stream=stream)
+                        if adamw is None:
+                            h.adam_apply(lr=self.update_learning_rate, grad_scale=scale, stream=stream)
+                        else:
+                            adamw.step(grad_scale=scale)
+                            h.param_arena()                        # (tells the handle that its parameters have changed)
                 losses = loss_buf[:len(sizes)].cpu().numpy().astype(np.float64)
                 self._dev_newer = True
                 dist.sync_params(h)            # reconcile per-rank BN running statistics (no-op on one GPU)
@@ -821,9 +974,29 @@ class Net:
             pass
         finally:
             h.set_fused_adam(False)            # the handle goes back to the two-call form (scs_train_step, scs_adam_apply)
+            if adamw is not None:
+                adamw.close()
             if not compact:
                 pool.shutdown(wait=False)
         return self
+
+    def _adamw(self, h):
+        """AdamW over the trained arrays of the parameter arena (batch-norm mean and inv_std are running statistics); weight decay on
+        the convolution and dense weights alone."""
+        from . import dist
+        from .optim import AdamW
+        dev = self._dev()
+        p, g = dist.wrap_device_floats(*h.param_arena(), dev), dist.wrap_device_floats(*h.grad_arena(), dev)
+        params, grads, decays, at = [], [], [], 0
+        for name, shapes in P.LAYER_SPEC:
+            for i, shape in enumerate(shapes):
+                n = int(np.prod(shape))
+                if P.is_trainable(name, i):
+                    params.append(p[at:at + n])
+                    grads.append(g[at:at + n])
+                    decays.append(self.weight_decay if len(shape) > 1 else 0.0)
+                at += n
+        return AdamW(h, params, lr=self.update_learning_rate, weight_decay=decays, state_bits=self.optimizer_bits, max_norm=self.max_norm).bind(grads)
 
     def _train_batch(self, h, views, atl, yy, nb, seed, stream, aug_rng, rank):
         if self.augment and nb > 1:
@@ -875,7 +1048,9 @@ def build_model(weights_path, options):
               max_epochs=options['max_epochs'], patience=options['patience'], eval_size=options['train_split'],
               batch_size=options.get('batch_size') or 128, verbose=options['net_verbose'],
               device=options.get('device'), augment=is_true(options.get('augment')),
-              seed=int(options.get('seed') or 0), fwd_split=is_true(options.get('fwd_split')), fit_split=is_true(options.get('fit_split')))
+              seed=int(options.get('seed') or 0), fwd_split=is_true(options.get('fwd_split')), fit_split=is_true(options.get('fit_split')),
+              optimizer=options.get('optimizer') or 'adam', weight_decay=float(options.get('weight_decay', 0.01)),
+              optimizer_bits=int(options.get('optimizer_bits') or 32), max_norm=options.get('max_norm'))
     if is_true(options['load_weights']):
         if net.verbose:
             print("    --> loading weights from ", net_weights)

@@ -1185,6 +1185,29 @@ int scs_forward(scs_handle h, const float* ax, const float* co, const float* sa,
     return forward_common(h, ax, co, sa, atlas, nullptr, 0, 0, 0, nullptr, nullptr, n, probs, labels, stream);
 }
 
+// the exact-f32 kernels chunk by chunk; the dense head's input is copied out before the next chunk writes over it (the head itself runs as well:
+// 4 % of the arithmetic)
+int scs_forward_features(scs_handle h, const float* ax, const float* co, const float* sa, const float* atlas, int64_t n, float* features, void* stream) {
+    SCS_ARG(h != nullptr, "null handle");
+    SCS_ARG(n >= 0, "n < 0");
+    SCS_ARG(n == 0 || (ax && co && sa && atlas && features), "null pointer");
+    if (!h->has_params) { set_error("scs_forward_features before scs_set_params"); return SCS_ERR_STATE; }
+    if (n == 0) return SCS_OK;
+    SCS_HIP(hipSetDevice(h->device));
+    const int step = balanced_chunk(n, h->chunk);
+    int rc = ensure_workspace(h, step);
+    if (rc != SCS_OK) return rc;
+    hipStream_t st = (hipStream_t)stream;
+    if (h->packed_dirty) { rc = repack_inference(h, st); if (rc != SCS_OK) return rc; h->packed_dirty = false; }
+    for (int64_t s = 0; s < n; s += step) {
+        const int m = (int)std::min<int64_t>(n - s, step);
+        rc = forward_chunk(h, ax + s * 1024, co + s * 1024, sa + s * 1024, atlas + s * 15, nullptr, 0, 0, 0, nullptr, nullptr, m, nullptr, nullptr, st, nullptr, nullptr, nullptr, kFwdF32);
+        if (rc != SCS_OK) return rc;
+        SCS_HIP(hipMemcpyAsync(features + s * kFlat, h->a_feat, (size_t)m * kFlat * sizeof(float), hipMemcpyDeviceToDevice, st));
+    }
+    return SCS_OK;
+}
+
 int scs_forward_volume(scs_handle h, const float* vol, int dx, int dy, int dz, const int32_t* centers,
                        const float* atlas4d, int64_t n, float* probs, int32_t* labels, void* stream) {
     SCS_ARG(n == 0 || (vol && centers && atlas4d), "null input pointer");

@@ -144,3 +144,200 @@ CASES = {
 def test_against_float64(handle, case, t):
     rows, n_in, n_out, rank, adapters, off, ids = CASES[case]
     check_all(handle, data(t, rows, n_in, n_out, rank, adapters, len(case) + rows, bias=rows % 2 == 0), off, ids, t, with_hidden=rows % 3 != 0)
+
+
+def some(t, rows=700, n_in=96, n_out=200, rank=8, adapters=3, seed=3):
+    d = data(t, rows, n_in, n_out, rank, adapters, seed)
+    return d, [0, 15, rows // 2, rows], [2, -1, 0]
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+@pytest.mark.parametrize('rows', [20, 700])
+@pytest.mark.parametrize('shift', [0, 1, 8])
+def test_strides_and_alignments(handle, t, rows, shift):
+    """Every matrix as a view inside a larger one, `shift` elements off its start; what lies around the outputs stays."""
+    d, off, ids = some(t, rows)
+    o, i = requests(off, ids)
+
+    def inside(m, fill):
+        r, c = m.shape
+        big = torch.full((r + 2, c + 24), fill, dtype=m.dtype, device='cuda:0')
+        big[1:r + 1, shift:shift + c] = m
+        return big, big[1:r + 1, shift:shift + c]
+
+    w = inside(d['w'], 9.0)[1]
+    x, dy = inside(d['x'], float('nan'))[1], inside(d['dy'], float('nan'))[1]
+    p = Projection(handle, w, d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    q = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    yb, y = inside(torch.zeros((rows, 200), dtype=TYPES[t], device='cuda:0'), 4.0)
+    db_, dx = inside(torch.zeros((rows, 96), dtype=TYPES[t], device='cuda:0'), 4.0)
+    p.forward(x, o, i, out=y)
+    assert torch.equal(y, q.forward(d['x'], o, i))
+    _, da, db = p.backward(x, dy, o, i, dx=dx)
+    ref = q.backward(d['x'], d['dy'], o, i)
+    assert torch.equal(dx, ref[0]) and torch.equal(da, ref[1]) and torch.equal(db, ref[2])
+    for big, part in ((yb, y), (db_, dx)):
+        part.fill_(4.0)
+        assert (big == 4.0).all()
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('rows', [40, 700])
+def test_what_is_not_finite_stays_with_its_own(handle, t, rows):
+    """An adapter of infinities, a row of NaN and NaN behind the last request touch their own rows (and gradients) alone."""
+    d, off, ids = some(t, rows)
+    clean = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    o, i = requests(off[:-1] + [rows - 5], ids)
+    y0 = clean.forward(d['x'], o, i)
+    g0 = clean.backward(d['x'], d['dy'], o, i)
+    a = d['a'].clone()
+    b = d['b'].clone()
+    a[2], b[2] = float('inf'), float('nan')                  # the first request's: rows 0..14
+    x, dy = d['x'].clone(), d['dy'].clone()
+    x[20], dy[20] = float('nan'), float('nan')                # a row of the request without an adapter (there is none at 20 rows of 40)
+    x[rows - 5:], dy[rows - 5:] = float('nan'), float('nan')
+    p = Projection(handle, d['w'], a, b, bias=d['bias'], scale=d['scale'])
+    y = p.forward(x, o, i)
+    g = p.backward(x, dy, o, i)
+    keep = torch.ones(rows, dtype=torch.bool, device='cuda:0')
+    keep[:15] = False
+    keep[20] = False
+    assert torch.equal(y[keep], y0[keep]) and torch.equal(g[0][keep], g0[0][keep])
+    if rows == 700:                                          # row 20 has no adapter: adapter 0's gradients do not see it
+        assert torch.equal(g[1][0], g0[1][0]) and torch.equal(g[2][0], g0[2][0])
+    assert torch.equal(g[1][1], torch.zeros_like(g[1][1]))
+    assert not torch.isfinite(y[:15].float()).any() and (y[rows - 5:] == 0).all()
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+@pytest.mark.parametrize('rows,n_in', [(9, 1024), (33, 2048), (700, 96), (2048, 128)])
+def test_captured_calls_replay(handle, t, rows, n_in):
+    """Forward and backward in one graph, replayed with new inputs between eager work, against eager calls."""
+    d, off, ids = some(t, rows, n_in)
+    off[1] = min(off[1], rows // 2)
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    y, hid = torch.zeros((rows, 200), dtype=TYPES[t], device='cuda:0'), torch.zeros((rows, 8), device='cuda:0')
+    dx, da, db = torch.zeros_like(d['x']), torch.zeros(d['a'].shape, device='cuda:0'), torch.zeros(d['b'].shape, device='cuda:0')
+    p.forward(d['x'], o, i, out=y, hidden=hid)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.forward(d['x'], o, i, out=y, hidden=hid)
+        p.backward(d['x'], d['dy'], o, i, hidden=hid, dx=dx, da=da, db=db)
+    for k in range(4):
+        fresh = data(t, rows, n_in, 200, 8, 3, 50 + k)
+        for key in ('x', 'dy', 'w', 'a', 'b'):
+            d[key].copy_(fresh[key])
+        graph.replay()
+        e = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+        hid2 = torch.zeros_like(hid)
+        y2 = e.forward(d['x'], o, i, hidden=hid2)
+        dx2, da2, db2 = e.backward(d['x'], d['dy'], o, i, hidden=hid2)
+        torch.cuda.synchronize()
+        for a_, b_ in ((y, y2), (hid, hid2), (dx, dx2), (da, da2), (db, db2)):
+            assert torch.equal(a_, b_), 'replay %d' % k
+
+
+def test_two_streams_and_two_threads_at_once(handle):
+    import threading
+    d, off, ids = some('bf16', 48, 2048)
+    off[1] = 15
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'], scale=d['scale'])
+    want = p.forward(d['x'], o, i)
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                outs = [p.forward(d['x'], o, i) for _ in range(20)]
+                torch.cuda.current_stream().synchronize()
+                got[k] = outs
+        except Exception as e:          # surfaced below
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(3)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    assert all(torch.equal(y, want) for outs in got.values() for y in outs)
+
+
+def test_hidden_may_be_formed_again(handle):
+    for rows in (60, 700):
+        d, off, ids = some('bf16', rows)
+        o, i = requests(off, ids)
+        p = Projection(handle, d['w'], d['a'], d['b'], scale=d['scale'])
+        hid = torch.empty((rows, 8), device='cuda:0')
+        p.forward(d['x'], o, i, hidden=hid)
+        a, b = p.backward(d['x'], d['dy'], o, i, hidden=hid), p.backward(d['x'], d['dy'], o, i)
+        assert all(torch.equal(s, t) for s, t in zip(a, b))
+        for want in (('dx',), ('da',), ('db',), ('da', 'db')):
+            c = p.backward(d['x'], d['dy'], o, i, want=want)
+            for k, s, t in zip(('dx', 'da', 'db'), a, c):
+                assert (t is None) if k not in want else torch.equal(s, t)
+
+
+def test_offsets_out_of_order_stay_inside(handle):
+    """Offsets are read on the device and clamped to the rows: wrong ones give wrong rows, and nothing around the outputs changes."""
+    for t in ('f32', 'bf16'):
+        for rows in (50, 700):
+            d, _, _ = some(t, rows)
+            p = Projection(handle, d['w'], d['a'], d['b'])
+            for off in ([rows, 5, 0, 3], [-7, 20, 2 * rows, 10 ** 9], [0, -2 ** 31, 2 ** 31 - 1, 9]):
+                o, i = requests(off, [0, 1, 2])
+                big = torch.full((rows + 4, 200), 2.0, dtype=TYPES[t], device='cuda:0')
+                bdx = torch.full((rows + 4, 96), 2.0, dtype=TYPES[t], device='cuda:0')
+                p.forward(d['x'], o, i, out=big[2:rows + 2])
+                p.backward(d['x'], d['dy'], o, i, dx=bdx[2:rows + 2])
+                torch.cuda.synchronize()
+                for b in (big, bdx):
+                    assert (b[:2] == 2.0).all() and (b[rows + 2:] == 2.0).all()
+
+
+@pytest.mark.parametrize('ld', [2097152, 2100000])
+def test_row_offsets_beyond_32_bits(handle, ld):
+    rows, n_in, n_out = 1100, 64, 72
+    d, off, ids = some('bf16', rows, n_in, n_out)
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    store = torch.empty((rows * ld,), dtype=torch.bfloat16, device='cuda:0')           # 4.6 GB
+    x = torch.as_strided(store, (rows, n_in), (ld, 1))
+    y = torch.as_strided(store, (rows, n_out), (ld, 1), 1024)
+    x.copy_(d['x'])
+    xin = x.clone()
+    with pytest.raises(ValueError, match='shares memory'):
+        p.forward(x, o, i, out=y)                                                          # (interleaved views count as shared)
+    other = torch.empty((rows * ld,), dtype=torch.bfloat16, device='cuda:0')
+    y = torch.as_strided(other, (rows, n_out), (ld, 1), 1024)
+    p.forward(x, o, i, out=y)
+    assert torch.equal(y, p.forward(xin, o, i))
+    dy = y
+    dx = torch.as_strided(store, (rows, n_in), (ld, 1), 512)
+    g = p.backward(xin, dy, o, i, dx=dx)
+    ref = p.backward(xin, dy.contiguous(), o, i)
+    assert all(torch.equal(a, b) for a, b in zip(g, ref))
+
+
+def test_refusals(handle):
+    d, off, ids = some('bf16')
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    x = d['x']
+    bad = [lambda: p.forward(x.float(), o, i), lambda: p.forward(x[:, :95], o, i), lambda: p.forward(x.t(), o, i), lambda: p.forward(x.cpu(), o, i),
+           lambda: p.forward(x, o[:-1], i), lambda: p.forward(x, o.long(), i), lambda: p.forward(x, o, i, out=x), lambda: p.forward(x[0], o, i),
+           lambda: p.forward(x, o, i, hidden=torch.empty((3, 8), device='cuda:0')), lambda: p.backward(x, d['dy'], o, i, want=()),
+           lambda: p.backward(x, d['dy'], o, i, want=('dw',)), lambda: p.backward(x, d['dy'], o, i, da=torch.empty((3, 8, 95), device='cuda:0')),
+           lambda: p.backward(x, d['dy'][:9], o, i), lambda: p.backward(x, d['dy'], o, i, dx=x),
+           lambda: Projection(handle, d['w'].double(), d['a'], d['b']), lambda: Projection(handle, d['w'], d['a'], d['b'][:2]),
+           lambda: Projection(handle, d['w'], d['a'].transpose(0, 1), d['b'].transpose(0, 1)), lambda: Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'][:-1]),
+           lambda: Projection(handle, d['w'], d['a'], d['b'], scale=d['scale'].half()),
+           lambda: Projection(handle, d['w'], d['a'].new_zeros((3, 129, 96)), d['b'].new_zeros((3, 129, 200)))]
+    for k, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            raise AssertionError('call %d was accepted' % k)
