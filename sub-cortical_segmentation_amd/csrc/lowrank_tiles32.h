@@ -3,7 +3,7 @@
 //
 // What bounds it: v_mfma_f32_16x16x4_f32, 32 cycles each on the vector ALUs, which every other vector instruction takes time from: so the copies
 // go to LDS without passing registers and addresses are a uniform base and a fixed offset a lane.  A workgroup of four waves owns
-// 128 rows x 16 NT columns (32 rows a wave), two workgroups a CU; NT is chosen for the least padding (540 columns: 5 x 112).
+// 64 MT rows x 16 NT columns (16 MT rows a wave), two workgroups a CU; NT is chosen for the least padding (540 columns: 5 x 112).
 // LDS images of a slab of 16 along the contraction, in 16-byte pieces:
 //   K-major [row][16]: piece c of a row at c ^ (row >> 2 & 3); a lane's piece is its operand of four products.  X, and W^T in the backward pass
 //   N-major [16][BN]:  column n of row k at (n + 16 (k >> 2)) mod BN, so that a fragment's four rows lie at different banks.  W, and P
@@ -18,9 +18,9 @@ __device__ __forceinline__ void copy_to_lds(const void* src, unsigned int lds) {
 }
 
 // EVEN: N is a multiple of 4
-template <int NT, bool TRANS, bool EVEN>
+template <int MT, int NT, bool TRANS, bool EVEN>
 __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<float> g) {
-    constexpr int BM = 128, BN = 16 * NT, BK = 16, STAGES = 4, NP = BN / 4, LOADS = 4;
+    constexpr int BM = 64 * MT, BN = 16 * NT, BK = 16, STAGES = 4, NP = BN / 4, LOADS = MT + 2;
     __shared__ __attribute__((aligned(16))) float s_a[STAGES][BM * BK];
     __shared__ __attribute__((aligned(16))) float s_b[STAGES][512 * 4];           // (BN <= 128; what lies behind a slab's end is never read)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -42,11 +42,12 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
     const float* base_a = g.x + (int64_t)m0 * g.ldx;
     const float* base_b = TRANS ? g.w + (int64_t)n0 * g.ldw : g.w + n0;
     const int64_t step_b = TRANS ? BK : BK * g.ldw;
-    unsigned int oa[2], ob[2];
+    unsigned int oa[MT], ob[2];
     int kb[2];                                              // contraction index of the thread's piece of W'
 #pragma unroll
+    for (int i = 0; i < MT; ++i) oa[i] = (unsigned int)(min((tid >> 2) + i * 64, r.rows - 1 - m0) * (int)g.ldx + pa * 4) * 4u;
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
-        oa[i] = (unsigned int)(min((tid >> 2) + i * 64, r.rows - 1 - m0) * (int)g.ldx + pa * 4) * 4u;
         if constexpr (TRANS) {
             kb[i] = pa * 4;
             ob[i] = (unsigned int)(min((tid >> 2) + i * 64, g.N - 1 - n0) * (int)g.ldw + pa * 4) * 4u;
@@ -64,34 +65,34 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
         const float* b = base_b + s * step_b;
         const unsigned int la = lds_a + (s % STAGES) * (BM * BK * 4), lb = lds_b + (s % STAGES) * 8192;
         if ((s + 1) * BK <= g.K) {
-            copy_to_lds(a, oa[0], la);
-            copy_to_lds(a, oa[1], la + 4096);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) copy_to_lds(a, oa[i], la + i * 4096);
             copy_to_lds(b, ob[0], lb);
             copy_to_lds(b, ob[1], lb + 4096);
         } else {
             const char* zero = (const char*)&kZeroPiece;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) copy_to_lds(s * BK + pa * 4 < g.K ? (const char*)a + oa[i] : zero, la + i * 4096);
+            for (int i = 0; i < MT; ++i) copy_to_lds(s * BK + pa * 4 < g.K ? (const char*)a + oa[i] : zero, la + i * 4096);
 #pragma unroll
             for (int i = 0; i < 2; ++i) copy_to_lds(s * BK + kb[i] < g.K ? (const char*)b + ob[i] : zero, lb + i * 4096);
         }
     };
 
-    f32x4 acc[2][NT];
+    f32x4 acc[MT][NT];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int t = 0; t < NT; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    const int ax = (wave * 32 + lr) * BK + (kq ^ (lr >> 2)) * 4, bx = lr * BK + (kq ^ (lr >> 2)) * 4;
+    const int ax = (wave * 16 * MT + lr) * BK + (kq ^ (lr >> 2)) * 4, bx = lr * BK + (kq ^ (lr >> 2)) * 4;
     int bn[NT];                                             // N-major: row 4 kq of column tile t
 #pragma unroll
     for (int t = 0; t < NT; ++t) bn[t] = 4 * kq * BN + ((t + kq) % NT) * 16 + lr;
-    auto read = [&](int s, f32x4 (&x)[2], f32x4 (&w)[NT]) {
+    auto read = [&](int s, f32x4 (&x)[MT], f32x4 (&w)[NT]) {
         const float* a = s_a[s % STAGES];
         const float* b = s_b[s % STAGES];
-        x[0] = *(const f32x4*)(a + ax);
-        x[1] = *(const f32x4*)(a + ax + 16 * BK);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) x[i] = *(const f32x4*)(a + ax + i * 16 * BK);
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             if constexpr (TRANS) w[t] = *(const f32x4*)(b + bx + t * 16 * BK);
@@ -100,24 +101,24 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
                 for (int j = 0; j < 4; ++j) w[t][j] = b[bn[t] + j * BN];
         }
     };
-    auto multiply = [&](const f32x4 (&x)[2], const f32x4 (&w)[NT]) {
+    auto multiply = [&](const f32x4 (&x)[MT], const f32x4 (&w)[NT]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[t][j], x[i][j], acc[i][t], 0, 0, 0);
+                for (int i = 0; i < MT; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[t][j], x[i][j], acc[i][t], 0, 0, 0);
     };
     auto spread = [&] {
-        constexpr int READS = 2 + (TRANS ? NT : 4 * NT), EACH = 8 * NT / READS;
+        constexpr int READS = MT + (TRANS ? NT : 4 * NT), ALL = 4 * MT * NT, EACH = ALL / READS;
 #pragma unroll
         for (int i = 0; i < READS; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+            if constexpr (EACH) __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
         }
-        __builtin_amdgcn_sched_group_barrier(0x008, 8 * NT - EACH * READS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, ALL - EACH * READS, 0);
     };
-    f32x4 x0[2], x1[2], w0[NT], w1[NT];
+    f32x4 x0[MT], x1[MT], w0[NT], w1[NT];
     const int slabs = (g.K + BK - 1) / BK;
 #pragma unroll
     for (int s = 0; s < STAGES; ++s) fetch(s);
@@ -142,7 +143,7 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
     workgroup_barrier();
 
     // the adapters: 16 directions a pass, each request under the mask of its rows
-    const int m1 = min(m0 + BM, r.rows), mw = m0 + wave * 32;
+    const int m1 = min(m0 + BM, r.rows), mw = m0 + wave * 16 * MT;
     Walk walk(r, m0, m1);
     int q;
     Span sp;
@@ -167,19 +168,23 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
                 *(f32x4*)&s_b[0][k * BN + (c + 4 * (k >> 2)) % NP * 4] = j0 + k < r.rank ? v : z;
             }
             __syncthreads();
-            const f32x4 x[2] = {*(const f32x4*)(s_a[0] + ax), *(const f32x4*)(s_a[0] + ax + 16 * BK)};
+            f32x4 x[MT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i) x[i] = *(const f32x4*)(s_a[0] + ax + i * 16 * BK);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                f32x4 part[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+                f32x4 part[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) part[i] = f32x4{0.f, 0.f, 0.f, 0.f};
                 const int at = 4 * kq * BN + ((t + kq) % NT) * 16 + lr;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float w = s_b[0][at + j * BN];
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) part[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x[i][j], part[i], 0, 0, 0);
+                    for (int i = 0; i < MT; ++i) part[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(w, x[i][j], part[i], 0, 0, 0);
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < MT; ++i) {
                     const int row = mw + i * 16 + lr;
                     const bool in = row >= sp.lo && row < sp.hi;
 #pragma unroll
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<flo
 
     const int live_lo = clamp_row(r.offsets[0], r.rows), live_hi = clamp_row(r.offsets[r.n], r.rows);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < MT; ++i) {
         const int row = mw + i * 16 + lr;
         if (row < live_lo || row >= live_hi) continue;
 #pragma unroll

@@ -473,10 +473,27 @@ int wgrad_block_rows(const scs_lowrank& p) {
 
 // ---- few rows (lowrank_few.h)
 struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; int tickets = 0; };      // mt 0: the tile kernels
+// f32 tiles (lowrank_tiles32.h): columns / 16 of the tile with the least padding, the widest among equals
+int f32_columns(int64_t N) {
+    int nt = 0;
+    int64_t waste = INT64_MAX;
+    for (const int n : {8, 7, 6, 5, 4}) {
+        const int64_t w = (N + 16 * n - 1) / (16 * n) * 16 * n;
+        if (w < waste) { waste = w; nt = n; }
+    }
+    return nt;
+}
+// ... and its rows / 64: the higher tile where that still gives every CU one, the lower where that gives most of them one, 0: neither does
+int f32_rows(int64_t rows, int64_t N) {
+    const int64_t across = (N + 16 * f32_columns(N) - 1) / (16 * f32_columns(N));
+    return (rows + 127) / 128 * across >= 256 ? 2 : (rows + 63) / 64 * across >= 192 ? 1 : 0;
+}
+// The few-rows form: up to 64 rows in 16 bits (128 rows at 4096 x 4096 take 28 us as tiles), in f32 wherever the tiles would leave CUs idle (512 rows
+// at 540 x 540: 18 us, as tiles 46)
 Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     Few f;
-    if (p.rows > (p.dtype == SCS_F32 ? 512 : 64)) return f;
-    f.mt = p.dtype == SCS_F32 ? 1 : (int)(p.rows + 15) / 16;
+    if (p.dtype == SCS_F32 ? f32_rows(p.rows, N) != 0 : p.rows > 64) return f;
+    f.mt = p.dtype == SCS_F32 ? (p.rows >= 256 && K * N >= (1 << 21) ? 2 : 1) : (int)(p.rows + 15) / 16;
     f.tiles_n = (int)((N + 63) / 64);
     f.tiles_m = (int)((p.rows + 16 * f.mt - 1) / (16 * f.mt));
     const int64_t steps = (K + 31) / 32;
@@ -585,10 +602,10 @@ template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, co
 template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
     const dim3 grid(f.tiles_n, f.tiles_m, f.splits);
     auto go = [&](auto mt) { hipLaunchKernelGGL((project_few_kernel<T, mt.value, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, rows, f.splits, part, tickets); };
-    if (sizeof(T) == 4 || f.mt == 1) go(std::integral_constant<int, 1>{});
+    if (f.mt == 1) go(std::integral_constant<int, 1>{});
+    else if (f.mt == 2) go(std::integral_constant<int, 2>{});
     else if constexpr (sizeof(T) == 2) {
-        if (f.mt == 2) go(std::integral_constant<int, 2>{});
-        else if (f.mt == 3) go(std::integral_constant<int, 3>{});
+        if (f.mt == 3) go(std::integral_constant<int, 3>{});
         else go(std::integral_constant<int, 4>{});
     }
 }
@@ -601,13 +618,11 @@ template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T
         else if (tiles(128, 128) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS, EVEN>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((project_tiles_kernel<T, 2, 2, 2, TRANS, EVEN>), dim3((unsigned)tiles(64, 64)), dim3(256), 0, st, g);
     } else {
-        // the column tile with the least padding, the widest among equals
-        int nt = 0, waste = 1 << 30;
-        for (const int n : {8, 7, 6, 5, 4}) {
-            const int w = (g.N + 16 * n - 1) / (16 * n) * 16 * n;
-            if (w < waste) { waste = w; nt = n; }
-        }
-        auto go = [&](auto n) { hipLaunchKernelGGL((project_tiles32_kernel<n.value, TRANS, EVEN>), dim3((unsigned)tiles(128, 16 * n.value)), dim3(256), 0, st, g); };
+        const int nt = f32_columns(g.N), mt = f32_rows(g.r.rows, g.N);
+        auto go = [&](auto n) {
+            if (mt == 2) hipLaunchKernelGGL((project_tiles32_kernel<2, n.value, TRANS, EVEN>), dim3((unsigned)tiles(128, 16 * n.value)), dim3(256), 0, st, g);
+            else hipLaunchKernelGGL((project_tiles32_kernel<1, n.value, TRANS, EVEN>), dim3((unsigned)tiles(64, 16 * n.value)), dim3(256), 0, st, g);
+        };
         if (nt == 8) go(std::integral_constant<int, 8>{});
         else if (nt == 7) go(std::integral_constant<int, 7>{});
         else if (nt == 6) go(std::integral_constant<int, 6>{});

@@ -132,6 +132,9 @@ CASES = {
     'tokens, long contractions': (48, 2000, 1111, 20, 5, list(range(49)), [i % 7 - 1 for i in range(48)]),
     'few rows above a tile': (61, 1033, 640, 8, 2, [0, 30, 60], [1, 0]),
     'many tiles': (3100, 264, 4104, 16, 3, [0, 100, 1500, 1501, 3000, 3090], [0, 1, 2, -1, 0]),
+    'low tiles': (2200, 132, 648, 8, 3, [0, 100, 900, 2200], [0, 1, 2]),
+    'low tiles, odd': (3000, 131, 517, 8, 3, [0, 100, 900, 3000], [0, 1, 2]),
+    'rows in between': (700, 2052, 1033, 8, 3, [0, 100, 300, 699], [0, 1, 2]),
     'medium tiles': (1500, 192, 2056, 16, 3, [0, 100, 900, 1500], [0, 1, 2]),
     'medium tiles, odd': (1600, 197, 2051, 9, 3, [0, 100, 900, 1600], [0, 1, 2]),
     'many tiles, odd': (3333, 131, 4099, 17, 3, [0, 1000, 2222, 3333], [2, 1, 0]),
