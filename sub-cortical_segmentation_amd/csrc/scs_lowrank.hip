@@ -79,18 +79,6 @@ struct Walk {
 // rows, each wave a share of the contraction, joined through LDS; operands go from global memory to the matrix cores without a stop (both are
 // contiguous along the contraction: a lane's 16 bytes are its operand of one 16-bit product or of four f32 ones, whose contraction
 // indices are permuted alike on both sides), four steps' loads in flight.
-template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
-template <class T> __device__ __forceinline__ u32x4 at16(const T* p) { return reinterpret_cast<const Loose<u32x4>*>(p)->v; }
-// 16 bytes of elements at any element alignment, zeros behind `left`
-template <class T> __device__ __forceinline__ u32x4 load16(const T* p, int64_t left) {
-    constexpr int N = 16 / sizeof(T);
-    if (left >= N) return at16(p);
-    T e[N] = {};
-    for (int i = 0; i < N - 1; ++i) if (i < left) e[i] = p[i];
-    u32x4 r;
-    __builtin_memcpy(&r, e, 16);
-    return r;
-}
 template <class T> __device__ __forceinline__ f32x4 product16(const u32x4& a, const u32x4& b, f32x4 c) {
     if constexpr (sizeof(T) == 4) {
         f32x4 x, y;

@@ -55,8 +55,22 @@ template <class T> __device__ __forceinline__ typename Vec4<T>::raw pack(const f
     return r;
 }
 
-// ---- operands of the 16-bit matrix cores
+// ---- vectors of elements at any element alignment
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+template <class T> __device__ __forceinline__ typename Vec4<T>::raw at4(const T* p) { return reinterpret_cast<const Loose<typename Vec4<T>::raw>*>(p)->v; }
+template <class T> __device__ __forceinline__ u32x4 at16(const T* p) { return reinterpret_cast<const Loose<u32x4>*>(p)->v; }
+// 16 bytes of elements at any element alignment, zeros behind `left`
+template <class T> __device__ __forceinline__ u32x4 load16(const T* p, int64_t left) {
+    constexpr int N = 16 / sizeof(T);
+    if (left >= N) return at16(p);
+    T e[N] = {};
+    for (int i = 0; i < N - 1; ++i) if (i < left) e[i] = p[i];
+    u32x4 r;
+    __builtin_memcpy(&r, e, 16);
+    return r;
+}
+
+// ---- operands of the 16-bit matrix cores
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 template <class T> struct Frag;
 template <> struct Frag<__bf16> { typedef __bf16 v8 __attribute__((ext_vector_type(8))); };

@@ -32,21 +32,22 @@ namespace {
 constexpr int kOptBlock = 256;             // elements that share a scale
 constexpr int kChunkBlocks = 16;           // blocks of one workgroup
 constexpr int kGradsPerLaunch = 384;       // gradient pointers that travel by value in one launch's arguments (at most 4 KB of them)
-constexpr int kNormGroups = 512;           // workgroups of the norm's first stage = partial sums in double
+constexpr int kNormGroups = 1024;          // workgroups of the norm's first stage = partial sums in double
 constexpr int kTickets = 64;               // leaves of the ticket tree, one 128-byte line each
 constexpr float kK127 = (float)(1.0 / 16129.0), kK255 = (float)(1.0 / 65025.0);
 
-struct OptTensor {
-    void* p;                 // parameter, `type`
-    float* master;           // f32 value of a 16-bit parameter, or null
-    int64_t n;
-    int64_t block0;          // its first block in the moment arenas
+// one workgroup's share of one tensor: up to kChunkBlocks blocks (64 bytes, one load)
+struct OptChunk {
+    void* p;                 // parameter at the chunk's first element
+    float* master;           // f32 value of a 16-bit parameter there, or null
+    int64_t block;           // first block in the moment arenas
+    int64_t first;           // first element, counted inside the tensor
     double wd;
-    int32_t type;
+    int32_t left;            // elements of the chunk
+    int32_t tensor;
+    int32_t type;            // of the parameter
     int32_t pad;
 };
-struct OptChunk { int32_t tensor, block; };      // first block of the chunk, counted inside the tensor
-
 struct OptState {            // device words of one optimiser
     int64_t step;            // steps taken
     double norm;             // of the last clipped step
@@ -63,7 +64,6 @@ struct GradArgs {
     int32_t tensor0;         // g[0] belongs to this tensor
 };
 struct StepArgs {
-    const OptTensor* tensors;
     const OptChunk* chunks;
     void* m; void* v; float* ms; float* vs;
     OptState* st;
@@ -86,22 +86,28 @@ __device__ __forceinline__ void adamw_elem(float& p, float& m, float v, float& v
     p = p * k.keep - __fdiv_rn(m, u * k.root + k.eps) * k.size;
 }
 
-// nearest code of t = |x| / s: q with q^2 - q + 1/2 <= t < q^2 + q + 1/2.  The hardware root is off by an ulp, the two comparisons are exact.
-__device__ __forceinline__ float nearest_code(float t, float levels) {
-    float q = floorf(__builtin_amdgcn_sqrtf(fmaxf(t - 0.25f, 0.f)) + 0.5f);
-    const float q2 = q * q;
-    if (t >= q2 + q + 0.5f) q += 1.f;
-    else if (t < q2 - q + 0.5f && q > 0.f) q -= 1.f;
-    return fminf(q, levels);
+// nearest code of t = |x| / s: q with q^2 - q + 1/2 <= t < q^2 + q + 1/2.  floor(sqrt(t - 1/4) + 1/2) from the hardware root (off by an ulp, below 4e-5
+// here), started low by 1e-4: that is q or q - 1, and one exact comparison tells.  No t exceeds the largest code's upper border.
+__device__ __forceinline__ float nearest_code(float t) {
+    const float q = floorf(__builtin_amdgcn_sqrtf(fabsf(t - 0.25f)) + (0.5f - 1e-4f));
+    return t >= fmaf(q, q, q + 0.5f) ? q + 1.f : q;
 }
 
-// block maximum of non-negative values over a wave, as integers so that a NaN counts as the largest value
+// block maximum of non-negative values over a wave, as integers so that a NaN counts as the largest value; in lane 63's row reductions and two
+// broadcasts (no LDS)
 __device__ __forceinline__ float wave_max_abs(float a, float b, float c, float d) {
     auto bits = [](float x) { return __float_as_uint(x) & 0x7fffffffu; };
     unsigned int r = max(max(bits(a), bits(b)), max(bits(c), bits(d)));
-#pragma unroll
-    for (int o = 32; o; o >>= 1) r = max(r, (unsigned int)__shfl_xor((int)r, o));
-    return __uint_as_float(r);
+    auto step = [&](auto ctrl, auto rows) {
+        r = max(r, (unsigned int)__builtin_amdgcn_update_dpp(0, (int)r, ctrl.value, rows.value, 0xf, true));
+    };
+    step(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xf>{});        // row_shr 1, 2, 4, 8: lane 15 of a row has the row's
+    step(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xf>{});
+    step(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{});        // row_bcast 15 into rows 1 and 3
+    step(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{});        // row_bcast 31 into rows 2 and 3
+    return __uint_as_float((unsigned int)__builtin_amdgcn_readlane((int)r, 63));
 }
 __device__ __forceinline__ float block_scale(float amax, float k) {
     const float s = amax * k;
@@ -110,25 +116,33 @@ __device__ __forceinline__ float block_scale(float amax, float k) {
 
 // one wave's blocks of one chunk; the moments' arenas are padded to whole blocks, the pads hold zeros and are written as such
 template <class PT, class GT, int BITS>
-__device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptTensor& t, const GT* __restrict__ g, int block, const Coef& k) {
+__device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptChunk& c, const GT* __restrict__ g, int wave, const Coef& k) {
     constexpr int NB = kChunkBlocks / 4;
-    const int lane = threadIdx.x & 63;
+    const int lane = threadIdx.x & 63, at0 = wave * NB * kOptBlock + lane * 4;
+    const bool full = c.left == kChunkBlocks * kOptBlock;
     typename Vec4<PT>::raw rp[NB];
     typename Vec4<GT>::raw rg[NB];
     f32x4 rw[NB], rm[NB], rv[NB];
     unsigned int qm[NB], qv[NB];
     float sm[NB], sv[NB];
-    PT* __restrict__ p = (PT*)t.p;
-    int left[NB];
+    PT* __restrict__ p = (PT*)c.p;
+    float* __restrict__ master = c.master;
+    const int64_t b0 = c.block + wave * NB;
+    const int mine = full ? NB : min(NB, (c.left + kOptBlock - 1) / kOptBlock - wave * NB);          // blocks of this wave
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int64_t at = (int64_t)(block + j) * kOptBlock + lane * 4, bb = t.block0 + block + j;
-        const int64_t l = t.n - at;
-        left[j] = l >= 4 ? 4 : l < 0 ? 0 : (int)l;
-        if ((int64_t)(block + j) * kOptBlock >= t.n) continue;       // no such block (whole waves)
-        raw_load<GT>(rg[j], g + at, left[j]);
-        raw_load<PT>(rp[j], p + at, left[j]);
-        if (t.master) raw_load<float>(rw[j], t.master + at, left[j]);
+        if (j >= mine) continue;
+        const int at = at0 + j * kOptBlock;
+        const int64_t bb = b0 + j;
+        if (full) {
+            rg[j] = at4(g + at);
+            rp[j] = at4(p + at);
+            if (master) rw[j] = at4(master + at);
+        } else {
+            raw_load<GT>(rg[j], g + at, c.left - at);
+            raw_load<PT>(rp[j], p + at, c.left - at);
+            if (master) raw_load<float>(rw[j], master + at, c.left - at);
+        }
         if constexpr (BITS == 32) {
             rm[j] = ((const f32x4*)a.m)[bb * 64 + lane];
             rv[j] = ((const f32x4*)a.v)[bb * 64 + lane];
@@ -139,13 +153,17 @@ __device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptTensor& t
             sv[j] = a.vs[bb];
         }
     }
+    f32x4 um[NB], uu[NB];                                  // 8 bits: the new m and root of v of every block, until their scales are known
+    float top[2 * NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-        const int64_t at = (int64_t)(block + j) * kOptBlock + lane * 4, bb = t.block0 + block + j;
-        if ((int64_t)(block + j) * kOptBlock >= t.n) continue;
+        top[2 * j] = top[2 * j + 1] = 0.f;
+        if (j >= mine) continue;
+        const int at = at0 + j * kOptBlock;
+        const int64_t bb = b0 + j;
         float gf[4], pf[4], m[4], v[4], u[4];
         unpack<GT>(rg[j], gf);
-        if (t.master) { pf[0] = rw[j].x; pf[1] = rw[j].y; pf[2] = rw[j].z; pf[3] = rw[j].w; }
+        if (master) { pf[0] = rw[j].x; pf[1] = rw[j].y; pf[2] = rw[j].z; pf[3] = rw[j].w; }
         else unpack<PT>(rp[j], pf);
         if constexpr (BITS == 32) {
             m[0] = rm[j].x; m[1] = rm[j].y; m[2] = rm[j].z; m[3] = rm[j].w;
@@ -164,31 +182,62 @@ __device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptTensor& t
             float vn;
             adamw_elem(pf[i], m[i], v[i], vn, u[i], gf[i], k);
             v[i] = vn;
-            if (i >= left[j]) { m[i] = 0.f; v[i] = 0.f; u[i] = 0.f; }
         }
-        if (t.master) raw_store<float>(f32x4{pf[0], pf[1], pf[2], pf[3]}, t.master + at, left[j]);
-        raw_store<PT>(pack<PT>(pf), p + at, left[j]);
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i >= c.left - at) { m[i] = 0.f; v[i] = 0.f; u[i] = 0.f; }
+            if (master) raw_store<float>(f32x4{pf[0], pf[1], pf[2], pf[3]}, master + at, c.left - at);
+            raw_store<PT>(pack<PT>(pf), p + at, c.left - at);
+        } else {
+            if (master) reinterpret_cast<Loose<f32x4>*>(master + at)->v = f32x4{pf[0], pf[1], pf[2], pf[3]};
+            reinterpret_cast<Loose<typename Vec4<PT>::raw>*>(p + at)->v = pack<PT>(pf);
+        }
         if constexpr (BITS == 32) {
             ((f32x4*)a.m)[bb * 64 + lane] = f32x4{m[0], m[1], m[2], m[3]};
             ((f32x4*)a.v)[bb * 64 + lane] = f32x4{v[0], v[1], v[2], v[3]};
         } else {
-            const float s = block_scale(wave_max_abs(m[0], m[1], m[2], m[3]), kK127);
-            const float w = block_scale(wave_max_abs(u[0], u[1], u[2], u[3]), kK255);
-            const float is = s > 0.f ? __fdiv_rn(1.f, s) : 0.f, iw = w > 0.f ? __fdiv_rn(1.f, w) : 0.f;
+            um[j] = f32x4{m[0], m[1], m[2], m[3]};
+            uu[j] = f32x4{u[0], u[1], u[2], u[3]};
+            top[2 * j] = wave_max_abs(m[0], m[1], m[2], m[3]);
+            top[2 * j + 1] = wave_max_abs(u[0], u[1], u[2], u[3]);
+        }
+    }
+    if constexpr (BITS == 8) {
+        // the eight scales side by side in eight lanes: one division gives all their reciprocals
+        float mine_top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2 * NB; ++i) mine_top = lane == i ? top[i] : mine_top;
+        const float scale = block_scale(mine_top, lane & 1 ? kK255 : kK127);
+        const float inverse = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            if (j >= mine) continue;
+            const int64_t bb = b0 + j;
+            const float is = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inverse), 2 * j));
+            const float iw = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inverse), 2 * j + 1));
             unsigned int cm = 0, cv = 0;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                int q = (int)nearest_code(fabsf(m[i]) * is, 127.f);
-                q = m[i] < 0.f ? -q : q;
-                int r = (int)nearest_code(u[i] * iw, 255.f);
-                if (u[i] > 0.f && r == 0) r = 1;
+                const int q = (int)copysignf(nearest_code(fabsf(um[j][i]) * is), um[j][i]);
+                int r = (int)nearest_code(uu[j][i] * iw);
+                r = uu[j][i] > 0.f ? max(r, 1) : r;
                 cm |= ((unsigned int)q & 255u) << (8 * i);
                 cv |= (unsigned int)r << (8 * i);
             }
             ((unsigned int*)a.m)[bb * 64 + lane] = cm;
             ((unsigned int*)a.v)[bb * 64 + lane] = cv;
-            if (lane == 0) { a.ms[bb] = s; a.vs[bb] = w; }
         }
+        if (lane < 2 * mine) (lane & 1 ? a.vs : a.ms)[b0 + (lane >> 1)] = scale;
+    }
+}
+
+// b1^t and b2^t by squaring (a library power of two doubles takes several times as long as the rest of a small step)
+__device__ __forceinline__ void powers(double b1, double b2, int64_t t, double& r1, double& r2) {
+    r1 = r2 = 1.0;
+    for (; t > 0; t >>= 1) {
+        if (t & 1) { r1 *= b1; r2 *= b2; }
+        b1 *= b1;
+        b2 *= b2;
     }
 }
 
@@ -197,32 +246,31 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a, GradArgs ga) {
     __shared__ Coef s_k;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const OptChunk c = a.chunks[blockIdx.x];
-    const OptTensor t = a.tensors[c.tensor];
     const bool skip = a.clipped && a.st->skip;
     if (tid == 0) {
-        const double step = (double)(a.st->step + 1);
+        double r1, r2;
+        powers(a.b1, a.b2, a.st->step + 1, r1, r2);
         s_k.b1 = (float)a.b1; s_k.c1 = (float)(1.0 - a.b1);
         s_k.b2 = (float)a.b2; s_k.c2 = (float)(1.0 - a.b2);
-        s_k.size = (float)(a.lr / (1.0 - pow(a.b1, step)));
-        s_k.root = (float)(1.0 / sqrt(1.0 - pow(a.b2, step)));
+        s_k.size = (float)(a.lr / (1.0 - r1));
+        s_k.root = (float)(1.0 / sqrt(1.0 - r2));
         s_k.eps = a.eps;
-        s_k.keep = (float)(1.0 - a.lr * t.wd);
+        s_k.keep = (float)(1.0 - a.lr * c.wd);
         s_k.gscale = a.clipped ? a.st->gscale : a.gscale;
     }
     __syncthreads();
     const Coef k = s_k;
     if (!skip) {
-        const int block = c.block + wave * (kChunkBlocks / 4);
         const void* g = ga.g[c.tensor - ga.tensor0];
         const int gt = ga.type[c.tensor - ga.tensor0];
         auto by_grad = [&](auto pt) {
             using PT = decltype(pt);
-            if (gt == SCS_F32) adamw_wave<PT, float, BITS>(a, t, (const float*)g, block, k);
-            else if (gt == SCS_BF16) adamw_wave<PT, __bf16, BITS>(a, t, (const __bf16*)g, block, k);
-            else adamw_wave<PT, _Float16, BITS>(a, t, (const _Float16*)g, block, k);
+            if (gt == SCS_F32) adamw_wave<PT, float, BITS>(a, c, (const float*)g + c.first, wave, k);
+            else if (gt == SCS_BF16) adamw_wave<PT, __bf16, BITS>(a, c, (const __bf16*)g + c.first, wave, k);
+            else adamw_wave<PT, _Float16, BITS>(a, c, (const _Float16*)g + c.first, wave, k);
         };
-        if (t.type == SCS_F32) by_grad(float{});
-        else if (t.type == SCS_BF16) by_grad(__bf16{});
+        if (c.type == SCS_F32) by_grad(float{});
+        else if (c.type == SCS_BF16) by_grad(__bf16{});
         else by_grad(_Float16{});
     }
     // the step is counted by the workgroup that finishes last (every workgroup has read the count by then): a ticket tree of two levels,
@@ -233,7 +281,6 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a, GradArgs ga) {
         unsigned int* tk = a.st->ticket;
         if (atomicAdd(&tk[32 * (1 + leaf)], 1u) == members - 1) {
             tk[32 * (1 + leaf)] = 0;
-            __threadfence();
             if (atomicAdd(&tk[0], 1u) == leaves - 1) {
                 tk[0] = 0;
                 if (!skip) a.st->step += 1;
@@ -255,14 +302,16 @@ __device__ __forceinline__ double block_sum256(double v, double* s_red) {
 }
 
 template <class GT>
-__device__ __forceinline__ double chunk_squares(const GT* __restrict__ g, int64_t n, int block) {
+__device__ __forceinline__ double chunk_squares(const GT* __restrict__ g, int n) {
     double sum = 0.0;
     typename Vec4<GT>::raw r[kChunkBlocks / 4];
-    const int64_t base = (int64_t)block * kOptBlock + threadIdx.x * 4;
+    const int base = threadIdx.x * 4;
+    if (n == kChunkBlocks * kOptBlock) {
 #pragma unroll
-    for (int j = 0; j < kChunkBlocks / 4; ++j) {
-        const int64_t l = n - (base + j * 1024);
-        raw_load<GT>(r[j], g + base + j * 1024, l >= 4 ? 4 : l < 0 ? 0 : (int)l);
+        for (int j = 0; j < kChunkBlocks / 4; ++j) r[j] = at4(g + base + j * 1024);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kChunkBlocks / 4; ++j) raw_load<GT>(r[j], g + base + j * 1024, n - (base + j * 1024));
     }
 #pragma unroll
     for (int j = 0; j < kChunkBlocks / 4; ++j) {
@@ -275,7 +324,7 @@ __device__ __forceinline__ double chunk_squares(const GT* __restrict__ g, int64_
 }
 
 struct NormArgs {
-    const OptTensor* tensors; const OptChunk* chunks; int32_t n_chunks;
+    const OptChunk* chunks; int32_t n_chunks;
     double* partial;          // [launches][kNormGroups]
     int32_t launch, n_partial, total_groups;
     OptState* st; double grad_scale, max_norm; float* norm_out;
@@ -286,25 +335,25 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(NormArgs a, GradArgs ga
     __shared__ double s_red[4];
     __shared__ bool s_last;
     double sum = 0.0;
+#pragma unroll 2
     for (int c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
-        const OptChunk ch = a.chunks[c];
-        const int64_t n = a.tensors[ch.tensor].n;
-        const void* g = ga.g[ch.tensor - ga.tensor0];
-        const int gt = ga.type[ch.tensor - ga.tensor0];
-        if (gt == SCS_F32) sum += chunk_squares((const float*)g, n, ch.block);
-        else if (gt == SCS_BF16) sum += chunk_squares((const __bf16*)g, n, ch.block);
-        else sum += chunk_squares((const _Float16*)g, n, ch.block);
+        const int tensor = a.chunks[c].tensor, left = a.chunks[c].left;
+        const int64_t first = a.chunks[c].first;
+        const void* g = ga.g[tensor - ga.tensor0];
+        const int gt = ga.type[tensor - ga.tensor0];
+        if (gt == SCS_F32) sum += chunk_squares((const float*)g + first, left);
+        else if (gt == SCS_BF16) sum += chunk_squares((const __bf16*)g + first, left);
+        else sum += chunk_squares((const _Float16*)g + first, left);
     }
     sum = block_sum256(sum, s_red);
     if (threadIdx.x == 0) {
         // (device scope: the workgroup that adds them up may sit on another XCD, behind another L2)
         __hip_atomic_store(&a.partial[(int64_t)a.launch * kNormGroups + blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __threadfence();
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // (written through to what all XCDs share: no cache has to be written back)
         s_last = atomicAdd(&a.st->norm_ticket, 1u) == (unsigned int)a.total_groups - 1;
     }
     __syncthreads();
     if (!s_last) return;
-    __threadfence();
     double all = 0.0;
     for (int i = threadIdx.x; i < a.n_partial; i += 256) all += __hip_atomic_load(&a.partial[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     all = block_sum256(all, s_red);
@@ -355,7 +404,6 @@ struct scs_adamw_ctx {
     unsigned char* mem = nullptr;              // OptState, partial sums, tensors, chunks
     scs::OptState* st = nullptr;
     double* partial = nullptr;
-    scs::OptTensor* tensors = nullptr;
     scs::OptChunk* chunks = nullptr;
     int launches = 0;
 };
@@ -373,7 +421,6 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
     SCS_ARG(state_bits == 32 || state_bits == 8, "state_bits is 32 or 8");
     SCS_ARG(step >= 0, "the step count is negative");
     return guarded([&]() -> int {
-        std::vector<OptTensor> tt(n);
         std::vector<OptChunk> ch;
         std::vector<std::pair<uintptr_t, uintptr_t>> spans;
         scs_adamw_ctx* o = new scs_adamw_ctx();
@@ -392,10 +439,13 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
                 spans.emplace_back((uintptr_t)t.param, (uintptr_t)t.param + (uintptr_t)t.n * e);
                 if (t.master) spans.emplace_back((uintptr_t)t.master, (uintptr_t)t.master + (uintptr_t)t.n * 4);
             }
-            tt[i] = OptTensor{t.param, t.master, t.n, o->blocks, t.weight_decay, t.type, 0};
             const int64_t blocks = (t.n + kOptBlock - 1) / kOptBlock;
             o->chunk0.push_back((int32_t)ch.size());
-            for (int64_t b = 0; b < blocks; b += kChunkBlocks) ch.push_back(OptChunk{i, (int32_t)b});
+            for (int64_t b = 0; b < blocks; b += kChunkBlocks) {
+                const int64_t at = b * kOptBlock;
+                ch.push_back(OptChunk{(char*)t.param + at * (int64_t)e, t.master ? t.master + at : nullptr, o->blocks + b, at, t.weight_decay,
+                                      (int32_t)std::min<int64_t>(t.n - at, kChunkBlocks * kOptBlock), i, t.type, 0});
+            }
             SCS_ARG(ch.size() < ((size_t)1 << 30), "more elements than one optimiser takes");
             o->blocks += blocks;
             o->sizes.push_back(t.n);
@@ -413,17 +463,15 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
         DeviceGuard dev(o->device);
         if (dev.rc != SCS_OK) return dev.rc;
         auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
-        const size_t b_st = up(sizeof(OptState)), b_pa = up(sizeof(double) * kNormGroups * o->launches), b_te = up(sizeof(OptTensor) * n),
+        const size_t b_st = up(sizeof(OptState)), b_pa = up(sizeof(double) * kNormGroups * o->launches),
                      b_ch = up(sizeof(OptChunk) * std::max<size_t>(1, ch.size()));
-        SCS_HIP(hipMalloc(&o->mem, b_st + b_pa + b_te + b_ch));
-        std::vector<unsigned char> host(b_st + b_pa + b_te + b_ch, 0);
+        SCS_HIP(hipMalloc(&o->mem, b_st + b_pa + b_ch));
+        std::vector<unsigned char> host(b_st + b_pa + b_ch, 0);
         o->st = (OptState*)o->mem;
         o->partial = (double*)(o->mem + b_st);
-        o->tensors = (OptTensor*)(o->mem + b_st + b_pa);
-        o->chunks = (OptChunk*)(o->mem + b_st + b_pa + b_te);
+        o->chunks = (OptChunk*)(o->mem + b_st + b_pa);
         memcpy(host.data() + offsetof(OptState, step), &step, sizeof(step));
-        memcpy(host.data() + b_st + b_pa, tt.data(), sizeof(OptTensor) * n);
-        if (!ch.empty()) memcpy(host.data() + b_st + b_pa + b_te, ch.data(), sizeof(OptChunk) * ch.size());
+        if (!ch.empty()) memcpy(host.data() + b_st + b_pa, ch.data(), sizeof(OptChunk) * ch.size());
         SCS_HIP(hipMemcpy(o->mem, host.data(), host.size(), hipMemcpyHostToDevice));
         *out = o;
         o = nullptr;
@@ -473,7 +521,7 @@ int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_ty
         for (int l = 0; l < o->launches; ++l) total += groups(l);
         for (int l = 0; l < o->launches; ++l) {
             const auto c = fill(l);
-            NormArgs na{o->tensors, o->chunks + c.first, c.second - c.first, o->partial, l, kNormGroups * o->launches, total, o->st, grad_scale, max_norm, norm_dev};
+            NormArgs na{o->chunks + c.first, c.second - c.first, o->partial, l, kNormGroups * o->launches, total, o->st, grad_scale, max_norm, norm_dev};
             hipLaunchKernelGGL(adamw_norm_kernel, dim3(groups(l)), dim3(256), 0, st, na, ga);
         }
     }
@@ -485,7 +533,7 @@ int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_ty
     for (int l = 0; l <= last; ++l) {
         const auto c = fill(l);
         if (c.second == c.first) continue;
-        StepArgs sa{o->tensors, o->chunks + c.first, o->m, o->v, o->ms, o->vs, o->st, lr, beta1, beta2, (float)eps, (float)grad_scale, max_norm > 0, l == last};
+        StepArgs sa{o->chunks + c.first, o->m, o->v, o->ms, o->vs, o->st, lr, beta1, beta2, (float)eps, (float)grad_scale, max_norm > 0, l == last};
         if (o->bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, dim3(c.second - c.first), dim3(256), 0, st, sa, ga);
         else hipLaunchKernelGGL(adamw_kernel<8>, dim3(c.second - c.first), dim3(256), 0, st, sa, ga);
     }
