@@ -134,9 +134,8 @@ class AdamW:
             ptrs, types = self._bound
         else:
             _, ptrs, types = self._gradients(grads)
-        for w, p in zip(self._where, self.params):
-            if p.data_ptr() != w:
-                raise RuntimeError('a parameter has moved since the optimiser was made')
+        if list(map(self._torch.Tensor.data_ptr, self.params)) != self._where:
+            raise RuntimeError('a parameter has moved since the optimiser was made')
         stream = self._torch.cuda.current_stream(self.device).cuda_stream
         _hip._check(self._lib.scs_adamw_step(self._o, ptrs, types, self.lr if lr is None else float(lr), self.betas[0], self.betas[1], self.eps,
                                              float(grad_scale), self.max_norm or 0.0,

@@ -16,8 +16,8 @@
 //
 // What bounds it: HBM.  f32 parameters and moments move 28 B an element, bf16 parameters and gradients with 8-bit moments 10.1 B
 // (at those bytes the division and three roots an element are the second bound: ~70 vector instructions).  Work unit: a wave takes four
-// blocks of 256 elements, a lane 4 consecutive elements of each (16-byte loads of f32, all four blocks' loads in flight before the first
-// use); a workgroup = 4 waves = one chunk of 16 blocks of one tensor; blocks never cross tensors.
+// blocks of 256 elements (one where there are few), a lane 4 consecutive elements of each (16-byte loads of f32, all four blocks' loads in flight before the first
+// use); a workgroup = 4 waves = one chunk of 16 (4) blocks of one tensor; blocks never cross tensors.
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -30,7 +30,9 @@ namespace scs {
 namespace {
 
 constexpr int kOptBlock = 256;             // elements that share a scale
-constexpr int kChunkBlocks = 16;           // blocks of one workgroup
+constexpr int kChunkBlocks = 16;           // blocks of one workgroup ...
+constexpr int kSmallBlocks = 4;            // ... and where that would make fewer than kManyChunks of them (a net of 883 455 parameters: 290)
+constexpr int kManyChunks = 2048;
 constexpr int kGradsPerLaunch = 384;       // gradient pointers that travel by value in one launch's arguments (at most 4 KB of them)
 constexpr int kNormGroups = 1024;          // workgroups of the norm's first stage = partial sums in double
 constexpr int kTickets = 64;               // leaves of the ticket tree, one 128-byte line each
@@ -53,8 +55,7 @@ struct OptState {            // device words of one optimiser
     double norm;             // of the last clipped step
     float gscale;            // its c
     int32_t skip;            // 1: its norm was not finite: parameters, moments and step stay
-    unsigned int norm_ticket;
-    unsigned int pad[23];
+    unsigned int pad[24];
     unsigned int ticket[(kTickets + 1) * 32];
 };
 
@@ -115,11 +116,10 @@ __device__ __forceinline__ float block_scale(float amax, float k) {
 }
 
 // one wave's blocks of one chunk; the moments' arenas are padded to whole blocks, the pads hold zeros and are written as such
-template <class PT, class GT, int BITS>
+template <class PT, class GT, int BITS, int NB>
 __device__ __forceinline__ void adamw_wave(const StepArgs& a, const OptChunk& c, const GT* __restrict__ g, int wave, const Coef& k) {
-    constexpr int NB = kChunkBlocks / 4;
     const int lane = threadIdx.x & 63, at0 = wave * NB * kOptBlock + lane * 4;
-    const bool full = c.left == kChunkBlocks * kOptBlock;
+    const bool full = c.left == 4 * NB * kOptBlock;
     typename Vec4<PT>::raw rp[NB];
     typename Vec4<GT>::raw rg[NB];
     f32x4 rw[NB], rm[NB], rv[NB];
@@ -241,7 +241,19 @@ __device__ __forceinline__ void powers(double b1, double b2, int64_t t, double& 
     }
 }
 
-template <int BITS>
+// Whether this is the last of `n` workgroups: a ticket tree of two levels (1024 tickets of one counter take 10 us), its counters left at zero for the
+// next launch.
+__device__ __forceinline__ bool last_ticket(OptState* st, unsigned int id, unsigned int n) {
+    const unsigned int leaf = id % kTickets, members = n / kTickets + (leaf < n % kTickets ? 1u : 0u);
+    unsigned int* leaf_ticket = &st->ticket[32 * (1 + leaf)];
+    if (__hip_atomic_fetch_add(leaf_ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != members - 1) return false;
+    __hip_atomic_store(leaf_ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__hip_atomic_fetch_add(&st->ticket[0], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != min(n, (unsigned int)kTickets) - 1) return false;
+    __hip_atomic_store(&st->ticket[0], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
+template <int BITS, int NB>
 __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a, GradArgs ga) {
     __shared__ Coef s_k;
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -265,28 +277,16 @@ __global__ __launch_bounds__(256) void adamw_kernel(StepArgs a, GradArgs ga) {
         const int gt = ga.type[c.tensor - ga.tensor0];
         auto by_grad = [&](auto pt) {
             using PT = decltype(pt);
-            if (gt == SCS_F32) adamw_wave<PT, float, BITS>(a, c, (const float*)g + c.first, wave, k);
-            else if (gt == SCS_BF16) adamw_wave<PT, __bf16, BITS>(a, c, (const __bf16*)g + c.first, wave, k);
-            else adamw_wave<PT, _Float16, BITS>(a, c, (const _Float16*)g + c.first, wave, k);
+            if (gt == SCS_F32) adamw_wave<PT, float, BITS, NB>(a, c, (const float*)g + c.first, wave, k);
+            else if (gt == SCS_BF16) adamw_wave<PT, __bf16, BITS, NB>(a, c, (const __bf16*)g + c.first, wave, k);
+            else adamw_wave<PT, _Float16, BITS, NB>(a, c, (const _Float16*)g + c.first, wave, k);
         };
         if (c.type == SCS_F32) by_grad(float{});
         else if (c.type == SCS_BF16) by_grad(__bf16{});
         else by_grad(_Float16{});
     }
-    // the step is counted by the workgroup that finishes last (every workgroup has read the count by then): a ticket tree of two levels,
-    // its counters left at zero for the next launch
-    if (a.last && tid == 0) {
-        const unsigned int leaf = blockIdx.x % kTickets, leaves = min((unsigned int)gridDim.x, (unsigned int)kTickets);
-        const unsigned int members = gridDim.x / kTickets + (leaf < gridDim.x % kTickets ? 1u : 0u);
-        unsigned int* tk = a.st->ticket;
-        if (atomicAdd(&tk[32 * (1 + leaf)], 1u) == members - 1) {
-            tk[32 * (1 + leaf)] = 0;
-            if (atomicAdd(&tk[0], 1u) == leaves - 1) {
-                tk[0] = 0;
-                if (!skip) a.st->step += 1;
-            }
-        }
-    }
+    // the step is counted by the workgroup that finishes last (every workgroup has read the count by then)
+    if (a.last && tid == 0 && last_ticket(a.st, blockIdx.x, gridDim.x) && !skip) a.st->step += 1;
 }
 
 // sum of squares of every gradient, in double: workgroup i takes chunks i, i + groups, ..., the last one to finish adds the partial sums
@@ -301,56 +301,89 @@ __device__ __forceinline__ double block_sum256(double v, double* s_red) {
     return v;
 }
 
-template <class GT>
-__device__ __forceinline__ double chunk_squares(const GT* __restrict__ g, int n) {
-    double sum = 0.0;
-    typename Vec4<GT>::raw r[kChunkBlocks / 4];
-    const int base = threadIdx.x * 4;
-    if (n == kChunkBlocks * kOptBlock) {
+template <class GT, int NB> struct ChunkLoad {
+    typename Vec4<GT>::raw r[NB];
+    __device__ __forceinline__ void load(const GT* __restrict__ g, int n) {
+        const int base = threadIdx.x * 4;
+        if (n == 4 * NB * kOptBlock) {
 #pragma unroll
-        for (int j = 0; j < kChunkBlocks / 4; ++j) r[j] = at4(g + base + j * 1024);
-    } else {
+            for (int j = 0; j < NB; ++j) r[j] = at4(g + base + j * 1024);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kChunkBlocks / 4; ++j) raw_load<GT>(r[j], g + base + j * 1024, n - (base + j * 1024));
+            for (int j = 0; j < NB; ++j) raw_load<GT>(r[j], g + base + j * 1024, n - (base + j * 1024));
+        }
     }
+    __device__ __forceinline__ double squares() const {
+        double sum = 0.0;
 #pragma unroll
-    for (int j = 0; j < kChunkBlocks / 4; ++j) {
-        float f[4];
-        unpack<GT>(r[j], f);
+        for (int j = 0; j < NB; ++j) {
+            float f[4];
+            unpack<GT>(r[j], f);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sum += (double)f[i] * (double)f[i];
+            for (int i = 0; i < 4; ++i) sum += (double)f[i] * (double)f[i];
+        }
+        return sum;
     }
-    return sum;
-}
+};
 
 struct NormArgs {
     const OptChunk* chunks; int32_t n_chunks;
     double* partial;          // [launches][kNormGroups]
-    int32_t launch, n_partial, total_groups;
+    int32_t launch, n_partial, group0, total_groups;
+    int32_t type;             // of every gradient of the launch, -1: they differ
     OptState* st; double grad_scale, max_norm; float* norm_out;
 };
 static_assert(sizeof(GradArgs) + sizeof(NormArgs) <= 4096, "kernel arguments");
 
+// one type throughout: the next two chunks are on their way while one is added up
+template <class GT, int NB> __device__ __forceinline__ double squares_of(const NormArgs& a, const GradArgs& ga) {
+    constexpr int AHEAD = 2;
+    ChunkLoad<GT, NB> l[AHEAD + 1];
+    auto load = [&](ChunkLoad<GT, NB>& to, int c) {
+        const OptChunk& ch = a.chunks[c];
+        to.load((const GT*)ga.g[ch.tensor - ga.tensor0] + ch.first, ch.left);
+    };
+    const int step = gridDim.x;
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) if ((int)blockIdx.x + i * step < a.n_chunks) load(l[i], blockIdx.x + i * step);
+    for (int c = blockIdx.x; c < a.n_chunks; c += (AHEAD + 1) * step) {
+#pragma unroll
+        for (int i = 0; i <= AHEAD; ++i) {
+            if (c + (i + AHEAD) * step < a.n_chunks) load(l[(i + AHEAD) % (AHEAD + 1)], c + (i + AHEAD) * step);
+            if (c + i * step < a.n_chunks) sum += l[i].squares();
+        }
+    }
+    return sum;
+}
+template <class GT, int NB> __device__ __forceinline__ double chunk_squares(const void* g, const OptChunk& c) {
+    ChunkLoad<GT, NB> l;
+    l.load((const GT*)g + c.first, c.left);
+    return l.squares();
+}
+
+template <int NB>
 __global__ __launch_bounds__(256) void adamw_norm_kernel(NormArgs a, GradArgs ga) {
     __shared__ double s_red[4];
     __shared__ bool s_last;
     double sum = 0.0;
-#pragma unroll 2
-    for (int c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
-        const int tensor = a.chunks[c].tensor, left = a.chunks[c].left;
-        const int64_t first = a.chunks[c].first;
-        const void* g = ga.g[tensor - ga.tensor0];
-        const int gt = ga.type[tensor - ga.tensor0];
-        if (gt == SCS_F32) sum += chunk_squares((const float*)g + first, left);
-        else if (gt == SCS_BF16) sum += chunk_squares((const __bf16*)g + first, left);
-        else sum += chunk_squares((const _Float16*)g + first, left);
+    if (a.type == SCS_F32) sum = squares_of<float, NB>(a, ga);
+    else if (a.type == SCS_BF16) sum = squares_of<__bf16, NB>(a, ga);
+    else if (a.type == SCS_F16) sum = squares_of<_Float16, NB>(a, ga);
+    else for (int c = blockIdx.x; c < a.n_chunks; c += gridDim.x) {
+        const OptChunk& ch = a.chunks[c];
+        const void* g = ga.g[ch.tensor - ga.tensor0];
+        const int gt = ga.type[ch.tensor - ga.tensor0];
+        if (gt == SCS_F32) sum += chunk_squares<float, NB>(g, ch);
+        else if (gt == SCS_BF16) sum += chunk_squares<__bf16, NB>(g, ch);
+        else sum += chunk_squares<_Float16, NB>(g, ch);
     }
     sum = block_sum256(sum, s_red);
     if (threadIdx.x == 0) {
         // (device scope: the workgroup that adds them up may sit on another XCD, behind another L2)
         __hip_atomic_store(&a.partial[(int64_t)a.launch * kNormGroups + blockIdx.x], sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");              // (written through to what all XCDs share: no cache has to be written back)
-        s_last = atomicAdd(&a.st->norm_ticket, 1u) == (unsigned int)a.total_groups - 1;
+        s_last = last_ticket(a.st, a.group0 + blockIdx.x, a.total_groups);
     }
     __syncthreads();
     if (!s_last) return;
@@ -363,7 +396,6 @@ __global__ __launch_bounds__(256) void adamw_norm_kernel(NormArgs a, GradArgs ga
         a.st->norm = norm;
         a.st->gscale = (float)(a.grad_scale * (f < 1.0 ? f : 1.0));
         a.st->skip = !(norm <= 1.7e308);
-        a.st->norm_ticket = 0;
         if (a.norm_out) *a.norm_out = (float)norm;
     }
 }
@@ -394,7 +426,7 @@ __global__ void adamw_set_step_kernel(OptState* st, int64_t step) { st->step = s
 }  // namespace scs
 
 struct scs_adamw_ctx {
-    int device = 0, bits = 32;
+    int device = 0, bits = 32, chunk_blocks = scs::kChunkBlocks;
     int n = 0;
     int64_t blocks = 0;
     void *m = nullptr, *v = nullptr;
@@ -426,6 +458,9 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
         scs_adamw_ctx* o = new scs_adamw_ctx();
         struct Drop { scs_adamw_ctx*& o; ~Drop() { if (o) { if (o->mem) (void)hipFree(o->mem); delete o; } } } drop{o};
         o->device = handle_device(h); o->bits = state_bits; o->n = n;
+        int64_t chunks = 0;
+        for (int i = 0; i < n; ++i) if (tensors[i].n > 0) chunks += (tensors[i].n + kChunkBlocks * kOptBlock - 1) / (kChunkBlocks * kOptBlock);
+        if (chunks < kManyChunks) o->chunk_blocks = kSmallBlocks;
         for (int i = 0; i < n; ++i) {
             const scs_adamw_tensor& t = tensors[i];
             SCS_ARG(t.n >= 0 && t.n <= ((int64_t)1 << 38), "a tensor's size is negative or above 2^38");
@@ -441,10 +476,10 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
             }
             const int64_t blocks = (t.n + kOptBlock - 1) / kOptBlock;
             o->chunk0.push_back((int32_t)ch.size());
-            for (int64_t b = 0; b < blocks; b += kChunkBlocks) {
+            for (int64_t b = 0; b < blocks; b += o->chunk_blocks) {
                 const int64_t at = b * kOptBlock;
                 ch.push_back(OptChunk{(char*)t.param + at * (int64_t)e, t.master ? t.master + at : nullptr, o->blocks + b, at, t.weight_decay,
-                                      (int32_t)std::min<int64_t>(t.n - at, kChunkBlocks * kOptBlock), i, t.type, 0});
+                                      (int32_t)std::min<int64_t>(t.n - at, o->chunk_blocks * kOptBlock), i, t.type, 0});
             }
             SCS_ARG(ch.size() < ((size_t)1 << 30), "more elements than one optimiser takes");
             o->blocks += blocks;
@@ -513,16 +548,23 @@ int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_ty
     };
     auto groups = [&](int l) {
         const int lo = l * kGradsPerLaunch, hi = std::min(o->n, lo + kGradsPerLaunch);
-        return std::max(1, std::min(kNormGroups, (int)(o->chunk0[hi] - o->chunk0[lo])));       // one at least: the last one writes the result
+        // one at least: the last one writes the result
+        return std::max(1, std::min(o->chunk_blocks == kChunkBlocks ? kNormGroups : kNormGroups / 4, (int)(o->chunk0[hi] - o->chunk0[lo])));
+    };
+    auto type_of = [&](int l) {
+        const int lo = l * kGradsPerLaunch, hi = std::min(o->n, lo + kGradsPerLaunch);
+        for (int i = lo; i < hi; ++i) if (grad_types[i] != grad_types[lo]) return -1;
+        return (int)grad_types[lo];
     };
     if (max_norm > 0) {
         // every launch has a row of kNormGroups partial sums; those that a short launch leaves out were cleared at creation and stay zero
         int total = 0;
         for (int l = 0; l < o->launches; ++l) total += groups(l);
-        for (int l = 0; l < o->launches; ++l) {
+        for (int l = 0, at = 0; l < o->launches; at += groups(l), ++l) {
             const auto c = fill(l);
-            NormArgs na{o->chunks + c.first, c.second - c.first, o->partial, l, kNormGroups * o->launches, total, o->st, grad_scale, max_norm, norm_dev};
-            hipLaunchKernelGGL(adamw_norm_kernel, dim3(groups(l)), dim3(256), 0, st, na, ga);
+            NormArgs na{o->chunks + c.first, c.second - c.first, o->partial, l, kNormGroups * o->launches, at, total, type_of(l), o->st, grad_scale, max_norm, norm_dev};
+            if (o->chunk_blocks == kChunkBlocks) hipLaunchKernelGGL(adamw_norm_kernel<kChunkBlocks / 4>, dim3(groups(l)), dim3(256), 0, st, na, ga);
+            else hipLaunchKernelGGL(adamw_norm_kernel<kSmallBlocks / 4>, dim3(groups(l)), dim3(256), 0, st, na, ga);
         }
     }
     int last = -1;
@@ -534,8 +576,14 @@ int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_ty
         const auto c = fill(l);
         if (c.second == c.first) continue;
         StepArgs sa{o->chunks + c.first, o->m, o->v, o->ms, o->vs, o->st, lr, beta1, beta2, (float)eps, (float)grad_scale, max_norm > 0, l == last};
-        if (o->bits == 32) hipLaunchKernelGGL(adamw_kernel<32>, dim3(c.second - c.first), dim3(256), 0, st, sa, ga);
-        else hipLaunchKernelGGL(adamw_kernel<8>, dim3(c.second - c.first), dim3(256), 0, st, sa, ga);
+        const dim3 grid(c.second - c.first);
+        if (o->chunk_blocks == kChunkBlocks) {
+            if (o->bits == 32) hipLaunchKernelGGL((adamw_kernel<32, kChunkBlocks / 4>), grid, dim3(256), 0, st, sa, ga);
+            else hipLaunchKernelGGL((adamw_kernel<8, kChunkBlocks / 4>), grid, dim3(256), 0, st, sa, ga);
+        } else {
+            if (o->bits == 32) hipLaunchKernelGGL((adamw_kernel<32, kSmallBlocks / 4>), grid, dim3(256), 0, st, sa, ga);
+            else hipLaunchKernelGGL((adamw_kernel<8, kSmallBlocks / 4>), grid, dim3(256), 0, st, sa, ga);
+        }
     }
     SCS_HIP(hipGetLastError());
     return SCS_OK;

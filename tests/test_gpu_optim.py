@@ -127,6 +127,22 @@ def test_same_bits_as_the_formulas(handle, bits, pt, gt, offset, clip, master):
     opt.close()
 
 
+@pytest.mark.parametrize('bits,pt,gt', [(32, 'f32', 'f32'), (8, 'bf16', 'bf16'), (8, 'f32', 'f16')])
+def test_many_chunks_give_the_same_bits(handle, bits, pt, gt):
+    """Enough elements for the larger chunks, with tensors that end inside them."""
+    sizes = [8400000, 4097, 1, 300001]
+    params = make(sizes, TYPES[pt], 2, 1)
+    opt = AdamW(handle, params, state_bits=bits, max_norm=1.0)
+    refs = [Ref(p.float().cpu().numpy(), TYPES[pt], bits, 0.01, False) for p in params]
+    for t in (1, 2):
+        grads = gradients(sizes, TYPES[gt], 40 + t)
+        gs, _ = gscale_of(grads, 1.0, 1.0)
+        opt.step(grads)
+        for r, g in zip(refs, grads):
+            r.step(g.float().cpu().numpy(), t, 1e-3, 0.9, 0.999, 1e-8, gs)
+    check_same(opt, refs, params)
+
+
 def test_against_float64(handle):
     """One step in 32 bits.  In units of 2^-24, counted along the formula (each constant and each operation one): m 5 (b1 |m| + c1 |g|) =: 5 M,
     v 8 relative, the denominator 8 relative, p 3 |p| + 18 size M / denominator."""
@@ -171,6 +187,20 @@ def test_eight_bit_codes_are_the_nearest_values(handle):
     for b in range(n // BLOCK):
         i = b * BLOCK + int(np.argmax(wm[b * BLOCK:(b + 1) * BLOCK]))
         assert abs(abs(m[i]) - wm[i]) <= 8 * U * wm[i]
+
+
+def test_gradients_of_several_types_in_one_step(handle):
+    sizes = [5000, 300, 70000]
+    params = make(sizes, torch.float32, 21)
+    opt = AdamW(handle, params, max_norm=0.5)
+    refs = [Ref(p.cpu().numpy(), torch.float32, 32, 0.01, False) for p in params]
+    grads = [g.to(t) for g, t in zip(gradients(sizes, torch.float32, 22), (torch.float32, torch.bfloat16, torch.float16))]
+    gs, norm = gscale_of(grads, 1.0, 0.5)
+    opt.step(grads)
+    assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+    for r, g in zip(refs, grads):
+        r.step(g.float().cpu().numpy(), 1, 1e-3, 0.9, 0.999, 1e-8, gs)
+    check_same(opt, refs, params)
 
 
 def test_zero_and_tiny_blocks(handle):
@@ -301,6 +331,10 @@ def test_refusals(handle):
         opt.step([g], lr=float('nan'))
     with pytest.raises(ValueError):
         AdamW(handle, [p], states=(torch.zeros((10,), device='cuda:0'), torch.zeros((256,), device='cuda:0'), None, None))
+    opt.step([g])
+    p.data = torch.zeros((10,), device='cuda:0')
+    with pytest.raises(RuntimeError, match='moved'):
+        opt.step([g])
     opt.close()
     with pytest.raises(RuntimeError, match='closed'):
         opt.step([g])
