@@ -1,9 +1,9 @@
 // The shared projection on the f32 matrix cores for many rows (scs_lowrank.hip): the pipeline of lowrank_tiles.h
-// (four slabs of LDS, copies in flight across barriers, the next slab's fragments read while this one is multiplied) with exact f32 products.
+// (slabs of LDS, copies in flight across barriers, the next slab's fragments read while this one is multiplied) with exact f32 products.
 //
 // What bounds it: v_mfma_f32_16x16x4_f32, 32 cycles each on the vector ALUs, which every other vector instruction takes time from: so the copies
 // go to LDS without passing registers and addresses are a uniform base and a fixed offset a lane.  A workgroup of four waves owns
-// 64 MT rows x 16 NT columns (16 MT rows a wave), two workgroups a CU; NT is chosen for the least padding (540 columns: 5 x 112).
+// 64 MT rows x 16 NT columns (16 MT rows a wave),
 // LDS images of a slab of 16 along the contraction, in 16-byte pieces:
 //   K-major [row][16]: piece c of a row at c ^ (row >> 2 & 3); a lane's piece is its operand of four products.  X, and W^T in the backward pass
 //   N-major [16][BN]:  column n of row k at (n + 16 (k >> 2)) mod BN, so that a fragment's four rows lie at different banks.  W, and P
@@ -19,8 +19,8 @@ __device__ __forceinline__ void copy_to_lds(const void* src, unsigned int lds) {
 
 // EVEN: N is a multiple of 4
 template <int MT, int NT, bool TRANS, bool EVEN>
-__global__ __launch_bounds__(256, 2) void project_tiles32_kernel(ProjectArgs<float> g) {
-    constexpr int BM = 64 * MT, BN = 16 * NT, BK = 16, STAGES = 4, NP = BN / 4, LOADS = MT + 2;
+__global__ __launch_bounds__(256, NT <= 6 ? 3 : 2) void project_tiles32_kernel(ProjectArgs<float> g) {
+    constexpr int BM = 64 * MT, BN = 16 * NT, BK = 16, STAGES = 3, NP = BN / 4, LOADS = MT + 2;
     __shared__ __attribute__((aligned(16))) float s_a[STAGES][BM * BK];
     __shared__ __attribute__((aligned(16))) float s_b[STAGES][512 * 4];           // (BN <= 128; what lies behind a slab's end is never read)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);

@@ -461,11 +461,12 @@ int wgrad_block_rows(const scs_lowrank& p) {
 
 // ---- few rows (lowrank_few.h)
 struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; int tickets = 0; };      // mt 0: the tile kernels
-// f32 tiles (lowrank_tiles32.h): columns / 16 of the tile with the least padding, the widest among equals
+// f32 tiles (lowrank_tiles32.h): columns / 16 of the tile with the least padding; among equals the one that ran fastest at 60 000 x 540 x 540 (6: 306 us,
+// 5: 303, 7: 321, 4: 322; 8 pads there)
 int f32_columns(int64_t N) {
     int nt = 0;
     int64_t waste = INT64_MAX;
-    for (const int n : {8, 7, 6, 5, 4}) {
+    for (const int n : {6, 5, 8, 7, 4}) {
         const int64_t w = (N + 16 * n - 1) / (16 * n) * 16 * n;
         if (w < waste) { waste = w; nt = n; }
     }
