@@ -154,14 +154,19 @@ template <class T> struct Cols16 {
     }
 };
 
+// LDS of the join: [wave][row][16 columns' quarters + 1], so that neither side of it meets a bank twice
+template <int MT> struct FewShared { f32x4 part[kFewWaves][MT * 16][17]; bool last; };
+struct FewGrid { int tiles_n, tiles_m, splits; };
+
+// workgroup `id` of grid.tiles_n x grid.tiles_m x grid.splits
 template <class T, int MT, bool TRANS>
-__global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs<T> g, const int* __restrict__ row_adapter, int splits, float* part, unsigned int* tickets) {
+__device__ __forceinline__ void project_few(const ProjectArgs<T>& g, const int* __restrict__ row_adapter, const FewGrid& grid, float* part, unsigned int* tickets, int id,
+                                            FewShared<MT>& sh) {
     typedef FewStep<T, MT, TRANS> Step;
-    __shared__ f32x4 s_part[kFewWaves][MT * 16][17];             // [row][16 columns' quarters + 1]: neither side of the join meets a bank twice
-    __shared__ bool s_last;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, kq = lane >> 4;
-    const int n0 = blockIdx.x * 64, m0 = blockIdx.y * MT * 16, split = blockIdx.z;
+    const int bn = id % grid.tiles_n, bm = id / grid.tiles_n % grid.tiles_m, split = id / (grid.tiles_n * grid.tiles_m), splits = grid.splits;
+    const int n0 = bn * 64, m0 = bm * MT * 16;
     const Requests& r = g.r;
 
     f32x4 acc[MT][4];
@@ -223,9 +228,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s_part[wave][i * 16 + lr][4 * kq + e] = f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
+        for (int e = 0; e < 4; ++e) sh.part[wave][i * 16 + lr][4 * kq + e] = f32x4{acc[i][0][e], acc[i][1][e], acc[i][2][e], acc[i][3][e]};
     __syncthreads();
-    const int ldp = gridDim.x * 64, plane = gridDim.y * MT * 16 * ldp;               // partial sums of one split, whole tiles
+    const int ldp = grid.tiles_n * 64, plane = grid.tiles_m * MT * 16 * ldp;               // partial sums of one split, whole tiles
     const __amdgpu_buffer_rsrc_t pb = part_buffer(part, (int64_t)splits * plane * 4);
     auto finish = [&](f32x4 v, int m, int n) {
         float b[4] = {};
@@ -241,9 +246,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
     for (int row = tid >> 4; row < MT * 16; row += 4 * kFewWaves) {
         const int m = m0 + row;
         if (m >= r.rows || n >= g.N || row_adapter[m] == -2) continue;
-        f32x4 v = s_part[0][row][c4];
+        f32x4 v = sh.part[0][row][c4];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; ++w) v += s_part[w][row][c4];
+        for (int w = 1; w < kFewWaves; ++w) v += sh.part[w][row][c4];
         if (splits == 1) finish(v, m, n);
         else coherent_store(pb, split * plane + m * ldp + n, v);
     }
@@ -251,9 +256,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
     stores_done();
     __syncthreads();
     if (tid == 0)
-        s_last = __hip_atomic_fetch_add(&tickets[blockIdx.y * gridDim.x + blockIdx.x], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned int)splits - 1;
+        sh.last = __hip_atomic_fetch_add(&tickets[bm * grid.tiles_n + bn], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned int)splits - 1;
     __syncthreads();
-    if (!s_last) return;
+    if (!sh.last) return;
     for (int row = tid >> 4; row < MT * 16; row += 4 * kFewWaves) {
         const int m = m0 + row;
         if (m >= r.rows || n >= g.N || row_adapter[m] == -2) continue;
@@ -262,6 +267,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs
         for (int i = 1; i < splits; ++i) v += coherent_load(pb, i * plane + m * ldp + n);
         finish(v, m, n);
     }
+}
+
+template <class T, int MT, bool TRANS>
+__global__ __launch_bounds__(64 * kFewWaves) void project_few_kernel(ProjectArgs<T> g, const int* __restrict__ row_adapter, FewGrid grid, float* part, unsigned int* tickets) {
+    __shared__ FewShared<MT> sh;
+    project_few<T, MT, TRANS>(g, row_adapter, grid, part, tickets, blockIdx.x, sh);
 }
 
 }  // namespace

@@ -220,7 +220,11 @@ __global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ 
     for (int i = (blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < n_tickets; i += gridDim.x * gridDim.y * 256) tickets[i] = 0;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int row = blockIdx.x, j0 = blockIdx.y * 4;
+    const T* xr = x + (int64_t)row * ldx;
+    const int per = (K + 2047) / 2048 * 512, k_lo = wave * per + lane * 8, k_hi = min(K, (wave + 1) * per);
     Walk walk(r, row, row + 1);
+    float first[8];                                     // the row's first piece, on its way while its request is looked up
+    load8f(xr + min(k_lo, K - 1), k_lo < k_hi ? K - k_lo : 0, first);
     int q;
     Span sp;
     const bool owned = walk.next(q, sp);
@@ -228,13 +232,14 @@ __global__ __launch_bounds__(256) void shrink_dots_kernel(const T* __restrict__ 
     if (!owned) return;
     float sum[4] = {};
     if (sp.s >= 0) {
-        const T* xr = x + (int64_t)row * ldx;
         const T* pr = p + ((int64_t)sp.s * r.rank + j0) * K;
-        const int per = (K + 2047) / 2048 * 512, k_hi = min(K, (wave + 1) * per);
 #pragma unroll 2
-        for (int k = wave * per + lane * 8; k < k_hi; k += 512) {
+        for (int k = k_lo; k < k_hi; k += 512) {
             float a[8], b[4][8];
-            load8f(xr + k, K - k, a);
+            if (k == k_lo)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) a[i] = first[i];
+            else load8f(xr + k, K - k, a);
 #pragma unroll
             for (int j = 0; j < 4; ++j) load8f(pr + (int64_t)min(j, r.rank - 1 - j0) * K + k, K - k, b[j]);
 #pragma unroll
@@ -302,8 +307,8 @@ namespace {
 
 // ------------------------------------------------------------------------------------------------------------------ wgrad
 // G_s[j][k] = scale_s sum over the rows of s of H[row][j] X[row][k], f32: reading X once is the work.  A workgroup owns 64 columns; a lane's
-// vector of X (four columns of a row) is its operand of four f32 products (columns 4 c + t of product t), its four waves take every fourth
-// group of sixteen rows and are joined through LDS in a fixed order.  dA and dB are one launch.
+// vector of X (four columns of a row) is its operand of four f32 products (columns 4 c + t of product t), its waves take the rows in
+// turn, sixteen at a time, and are joined through LDS in a fixed order.  dA and dB are one launch.
 //   by blocks: a workgroup owns a block of rows as well and leaves one partial sum for each request in it, in slot request + block (along the
 //              rows one of the two grows from each partial sum to the next: no slot is met twice); wgrad_join_kernel adds an adapter's slots up
 //   direct:    a workgroup owns one adapter and walks its requests (few rows, or requests so many that their slots would outweigh X)
@@ -311,10 +316,10 @@ template <class T> struct WgradProblem { const float* h; const T* x; int64_t ldx
 template <class T> struct WgradArgs { WgradProblem<T> p[2]; int32_t block_rows; Requests r; };
 
 // rows [lo, hi) of one request into the accumulators
-template <class T, int JT> __device__ __forceinline__ void wgrad_rows(const WgradProblem<T>& w, const Requests& r, int col, int lo, int hi, int wave, f32x4 (&acc)[JT][4]) {
+template <class T, int JT, int W> __device__ __forceinline__ void wgrad_rows(const WgradProblem<T>& w, const Requests& r, int col, int lo, int hi, int wave, f32x4 (&acc)[JT][4]) {
     constexpr int UNROLL = JT <= 2 ? 4 : 2;
     const int lane = threadIdx.x & 63, lr = lane & 15, kq = lane >> 4, left = w.F - col;
-    for (int b = lo + wave * 4 * UNROLL; b < hi; b += 16 * UNROLL) {
+    for (int b = lo + wave * 4 * UNROLL; b < hi; b += 4 * W * UNROLL) {
         typename Vec4<T>::raw rx[UNROLL];
         float a[UNROLL][JT];
 #pragma unroll
@@ -340,8 +345,8 @@ template <class T, int JT> __device__ __forceinline__ void wgrad_rows(const Wgra
         }
     }
 }
-// the four waves' sums, in their order, times sc, to out [rank][F]
-template <int JT> __device__ __forceinline__ void wgrad_store(float (&s_part)[3][JT * 16][64], const f32x4 (&acc)[JT][4], int wave, int rank, int F, int col, float sc, float* out) {
+// the waves' sums, in their order, times sc, to out [rank][F]
+template <int JT, int W> __device__ __forceinline__ void wgrad_store(float (&s_part)[W - 1][JT * 16][64], const f32x4 (&acc)[JT][4], int wave, int rank, int F, int col, float sc, float* out) {
     const int lane = threadIdx.x & 63, kq = lane >> 4, left = F - col;
     __syncthreads();
     if (wave) {
@@ -363,7 +368,10 @@ template <int JT> __device__ __forceinline__ void wgrad_store(float (&s_part)[3]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int at = t * 16 + i * 4 + e;
-                v[i] = sc * (((acc[t][i][e] + s_part[0][at][lane]) + s_part[1][at][lane]) + s_part[2][at][lane]);
+                float sum = acc[t][i][e];
+#pragma unroll
+                for (int w = 0; w < W - 1; ++w) sum += s_part[w][at][lane];
+                v[i] = sc * sum;
             }
             if (j < rank) raw_store<float>(v, out + (int64_t)j * F + col, left);
         }
@@ -390,17 +398,14 @@ __global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
         if (sp.s < 0) continue;
         f32x4 acc[JT][4];
         wgrad_clear<JT>(acc);
-        wgrad_rows<T, JT>(w, r, col, sp.lo, sp.hi, wave, acc);
-        wgrad_store<JT>(s_part, acc, wave, r.rank, w.F, col, 1.f, w.part + (int64_t)(q + blockIdx.y) * r.rank * w.F);
+        wgrad_rows<T, JT, 4>(w, r, col, sp.lo, sp.hi, wave, acc);
+        wgrad_store<JT, 4>(s_part, acc, wave, r.rank, w.F, col, 1.f, w.part + (int64_t)(q + blockIdx.y) * r.rank * w.F);
     }
 }
 
-template <class T, int JT>
-__global__ __launch_bounds__(256) void wgrad_direct_kernel(WgradArgs<T> g) {
-    __shared__ float s_part[3][JT * 16][64];
-    const WgradProblem<T>& w = g.p[blockIdx.z];
-    const Requests& r = g.r;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.x * 64, col = c0 + 4 * (lane & 15), s = blockIdx.y;
+template <class T, int JT, int W>
+__device__ __forceinline__ void wgrad_direct(const WgradProblem<T>& w, const Requests& r, int tile, int s, float (&s_part)[W - 1][JT * 16][64]) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = tile * 64, col = c0 + 4 * (lane & 15);
     if (c0 >= w.F) return;
     f32x4 acc[JT][4];
     wgrad_clear<JT>(acc);
@@ -410,10 +415,36 @@ __global__ __launch_bounds__(256) void wgrad_direct_kernel(WgradArgs<T> g) {
         unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
         for (; todo; todo &= todo - 1) {
             const int at = __builtin_ctzll(todo);
-            wgrad_rows<T, JT>(w, r, col, __builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(hi, at), wave, acc);
+            wgrad_rows<T, JT, W>(w, r, col, __builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(hi, at), wave, acc);
         }
     }
-    wgrad_store<JT>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
+    wgrad_store<JT, W>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
+}
+
+template <int JT> constexpr int direct_waves() { return JT <= 2 ? kFewWaves : 4; }             // (the join's LDS)
+template <class T, int JT>
+__global__ __launch_bounds__(64 * direct_waves<JT>()) void wgrad_direct_kernel(WgradArgs<T> g) {
+    __shared__ float s_part[direct_waves<JT>() - 1][JT * 16][64];
+    wgrad_direct<T, JT, direct_waves<JT>()>(g.p[blockIdx.z], g.r, blockIdx.x, blockIdx.y, s_part);
+}
+
+// dx of few rows and the adapters' gradients in one launch: both follow from u alone, and neither fills the card (a mini-batch of 256 rows at 540 x
+// 540: 11 us together, 11 and 7 one after the other)
+template <class T, int MT, int JT>
+__global__ __launch_bounds__(64 * kFewWaves) void few_and_wgrad_kernel(ProjectArgs<T> g, const int* __restrict__ row_adapter, FewGrid grid, float* part, unsigned int* tickets,
+                                                                       WgradArgs<T> w, int tiles) {
+    __shared__ union Shared {
+        __device__ Shared() {}
+        FewShared<MT> few;
+        float part[kFewWaves - 1][JT * 16][64];
+    } sh;
+    const int few = grid.tiles_n * grid.tiles_m * grid.splits;
+    if ((int)blockIdx.x < few) {
+        project_few<T, MT, true>(g, row_adapter, grid, part, tickets, blockIdx.x, sh.few);
+        return;
+    }
+    const int id = blockIdx.x - few, tile = id % tiles, rest = id / tiles;
+    wgrad_direct<T, JT, kFewWaves>(w.p[rest / w.r.n_adapters], w.r, tile, rest % w.r.n_adapters, sh.part);
 }
 
 // an adapter's gradient from its requests' slots, in the order of the rows
@@ -449,13 +480,14 @@ constexpr int kDotRows = 512;               // up to so many rows the shrink is 
 
 size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows; direct where that
-// is one block, or where the slots (requests + blocks, rank f32 values a column each) would outweigh X's own rows.
+// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows; direct up to
+// 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank f32 values a column each) would outweigh X's own rows.
+constexpr int kDirectRows = 512;
 int wgrad_block_rows(const scs_lowrank& p) {
     const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
     const int64_t rows = std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64));
     const int64_t blocks = (p.rows + rows - 1) / rows;
-    if (blocks <= 1 || blocks > 65535 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
+    if (p.rows <= kDirectRows || blocks <= 1 || blocks > 65535 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
     return (int)rows;
 }
 
@@ -481,6 +513,7 @@ int f32_rows(int64_t rows, int64_t N) {
 // at 540 x 540: 18 us, as tiles 46)
 Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     Few f;
+    if (p.rows == 0) return f;
     if (p.dtype == SCS_F32 ? f32_rows(p.rows, N) != 0 : p.rows > 64) return f;
     f.mt = p.dtype == SCS_F32 ? (p.rows >= 256 && K * N >= (1 << 21) ? 2 : 1) : (int)(p.rows + 15) / 16;
     f.tiles_n = (int)((N + 63) / 64);
@@ -512,7 +545,7 @@ Pack pack_of(const scs_lowrank& p, int64_t K, int64_t N, bool trans, const void*
     return k;
 }
 
-struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, slots = 0, pieces = 0, pack_x = 0, pack_w = 0, bytes = 0; };
+struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, rows2 = 0, slots = 0, pieces = 0, pack_x = 0, pack_w = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward, const void* x, int64_t ldx) {
     Layout l;
     size_t at = 0;
@@ -524,6 +557,7 @@ Layout layout_of(const scs_lowrank& p, bool backward, const void* x, int64_t ldx
     l.rows = take((size_t)p.rows * 4);
     if (p.dtype != SCS_F32 && !f.mt) l.pieces = take((size_t)p.rows * ((p.rank + 15) / 16) * 64);
     if (backward) {
+        l.rows2 = take((size_t)p.rows * 4);
         l.hid2 = take((size_t)p.rows * p.rank * 4);
         if (const int b = wgrad_block_rows(p)) l.slots = take((size_t)(p.n_requests + (p.rows + b - 1) / b) * p.rank * (p.in_features + p.out_features) * 4);
     }
@@ -588,9 +622,11 @@ template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, co
     });
 }
 
-template <class T, bool TRANS> void project_few(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
-    const dim3 grid(f.tiles_n, f.tiles_m, f.splits);
-    auto go = [&](auto mt) { hipLaunchKernelGGL((project_few_kernel<T, mt.value, TRANS>), grid, dim3(64 * kFewWaves), 0, st, g, rows, f.splits, part, tickets); };
+template <class T, bool TRANS> void launch_few(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
+    const FewGrid grid{f.tiles_n, f.tiles_m, f.splits};
+    auto go = [&](auto mt) {
+        hipLaunchKernelGGL((project_few_kernel<T, mt.value, TRANS>), dim3(f.tiles_n * f.tiles_m * f.splits), dim3(64 * kFewWaves), 0, st, g, rows, grid, part, tickets);
+    };
     if (f.mt == 1) go(std::integral_constant<int, 1>{});
     else if (f.mt == 2) go(std::integral_constant<int, 2>{});
     else if constexpr (sizeof(T) == 2) {
@@ -623,7 +659,7 @@ template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T
 template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T> g, const Few& f, const int* rows, float* part, unsigned int* tickets, T* pack_x, T* pack_w,
                                             hipStream_t st) {
     g.nw = g.N;
-    if (f.mt) { project_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
+    if (f.mt) { launch_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
     const Pack k = pack_of(p, g.K, g.N, TRANS, g.x, g.ldx);
     PackArgs pa{};
     int n = 0;
@@ -651,7 +687,9 @@ template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&prob
     WgradArgs<T> g{{problems[0], problems[1]}, wgrad_block_rows(p), requests_of(p)};
     const int F = std::max(problems[0].F, n > 1 ? problems[1].F : 0), tiles = (F + 63) / 64;
     if (!g.block_rows) {
-        by_tiles(p.rank, [&](auto jt) { hipLaunchKernelGGL((wgrad_direct_kernel<T, jt.value>), dim3(tiles, p.n_adapters, n), dim3(256), 0, st, g); });
+        by_tiles(p.rank, [&](auto jt) {
+            hipLaunchKernelGGL((wgrad_direct_kernel<T, jt.value>), dim3(tiles, p.n_adapters, n), dim3(64 * direct_waves<jt.value>()), 0, st, g);
+        });
         return;
     }
     const int64_t blocks = (p.rows + g.block_rows - 1) / g.block_rows;
@@ -684,11 +722,10 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     const bool any = p.rows > 0 && p.n_requests > 0;          // (without rows dA and dB are zeros: the wgrad kernels write them)
     const Few f = few_of(p, p.out_features, p.in_features);
     int* rows = (int*)(ws + l.rows);
+    int* rows2 = (int*)(ws + l.rows2);                 // (of the second shrink: the same numbers)
     T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
     if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
-    if (dx)
-        project<T, true>(p, ProjectArgs<T>{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, 0, requests_of(p)},
-                         f, rows, part, (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
+    const ProjectArgs<T> back{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, 0, requests_of(p)};
     WgradProblem<T> w[2]{};
     int n = 0;
     if (da) w[n++] = WgradProblem<T>{u, (const T*)x, ldx, da, nullptr, (int)p.in_features};
@@ -696,11 +733,28 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         const float* h = hidden;
         if (!h) {
             h = (float*)(ws + l.hid2);
-            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), (T*)nullptr, st, rows);
+            if (any) shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, (float*)(ws + l.hid2), (T*)nullptr, st, rows2);
         }
         w[n++] = WgradProblem<T>{h, (const T*)dy, lddy, db, nullptr, (int)p.out_features};
     }
-    if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st);
+    if (dx && n && f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && !wgrad_block_rows(p)) {
+        const int tiles = (std::max(w[0].F, n > 1 ? w[1].F : 0) + 63) / 64;
+        const FewGrid grid{f.tiles_n, f.tiles_m, f.splits};
+        ProjectArgs<T> g = back;
+        g.nw = g.N;
+        const WgradArgs<T> wa{{w[0], w[1]}, 0, requests_of(p)};
+        const dim3 all((unsigned)(f.tiles_n * f.tiles_m * f.splits + tiles * p.n_adapters * n));
+        auto go = [&](auto mt, auto jt) {
+            hipLaunchKernelGGL((few_and_wgrad_kernel<T, mt.value, jt.value>), all, dim3(64 * kFewWaves), 0, st, g, rows, grid, part, (unsigned int*)(ws + l.tickets), wa, tiles);
+        };
+        typedef std::integral_constant<int, 1> One;
+        typedef std::integral_constant<int, 2> Two;
+        if (f.mt == 1) { if (p.rank <= 16) go(One{}, One{}); else go(One{}, Two{}); }
+        else { if (p.rank <= 16) go(Two{}, One{}); else go(Two{}, Two{}); }
+    } else {
+        if (dx) project<T, true>(p, back, f, rows, part, (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
+        if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st);
+    }
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }

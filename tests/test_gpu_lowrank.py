@@ -326,6 +326,18 @@ def test_row_offsets_beyond_32_bits(handle, ld):
     assert all(torch.equal(a, b) for a, b in zip(g, ref))
 
 
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+def test_no_rows(handle, t):
+    d, _, _ = some(t, 8)
+    p = Projection(handle, d['w'], d['a'], d['b'])
+    for off, ids in (([0], []), ([0, 0, 0], [1, -1])):
+        o, i = requests(off, ids)
+        x, dy = d['x'][:0], d['dy'][:0]
+        assert p.forward(x, o, i).shape == (0, 200)
+        dx, da, db = p.backward(x, dy, o, i, da=torch.ones((3, 8, 96), device='cuda:0'), db=torch.ones((3, 8, 200), device='cuda:0'))
+        assert dx.shape == (0, 96) and not da.any() and not db.any()
+
+
 def test_refusals(handle):
     d, off, ids = some('bf16')
     o, i = requests(off, ids)
