@@ -256,6 +256,12 @@ class SiteAdapters:
             self.tensors += [a, d]
             self.names += [name + '.a', name + '.b']
 
+    def set_weights(self, params):
+        """The shared weights of another parameter dict, into the layers' own tensors."""
+        for name, layer in zip(self.LAYERS, self.layers):
+            for t, a in zip((layer.w, layer.bias), params[name]):
+                t.copy_(self._torch.from_numpy(np.array(a, dtype=np.float32, order='C')))
+
     def state_dict(self):
         """Host arrays: scale, <layer>.a, <layer>.b."""
         d = {n: t.cpu().numpy() for n, t in zip(self.names, self.tensors)}

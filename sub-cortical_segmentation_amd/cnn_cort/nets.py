@@ -140,6 +140,7 @@ class Net:
         self.optimizer, self.weight_decay = optimizer, float(weight_decay)
         self.optimizer_bits, self.max_norm = int(optimizer_bits), None if max_norm is None else float(max_norm)
         self.adapters = None         # SiteAdapters (fit_adapters, load_adapters_from)
+        self._adapters_behind = False                # the shared weights have changed since the adapters' layers took them
         self.seed = int(seed)
         self.device = device
         self.train_history_ = []
@@ -207,6 +208,7 @@ class Net:
         else:
             params = P.check_params({k: [np.asarray(a, np.float32) for a in v] for k, v in source.items()})
         self._params = params
+        self._adapters_behind = True
         self._dirty = True
         self._dev_newer = False
         return self
@@ -376,6 +378,11 @@ class Net:
             raise RuntimeError('no site adapters: fit_adapters or load_adapters_from first')
         n = self._check_X(X)
         sites = self._check_sites(sites, n, self.adapters.sites)
+        if self._adapters_behind:                    # (fit or load_params_from since: the head's shared weights are the net's)
+            self._ensure_handle()
+            self._sync_host()
+            self.adapters.set_weights(self._params)
+            self._adapters_behind = False
         order, offsets, ids = group_rows(sites)
         dev = self.adapters.device
         back = torch.from_numpy(order).to(dev)
@@ -453,7 +460,7 @@ class Net:
             for t, b in zip(ad.tensors, best_state):
                 t.copy_(b)
         opt.close()
-        self.adapters = ad
+        self.adapters, self._adapters_behind = ad, False
         return history
 
     def save_adapters_to(self, path):
@@ -475,7 +482,7 @@ class Net:
         h = self._ensure_handle()
         self._sync_host()
         sites, rank = state['FC1.a'].shape[:2]
-        self.adapters = SiteAdapters(h, self._params, sites, rank=rank, state=state)
+        self.adapters, self._adapters_behind = SiteAdapters(h, self._params, sites, rank=rank, state=state), False
         return self
 
     def _wait(self, stream=None):
@@ -914,6 +921,7 @@ class Net:
         adamw = self._adamw(h) if self.optimizer == 'adamw' else None
         fused = adamw is None and not dist.is_dist()
         h.set_fused_adam(fused, lr=self.update_learning_rate)
+        self._adapters_behind = True
         try:
             for ep in range(epochs or self.max_epochs):
                 t0 = time.time()

@@ -205,3 +205,22 @@ def test_fit_with_adamw_is_the_two_calls(weights, bits, clip):
 def test_optimizer_options():
     with pytest.raises(ValueError, match='optimizer'):
         Net(optimizer='sgd')
+
+
+def test_new_weights_reach_the_adapted_head(weights, batch):
+    """load_params_from and fit change the shared weights: predict with sites takes the new ones."""
+    X, y, sites = batch
+    net = make_net(weights)
+    h = net._ensure_handle()
+    h.set_option('fwd_split', 0)
+    net.adapters = SiteAdapters(h, net.get_all_params_values(), 3, rank=4)
+    other = {k: [a * np.float32(0.5) for a in v] if k in SiteAdapters.LAYERS else v for k, v in net.get_all_params_values().items()}
+    net.load_params_from(other)
+    net._ensure_handle().set_option('fwd_split', 0)
+    base = net.predict_proba(X)
+    assert np.abs(net.predict_proba(X, sites=-1) - base).max() < 1e-4
+    net.max_epochs, net.eval_size, net.batch_size = 1, 0.0, 64
+    net.fit(X, y)
+    fitted = net.predict_proba(X)
+    assert np.abs(fitted - base).max() > 1e-3
+    assert np.abs(net.predict_proba(X, sites=sites) - fitted).max() < 1e-4
