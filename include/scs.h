@@ -338,15 +338,15 @@ int scs_eval_batch(scs_handle h, const float* ax_dev, const float* co_dev, const
  *   forward   y_i = x_i W + bias + scale_s (x_i A_s^T) B_s
  *   backward  dx_i = dy_i W^T + u_i A_s,  u_i = scale_s dy_i B_s^T;   dA_s = sum_i u_i^T x_i;   dB_s = scale_s sum_i (x_i A_s^T)^T dy_i
  * over the rows of all requests that use s (an adapter that none uses gets zeros).  W and bias are shared and fixed: no gradients of them.
- * Products are summed in f32 whatever the type, x_i A_s^T is kept in f32, and each output is rounded once; for 16-bit types the adapters'
- * products scale_s x_i A_s^T (u_i) enter the matrix cores as two 16-bit pieces.
+ * Products are summed in f32 whatever the type, x_i A_s^T is kept in f32, and each output is rounded once; in bf16 calls of many rows
+ * scale_s x_i A_s^T (u_i) enters the matrix cores as two bf16 pieces (2^-17 of it is lost).
  * Beside the net's dense layers (nets.py:179, 217, 227): W in (in, out) order, as the parameter arena holds it. */
 typedef struct {
     int32_t dtype;                 /* SCS_F32, SCS_BF16 or SCS_F16: x, W, bias, A, B, y, dy, dx */
     int32_t rank;                  /* 1..128; adapters of lower rank are filled up with zeros */
     int32_t n_adapters;            /* 1..65535 */
     int32_t n_requests;            /* 0..2^24 */
-    int64_t rows;                  /* rows of x, y, dy, dx: 0..2^30 */
+    int64_t rows;                  /* rows of x, y, dy, dx: 0..2^26 */
     int64_t in_features, out_features;      /* 1..2^20 each */
     int64_t ldw;                   /* row stride of W in elements, >= out_features */
     const void* w;                 /* [in][out] */

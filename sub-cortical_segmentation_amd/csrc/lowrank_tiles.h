@@ -174,7 +174,8 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     copies_but<0>();                                                     // (none may land in LDS that holds something else by then)
     workgroup_barrier();
 
-    // the adapters: 16 directions a pass, scale_s H as its upper and lower 16-bit piece side by side along the contraction, P's rows repeated
+    // the adapters, 16 directions a pass.  bf16: scale_s H as its upper and lower 16-bit piece side by side along the contraction, P's rows
+    // repeated.  f16: on the f32 matrix cores, because scale_s H may lie outside f16's range (or among its smallest steps) where Y does not
     const int m1 = min(m0 + BM, r.rows), mw = m0 + wm * MT * 16;
     auto frag_x_at = [&](int lr, int kq, int tile) { return *(const v8*)&s_a[0][(tile * 16 + lr) * BK + ((kq ^ (lr >> 2)) * 8)]; };
     auto frag_n_at = [&](int lr, int kq, int tile) {
@@ -195,35 +196,70 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
             // (opaque copies: addresses formed from them are formed here, not kept in registers beside the sums from the kernel's start on)
             int tid = threadIdx.x, lr = tid & 15, kq = (tid >> 4) & 3;
             asm volatile("" : "+v"(tid), "+v"(lr), "+v"(kq));
-            for (int e = tid; e < BM * 4; e += THREADS) {
-                const int m = e >> 2, c = e & 3, row = m0 + m;
-                const u32x4* at = (const u32x4*)(g.pieces + ((int64_t)min(row, r.rows - 1) * ((r.rank + 15) / 16) + j0 / 16) * 32) + c;
-                const u32x4 v = *at;
-                const bool in = row >= sp.lo && row < sp.hi;
-                *(u32x4*)&s_a[0][m * BK + ((c ^ ((m >> 2) & 3)) * 8)] = in ? v : u32x4{0, 0, 0, 0};
-            }
-            for (int e = tid; e < 16 * NP; e += THREADS) {
-                const int k = e / NP, c = e % NP, j = j0 + k;
+            auto piece_of_p = [&](int j, int c) {
                 const T* at_p = ps + (int64_t)min(j, r.rank - 1) * g.N;
                 const u32x4 v = EVEN ? at16(at_p + min(n0 + c * 8, g.N - 8)) : load8(at_p + n0 + c * 8, g.N - (n0 + c * 8));
-                const u32x4 w = j < r.rank ? v : u32x4{0, 0, 0, 0};
-                const int f = ((k & 3) | ((k >> 3) & 1) << 2) & UNITS, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
-                *(u32x4*)&s_b[0][k * BN + at] = w;
-                *(u32x4*)&s_b[0][(k + 16) * BN + at] = w;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                const v8 w = frag_n_at(lr, kq, wn * NT + j);
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    const f32x4 part = mfma16(w, frag_x_at(lr, kq, wm * MT + i), f32x4{0.f, 0.f, 0.f, 0.f});
-                    const int row = mw + i * 16 + lr;
-                    const bool in = row >= sp.lo && row < sp.hi;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j][e] += in ? part[e] : 0.f;
+                return j < r.rank ? v : u32x4{0, 0, 0, 0};
+            };
+            if constexpr (sizeof(T) == 2 && !kPieces<T>) {
+                float* s_h = (float*)&s_a[0][0];                        // [row][16], direction j at j + row
+                const float sc = walk.scale(sp);
+                for (int e = tid; e < BM * 16; e += THREADS) {
+                    const int m = e >> 4, j = j0 + (e & 15), row = m0 + m;
+                    const bool in = row >= sp.lo && row < sp.hi && j < r.rank;
+                    s_h[m * 16 + ((j + m) & 15)] = in ? sc * g.h[(int64_t)row * r.rank + j] : 0.f;
                 }
-                __builtin_amdgcn_sched_barrier(0);                      // (all columns' partial products at once do not fit beside the sums)
+                for (int e = tid; e < 16 * NP; e += THREADS) {
+                    const int k = e / NP, c = e % NP;
+                    *(u32x4*)&s_b[0][k * BN + ((((c >> 1) ^ (k & 3)) << 1) | (c & 1)) * 8] = piece_of_p(j0 + k, c);
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    float w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) w[k] = to_f32(s_b[0][(4 * k + kq) * BN + (((wn * NT + j) ^ kq) << 4) + lr]);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const int m = (wm * MT + i) * 16 + lr, row = m0 + m;
+                        f32x4 part = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) part = __builtin_amdgcn_mfma_f32_16x16x4f32(w[k], s_h[m * 16 + ((4 * k + kq + m) & 15)], part, 0, 0, 0);
+                        const bool in = row >= sp.lo && row < sp.hi;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] += in ? part[e] : 0.f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                for (int e = tid; e < BM * 4; e += THREADS) {
+                    const int m = e >> 2, c = e & 3, row = m0 + m;
+                    const u32x4* at = (const u32x4*)(g.pieces + ((int64_t)min(row, r.rows - 1) * ((r.rank + 15) / 16) + j0 / 16) * 32) + c;
+                    const u32x4 v = *at;
+                    const bool in = row >= sp.lo && row < sp.hi;
+                    *(u32x4*)&s_a[0][m * BK + ((c ^ ((m >> 2) & 3)) * 8)] = in ? v : u32x4{0, 0, 0, 0};
+                }
+                for (int e = tid; e < 16 * NP; e += THREADS) {
+                    const int k = e / NP, c = e % NP, j = j0 + k;
+                    const u32x4 w = piece_of_p(j, c);
+                    const int f = ((k & 3) | ((k >> 3) & 1) << 2) & UNITS, at = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;       // (the same for row k + 16)
+                    *(u32x4*)&s_b[0][k * BN + at] = w;
+                    *(u32x4*)&s_b[0][(k + 16) * BN + at] = w;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const v8 w = frag_n_at(lr, kq, wn * NT + j);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        const f32x4 part = mfma16(w, frag_x_at(lr, kq, wm * MT + i), f32x4{0.f, 0.f, 0.f, 0.f});
+                        const int row = mw + i * 16 + lr;
+                        const bool in = row >= sp.lo && row < sp.hi;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][e] += in ? part[e] : 0.f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);                      // (all columns' partial products at once do not fit beside the sums)
+                }
             }
             __syncthreads();
         }

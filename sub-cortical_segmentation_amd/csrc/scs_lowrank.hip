@@ -11,6 +11,7 @@
 // A row's request is found from the offsets inside the kernels.  A 16-row tile that several requests share is multiplied with each one's
 // adapter, and every product is added under the mask of its own rows: an adapter that holds infinities touches its own requests only.
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "scs_ops.h"
@@ -95,10 +96,10 @@ template <class T> __device__ __forceinline__ f32x4 product16(const u32x4& a, co
     }
 }
 
-// a value as the nearest 16-bit one and what is left of it (bf16: 2^-17 of the value is lost, f16: 2^-23 down to its smallest steps).  Beyond f16's
-// range the upper piece is infinite, as the value is in f16
+// a value as the nearest bf16 one and what is left of it (2^-17 of the value is lost)
+template <class T> constexpr bool kPieces = std::is_same<T, __bf16>::value;
 template <class T> __device__ __forceinline__ void write_pieces(T* pieces, int64_t row, int j, int rank, float v) {
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (kPieces<T>) {
         T* at = pieces + (row * ((rank + 15) / 16) + j / 16) * 32 + j % 16;
         const T hi = from_f32<T>(v);
         const float up = to_f32(hi);
@@ -273,7 +274,7 @@ struct ProjectArgs {
     const T* bias;
     const T* low;                     // P: [n_adapters][rank][N]
     const float* h;                   // [rows][rank]
-    const T* pieces;                  // 16-bit types, many rows: scale_s h as two 16-bit pieces, [rows][ceil(rank / 16)][16 upper | 16 lower]
+    const T* pieces;                  // bf16, many rows: scale_s h as two pieces, [rows][ceil(rank / 16)][16 upper | 16 lower]
     T* y; int64_t ldy;
     int32_t K, N;
     int32_t nw;                       // columns of W's rows that can be read (N-major W: N, or more where it was laid out anew)
@@ -315,9 +316,10 @@ namespace {
 template <class T> struct WgradProblem { const float* h; const T* x; int64_t ldx; float* out; float* part; int32_t F; };
 template <class T> struct WgradArgs { WgradProblem<T> p[2]; int32_t block_rows; Requests r; };
 
+template <int JT> constexpr int kWgradRows = JT <= 2 ? 16 : 8;               // rows that a wave takes at once
 // rows [lo, hi) of one request into the accumulators
 template <class T, int JT, int W> __device__ __forceinline__ void wgrad_rows(const WgradProblem<T>& w, const Requests& r, int col, int lo, int hi, int wave, f32x4 (&acc)[JT][4]) {
-    constexpr int UNROLL = JT <= 2 ? 4 : 2;
+    constexpr int UNROLL = kWgradRows<JT> / 4;
     const int lane = threadIdx.x & 63, lr = lane & 15, kq = lane >> 4, left = w.F - col;
     for (int b = lo + wave * 4 * UNROLL; b < hi; b += 4 * W * UNROLL) {
         typename Vec4<T>::raw rx[UNROLL];
@@ -409,13 +411,16 @@ __device__ __forceinline__ void wgrad_direct(const WgradProblem<T>& w, const Req
     if (c0 >= w.F) return;
     f32x4 acc[JT][4];
     wgrad_clear<JT>(acc);
+    int turn = 0;                                             // (requests of a row or two each: the waves take them in turn)
     for (int q0 = 0; q0 < r.n; q0 += 64) {
         const int q = q0 + lane, c = min(q, r.n - 1);
         const int lo = clamp_row(r.offsets[c], r.rows), hi = clamp_row(r.offsets[c + 1], r.rows);
         unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
         for (; todo; todo &= todo - 1) {
             const int at = __builtin_ctzll(todo);
-            wgrad_rows<T, JT, W>(w, r, col, __builtin_amdgcn_readlane(lo, at), __builtin_amdgcn_readlane(hi, at), wave, acc);
+            const int a = __builtin_amdgcn_readlane(lo, at), b = __builtin_amdgcn_readlane(hi, at);
+            wgrad_rows<T, JT, W>(w, r, col, a, b, (wave + W - turn) % W, acc);
+            turn = (turn + (b - a + kWgradRows<JT> - 1) / kWgradRows<JT>) % W;
         }
     }
     wgrad_store<JT, W>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
@@ -480,14 +485,15 @@ constexpr int kDotRows = 512;               // up to so many rows the shrink is 
 
 size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
 
-// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows; direct up to
-// 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank f32 values a column each) would outweigh X's own rows.
+// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows (more where a
+// grid's 65535 would not do); direct up to 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank
+// f32 values a column each) would hold more than four times X's own bytes.
 constexpr int kDirectRows = 512;
 int wgrad_block_rows(const scs_lowrank& p) {
     const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
-    const int64_t rows = std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64));
+    const int64_t rows = std::max<int64_t>(std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64)), (p.rows / 65535 + 64) / 64 * 64);
     const int64_t blocks = (p.rows + rows - 1) / rows;
-    if (p.rows <= kDirectRows || blocks <= 1 || blocks > 65535 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
+    if (p.rows <= kDirectRows || blocks <= 1 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
     return (int)rows;
 }
 
@@ -555,7 +561,7 @@ Layout layout_of(const scs_lowrank& p, bool backward, const void* x, int64_t ldx
     size_t part = f.part;
     l.tickets = take((size_t)f.tickets * 4);
     l.rows = take((size_t)p.rows * 4);
-    if (p.dtype != SCS_F32 && !f.mt) l.pieces = take((size_t)p.rows * ((p.rank + 15) / 16) * 64);
+    if (p.dtype == SCS_BF16 && !f.mt) l.pieces = take((size_t)p.rows * ((p.rank + 15) / 16) * 64);
     if (backward) {
         l.rows2 = take((size_t)p.rows * 4);
         l.hid2 = take((size_t)p.rows * p.rank * 4);
@@ -577,7 +583,7 @@ int check(const scs_lowrank* p) {
     SCS_ARG(p->rank >= 1 && p->rank <= 128, "rank lies in 1..128");
     SCS_ARG(p->n_adapters >= 1 && p->n_adapters <= 65535, "n_adapters lies in 1..65535");
     SCS_ARG(p->n_requests >= 0 && p->n_requests <= (1 << 24), "n_requests lies in 0..2^24");
-    SCS_ARG(p->rows >= 0 && p->rows <= (1 << 30), "rows lies in 0..2^30");
+    SCS_ARG(p->rows >= 0 && p->rows <= (1 << 26), "rows lies in 0..2^26");             // (a launch has at most 2^32 threads along x)
     SCS_ARG(p->in_features >= 1 && p->in_features <= (1 << 20) && p->out_features >= 1 && p->out_features <= (1 << 20), "features lie in 1..2^20");
     SCS_ARG(p->ldw >= p->out_features, "ldw is below out_features");
     SCS_ARG(p->w && p->a && p->b && p->offsets && (p->adapters || p->n_requests == 0), "a table is NULL");
@@ -705,7 +711,7 @@ int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t l
     float* h = hidden ? hidden : (float*)(ws + l.hid);
     const Few f = few_of(p, p.in_features, p.out_features);
     int* rows = (int*)(ws + l.rows);
-    T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
+    T* pieces = kPieces<T> && !f.mt ? (T*)(ws + l.pieces) : nullptr;
     shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     project<T, false>(p, ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, 0, requests_of(p)},
                       f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
@@ -723,7 +729,7 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     const Few f = few_of(p, p.out_features, p.in_features);
     int* rows = (int*)(ws + l.rows);
     int* rows2 = (int*)(ws + l.rows2);                 // (of the second shrink: the same numbers)
-    T* pieces = sizeof(T) == 2 && !f.mt ? (T*)(ws + l.pieces) : nullptr;
+    T* pieces = kPieces<T> && !f.mt ? (T*)(ws + l.pieces) : nullptr;
     if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
     const ProjectArgs<T> back{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, 0, requests_of(p)};
     WgradProblem<T> w[2]{};
@@ -737,7 +743,8 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         }
         w[n++] = WgradProblem<T>{h, (const T*)dy, lddy, db, nullptr, (int)p.out_features};
     }
-    if (dx && n && f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && !wgrad_block_rows(p)) {
+    // (not with thousands of adapters: the one launch's threads along x have to stay below 2^32)
+    if (dx && n && f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && p.n_adapters <= 128 && !wgrad_block_rows(p)) {
         const int tiles = (std::max(w[0].F, n > 1 ? w[1].F : 0) + 63) / 64;
         const FewGrid grid{f.tiles_n, f.tiles_m, f.splits};
         ProjectArgs<T> g = back;

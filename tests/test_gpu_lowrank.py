@@ -356,3 +356,27 @@ def test_refusals(handle):
         with pytest.raises(ValueError):
             call()
             raise AssertionError('call %d was accepted' % k)
+
+
+@pytest.mark.parametrize('rows,n_in,n_out', [(40, 96, 200), (700, 96, 200), (1500, 96, 2056), (3100, 96, 4104)])
+def test_f16_inner_values_outside_its_range(handle, rows, n_in, n_out):
+    """x A^T beyond f16's largest number (and, backward, among its smallest steps) where y and dx are ordinary."""
+    d = data('f16', rows, n_in, n_out, 20, 3, rows)
+    d['x'] *= 512
+    d['a'] *= 256
+    d['b'] *= 2.0 ** -13
+    d['dy'] *= 2.0 ** -6
+    off, ids = [0, 15, rows // 2, rows], [2, 1, 0]
+    h = f64(d['x'][rows // 2:]) @ f64(d['a'][0]).T
+    assert np.abs(h).max() > 2 * 65504
+    check_all(handle, d, off, ids, 'f16')
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+@pytest.mark.parametrize('rank', [8, 40])
+def test_gradients_of_many_short_requests(handle, t, rank):
+    """Requests of no row to a few rows: the gradients' waves take them in turn."""
+    rng = np.random.default_rng(rank)
+    off = np.concatenate([[0], np.cumsum(rng.integers(0, 5, 300))]).tolist()
+    ids = rng.integers(-1, 3, 300).tolist()
+    check_all(handle, data(t, off[-1], 72, 200, rank, 3, 5), off, ids, t)

@@ -38,3 +38,15 @@ def test_group_rows():
     assert order.tolist() == [2, 1, 4, 5, 0, 3] and offsets.tolist() == [0, 1, 4, 6] and ids.tolist() == [-1, 0, 2]
     order, offsets, ids = group_rows(np.zeros((0,), np.int64))
     assert order.size == 0 and offsets.tolist() == [0] and ids.size == 0
+
+
+def test_rows_beyond_a_launch_are_refused():
+    """2^26 rows are the most of one call: the limit is checked before anything else happens."""
+    from cnn_cort.adapters import _Call
+    lib, n = _hip.load_library(), ctypes.c_size_t(0)
+    some = ctypes.c_void_p(16)
+    call = _Call(4, 8, 2, 1, (1 << 26) + 1, 64, 64, 64, some, None, some, some, None, some, some)
+    assert lib.scs_lowrank_workspace(some, ctypes.byref(call), 0, None, 64, ctypes.byref(n)) == -1
+    assert b'rows lies in' in lib.scs_last_error()
+    call.rows = 1 << 26
+    assert lib.scs_lowrank_workspace(some, ctypes.byref(call), 1, None, 64, ctypes.byref(n)) == 0 and n.value > 0
