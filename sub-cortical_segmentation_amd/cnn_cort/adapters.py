@@ -31,9 +31,10 @@ class Projection:
       a       [adapters, rank, in], contiguous         b     [adapters, rank, out], contiguous       rank 1..128
       scale   float32 [adapters] or None (1)
     w, bias, a and b share one type: float32, bfloat16 or float16.  The tensors are used where they lie: updating a and b in place
-    (an optimiser's step) is seen by the next call.
+    (an optimiser's step) is seen by the next call, and one that has moved since is refused.
 
-    Calls run on the current torch stream of the device and may be captured into a graph."""
+    Calls run on the current torch stream of the device and may be captured into a graph.  They record nothing for autograd: gradients are
+    backward()'s.  An output may not lie inside the span of memory that an input's rows cover, not even between the rows."""
 
     def __init__(self, handle, w, a, b, bias=None, scale=None):
         import torch
@@ -68,6 +69,10 @@ class Projection:
             if tuple(scale.shape) != (self.n_adapters,) or not scale.is_contiguous():
                 raise ValueError('scale must be a contiguous [%d]' % self.n_adapters)
         self._lib = _hip.load_library()
+        self._where = [t.data_ptr() for t in (w, a, b)]
+        self._at = (w.data_ptr, a.data_ptr, b.data_ptr)
+        self._tensor, self._int32, self._bytes, self._index = torch.Tensor, torch.int32, torch.uint8, handle.device
+        self._empty, self._stream = torch.empty, torch._C._cuda_getCurrentRawStream             # (of a device's current stream, without an object for it)
         self._item = w.element_size()
         self._plan = (self._types[self.dtype], self.rank, self.n_adapters, 0, 0, self.n_in, self.n_out, ldw, w.data_ptr(), _hip._ptr(bias), a.data_ptr(),
                       b.data_ptr(), _hip._ptr(scale), None, None)
@@ -91,10 +96,14 @@ class Projection:
 
     def _rows(self, t, rows, cols, what):
         """(address, row stride, end address) of a [rows, cols] tensor of the projection's type."""
-        self._own(t, what, self.dtype)
-        if tuple(t.shape) != (rows, cols):
+        if not isinstance(t, self._tensor) or t.dtype is not self.dtype or t.get_device() != self._index:
+            self._own(t, what, self.dtype)
+        if t.shape != (rows, cols):
             raise ValueError('%s must be [%d, %d], got %r' % (what, rows, cols, tuple(t.shape)))
-        ld, at = self._stride(t, what), t.data_ptr()
+        ld, step = t.stride()
+        if rows <= 1 or step != 1 or ld < cols:
+            ld = self._stride(t, what)
+        at = t.data_ptr()
         return at, ld, at + (((rows - 1) * ld + cols) * self._item if rows else 0)
 
     def _flat(self, t, shape, what):
@@ -118,11 +127,13 @@ class Projection:
 
     def _call(self, x, rows, offsets, adapters):
         """The call's description on this thread (one per thread: two threads may call at once)."""
-        torch = self._torch
+        if [f() for f in self._at] != self._where:
+            raise RuntimeError('w, a or b has moved since the projection was made')
         if x.dim() != 2:
             raise ValueError('x must be [rows, %d], got %r' % (self.n_in, tuple(x.shape)))
         for t, what in ((offsets, 'offsets'), (adapters, 'adapters')):
-            self._own(t, what, torch.int32)
+            if not isinstance(t, self._tensor) or t.dtype is not self._int32 or t.get_device() != self._index:
+                self._own(t, what, self._int32)
             if t.dim() != 1 or not t.is_contiguous():
                 raise ValueError('%s must be 1-D and contiguous' % what)
         n = adapters.numel()
@@ -145,7 +156,7 @@ class Projection:
             if len(self._sizes) > 4096:
                 self._sizes.clear()
             n = self._sizes[key] = size.value
-        return self._torch.empty((n + 16,), dtype=self._torch.uint8, device=self.device), n
+        return self._empty(n + 16, dtype=self._bytes, device=self.device), n
 
     def forward(self, x, offsets, adapters, out=None, hidden=None):
         """y [rows, out] for x [rows, in].  Request q owns rows [offsets[q], offsets[q + 1]) (int32 on the device, ascending) and uses adapter
@@ -164,7 +175,7 @@ class Projection:
         self._apart(outs, [(px[0], px[2])] + self._reads)
         ws, n = self._workspace(call, 0, rows, adapters.numel(), px[0], px[1])
         rc = self._lib.scs_lowrank_forward(self.handle.h, call, px[0], px[1], py[0], py[1], outs[1][1][0] if hidden is not None else None,
-                                           ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
+                                           ws.data_ptr(), n, self._stream(self._index) or None)
         if rc:
             _hip._check(rc, 'scs_lowrank_forward')
         return out
@@ -205,7 +216,7 @@ class Projection:
         self._apart(outs, reads)
         ws, n = self._workspace(call, 1, rows, adapters.numel(), pdy[0], pdy[1])
         rc = self._lib.scs_lowrank_backward(self.handle.h, call, px[0], px[1], pdy[0], pdy[1], ph and ph[0], pdx[0], pdx[1], pg[0][1], pg[1][1],
-                                            ws.data_ptr(), n, torch.cuda.current_stream(self.device).cuda_stream or None)
+                                            ws.data_ptr(), n, self._stream(self._index) or None)
         if rc:
             _hip._check(rc, 'scs_lowrank_backward')
         return dx, pg[0][0], pg[1][0]

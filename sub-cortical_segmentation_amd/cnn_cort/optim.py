@@ -136,7 +136,7 @@ class AdamW:
             _, ptrs, types = self._gradients(grads)
         if list(map(self._torch.Tensor.data_ptr, self.params)) != self._where:
             raise RuntimeError('a parameter has moved since the optimiser was made')
-        stream = self._torch.cuda.current_stream(self.device).cuda_stream
+        stream = self._torch._C._cuda_getCurrentRawStream(self.handle.device)
         _hip._check(self._lib.scs_adamw_step(self._o, ptrs, types, self.lr if lr is None else float(lr), self.betas[0], self.betas[1], self.eps,
                                              float(grad_scale), self.max_norm or 0.0,
                                              None if self.grad_norm is None else self.grad_norm.data_ptr(), stream or None), 'scs_adamw_step')

@@ -380,3 +380,17 @@ def test_gradients_of_many_short_requests(handle, t, rank):
     off = np.concatenate([[0], np.cumsum(rng.integers(0, 5, 300))]).tolist()
     ids = rng.integers(-1, 3, 300).tolist()
     check_all(handle, data(t, off[-1], 72, 200, rank, 3, 5), off, ids, t)
+
+
+def test_a_moved_tensor_is_refused(handle):
+    """The projection reads its tensors where they lay: one whose memory was replaced is refused, not read behind the owner's back."""
+    d, off, ids = some('f32')
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'])
+    y = p.forward(d['x'], o, i)
+    old = d['b'].data
+    d['b'].data = d['b'].clone()
+    with pytest.raises(RuntimeError):
+        p.forward(d['x'], o, i)
+    d['b'].data = old
+    assert torch.equal(p.forward(d['x'], o, i), y)
