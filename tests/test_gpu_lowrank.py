@@ -394,3 +394,40 @@ def test_a_moved_tensor_is_refused(handle):
         p.forward(d['x'], o, i)
     d['b'].data = old
     assert torch.equal(p.forward(d['x'], o, i), y)
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('n_in,n_out,rank', [(1, 32, 1), (7, 33, 5), (8, 47, 16), (540, 270, 8), (2049, 100, 17), (4100, 64, 32), (9001, 5000, 16), (8193, 48, 8), (555, 31, 8), (300, 64, 33)])
+def test_one_row(handle, t, n_in, n_out, rank):
+    """One new token: every adapter, none, and a row that no request owns; rows at any element."""
+    d = data(t, 1, n_in, n_out, rank, 3, n_in + n_out, bias=n_out % 2 == 0)
+    for off, ids in (([0, 1], [2]), ([0, 0, 1, 1], [1, 0, 2]), ([0, 1], [-1]), ([1, 1], [0]), ([0, 0], [0])):
+        check_all(handle, d, off, ids, t)
+    wide = torch.zeros((n_in, n_out + 3), dtype=TYPES[t], device='cuda:0')
+    wide[:, 1:n_out + 1] = d['w']
+    wide[:, 0], wide[:, n_out + 1:] = float('nan'), float('inf')
+    flat = torch.full((n_in + 2,), float('nan'), dtype=TYPES[t], device='cuda:0')
+    flat[1:n_in + 1] = d['x'][0]
+    d['w'], d['x'] = wide[:, 1:n_out + 1], flat[1:n_in + 1].view(1, n_in)
+    check_all(handle, d, [0, 1], [1], t)
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16'])
+def test_one_row_in_a_graph(handle, t):
+    d = data(t, 1, 1000, 520, 12, 3, 4)
+    o, i = requests([0, 1], [2])
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    out, hidden = torch.zeros((1, 520), dtype=TYPES[t], device='cuda:0'), torch.zeros((1, 12), device='cuda:0')
+    p.forward(d['x'], o, i, out=out, hidden=hidden)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.forward(d['x'], o, i, out=out, hidden=hidden)
+    for k in range(4):
+        d['x'].normal_()
+        i.fill_(k - 1)
+        graph.replay()
+        h2 = torch.empty_like(hidden)
+        y = p.forward(d['x'], o, i, hidden=h2)
+        torch.cuda.synchronize()
+        assert torch.equal(out, y) and torch.equal(hidden, h2), 'replay %d' % k
