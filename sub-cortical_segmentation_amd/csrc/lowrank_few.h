@@ -8,6 +8,9 @@
 // The adapters' directions are dealt over the waves the same way: each adds scale_s H[row][j] P_s[j][..] for its j to its own sums, row by row
 // with the row's own adapter.  The waves join through LDS, the workgroups through f32 partial sums and a ticket: the last one adds them
 // up in their order, so the result does not depend on which one that is.
+// One row, 4096 x 4096, bf16: 10.5 us (3.2 TB/s) behind 4.7 us of shrink; 48 rows, 2048 x 8192, f16, 24 adapters of rank 32: 18.3 us.  W's own
+// time at a copy's rate is 6.5 us of either; the rest is the start, the adapters' dependent loads and the join.  Half as many workgroups along
+// the contraction: 14.3 for 14.5 us and 28 for 21.5; twice as many: 17.4 and 29.
 #pragma once
 #include "scs_ops.h"
 #include "lowrank_tiles.h"

@@ -15,7 +15,8 @@
 // A v that is not zero never takes the code 0: m / (0 + eps) would be a step of 1 / eps.
 //
 // What bounds it: HBM.  f32 parameters and moments move 28 B an element, bf16 parameters and gradients with 8-bit moments 10.1 B
-// (at those bytes the division and three roots an element are the second bound: ~70 vector instructions).  Work unit: a wave takes four
+// (at those bytes the division and three roots an element are the second bound: ~70 vector instructions).  96 M elements of 60 tensors: f32 520 us,
+// 5.2 TB/s, a copy's rate; bf16 with 8-bit moments 280 us, 3.5 TB/s, and 64 us for the norm; the 77 trained tensors of the net, 0.88 M: 7 us and 7 us.  Work unit: a wave takes four
 // blocks of 256 elements (one where there are few), a lane 4 consecutive elements of each (16-byte loads of f32, all four blocks' loads in flight before the first
 // use); a workgroup = 4 waves = one chunk of 16 (4) blocks of one tensor; blocks never cross tensors.
 #include <algorithm>
