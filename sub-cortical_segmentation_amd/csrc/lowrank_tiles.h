@@ -49,15 +49,20 @@ __device__ __forceinline__ void workgroup_barrier() {
     asm volatile("" : : : "memory");
 }
 
-// EVEN: N is a multiple of 8 (outputs, bias and P are read and written four and eight columns at a time)
+template <class T, int WN, int MT, int NT> struct TilesShared {
+    __attribute__((aligned(16))) T a[4][32 * MT * 32];
+    __attribute__((aligned(16))) T b[4][16 * WN * NT * 32];
+};
+
+// Tile `pid` (in the order of the workgroups).  EVEN: N is a multiple of 8 (outputs, bias and P are read and written four and eight columns at a time)
 template <class T, int WN, int MT, int NT, bool TRANS, bool EVEN>
-__global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<T> g) {
+__device__ __forceinline__ void project_tile(const ProjectArgs<T>& g, int pid, TilesShared<T, WN, MT, NT>& sh) {
     typedef typename Frag<T>::v8 v8;
     constexpr int THREADS = 128 * WN, BM = 32 * MT, BN = 16 * WN * NT, BK = 32, STAGES = 4, NP = BN / 8;
     constexpr int UNITS = BN / 16 < 8 ? BN / 16 - 1 : 7;               // bits of f(k) that a row has units for
     constexpr int A_IT = BM * 4 / THREADS, B_IT = BN * 4 / THREADS, LOADS = A_IT + B_IT;
-    __shared__ __attribute__((aligned(16))) T s_a[STAGES][BM * BK];
-    __shared__ __attribute__((aligned(16))) T s_b[STAGES][BN * BK];
+    auto& s_a = sh.a;
+    auto& s_b = sh.b;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lr = lane & 15, kq = lane >> 4, wm = wave / WN, wn = wave % WN;
     const Requests& r = g.r;
@@ -66,7 +71,7 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
     // serves W's columns and X's rows again
     int m0, n0;
     {
-        const int tm = (r.rows + BM - 1) / BM, tn = (g.N + BN - 1) / BN, total = tm * tn, pid = blockIdx.x;
+        const int tm = (r.rows + BM - 1) / BM, tn = (g.N + BN - 1) / BN, total = tm * tn;
         const int xcd = pid & 7, each = total >> 3, rest = total & 7;
         const int t = xcd * each + min(xcd, rest) + (pid >> 3);
         const int band = t / (8 * tn), in = t - band * 8 * tn, high = min(8, tm - band * 8);
@@ -294,6 +299,12 @@ __global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<
         }
         __builtin_amdgcn_sched_barrier(0);
     }
+}
+
+template <class T, int WN, int MT, int NT, bool TRANS, bool EVEN>
+__global__ __launch_bounds__(128 * WN, 2) void project_tiles_kernel(ProjectArgs<T> g) {
+    __shared__ TilesShared<T, WN, MT, NT> sh;
+    project_tile<T, WN, MT, NT, TRANS, EVEN>(g, blockIdx.x, sh);
 }
 
 }  // namespace

@@ -388,13 +388,12 @@ template <int JT> __device__ __forceinline__ void wgrad_clear(f32x4 (&acc)[JT][4
 }
 
 template <class T, int JT>
-__global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
-    __shared__ float s_part[3][JT * 16][64];
-    const WgradProblem<T>& w = g.p[blockIdx.z];
+__device__ __forceinline__ void wgrad_block(const WgradArgs<T>& g, int tile, int block, int problem, float (&s_part)[3][JT * 16][64]) {
+    const WgradProblem<T>& w = g.p[problem];
     const Requests& r = g.r;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.x * 64, col = c0 + 4 * (threadIdx.x & 15);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = tile * 64, col = c0 + 4 * (threadIdx.x & 15);
     if (c0 >= w.F) return;
-    const int m0 = blockIdx.y * g.block_rows, m1 = min(m0 + g.block_rows, r.rows);
+    const int m0 = block * g.block_rows, m1 = min(m0 + g.block_rows, r.rows);
     Walk walk(r, m0, m1);
     int q;
     Span sp;
@@ -403,8 +402,29 @@ __global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
         f32x4 acc[JT][4];
         wgrad_clear<JT>(acc);
         wgrad_rows<T, JT, 4>(w, r, col, sp.lo, sp.hi, wave, acc);
-        wgrad_store<JT, 4>(s_part, acc, wave, r.rank, w.F, col, 1.f, w.part + (int64_t)(q + blockIdx.y) * r.rank * w.F);
+        wgrad_store<JT, 4>(s_part, acc, wave, r.rank, w.F, col, 1.f, w.part + (int64_t)(q + block) * r.rank * w.F);
     }
+}
+template <class T, int JT>
+__global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
+    __shared__ float s_part[3][JT * 16][64];
+    wgrad_block<T, JT>(g, blockIdx.x, blockIdx.y, blockIdx.z, s_part);
+}
+
+// dx in small tiles and the adapters' gradients by blocks of rows in one launch, the tiles first
+template <class T, int JT, bool EVEN>
+__global__ __launch_bounds__(256, 2) void tiles_and_wgrad_kernel(ProjectArgs<T> g, int n_tiles, WgradArgs<T> w, int tiles, int blocks) {
+    __shared__ union Shared {
+        __device__ Shared() {}
+        TilesShared<T, 2, 2, 2> tile;
+        float part[3][JT * 16][64];
+    } sh;
+    if ((int)blockIdx.x < n_tiles) {
+        project_tile<T, 2, 2, 2, true, EVEN>(g, blockIdx.x, sh.tile);
+        return;
+    }
+    const int id = blockIdx.x - n_tiles, rest = id / tiles;
+    wgrad_block<T, JT>(w, id % tiles, rest % blocks, rest / blocks, sh.part);
 }
 
 template <class T, int JT, int W>
@@ -643,12 +663,17 @@ template <class T, bool TRANS> void launch_few(const ProjectArgs<T>& g, const Fe
     }
 }
 
+// the largest 16-bit tile that still gives most of the 256 CUs one
+int tile16(int64_t rows, int64_t N) {
+    auto tiles = [&](int64_t b) { return (rows + b - 1) / b * ((N + b - 1) / b); };
+    return tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+}
+
 template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T>& g, hipStream_t st) {
     auto tiles = [&](int64_t bm, int64_t bn) { return (g.r.rows + bm - 1) / bm * ((g.N + bn - 1) / bn); };
     if constexpr (sizeof(T) == 2) {
-        // the largest tile that still gives most of the 256 CUs one
-        if (tiles(256, 256) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 4, 8, 4, TRANS, EVEN>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, st, g);
-        else if (tiles(128, 128) >= 192) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS, EVEN>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, g);
+        if (tile16(g.r.rows, g.N) == 256) hipLaunchKernelGGL((project_tiles_kernel<T, 4, 8, 4, TRANS, EVEN>), dim3((unsigned)tiles(256, 256)), dim3(512), 0, st, g);
+        else if (tile16(g.r.rows, g.N) == 128) hipLaunchKernelGGL((project_tiles_kernel<T, 2, 4, 4, TRANS, EVEN>), dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, g);
         else hipLaunchKernelGGL((project_tiles_kernel<T, 2, 2, 2, TRANS, EVEN>), dim3((unsigned)tiles(64, 64)), dim3(256), 0, st, g);
     } else {
         const int nt = f32_columns(g.N), mt = f32_rows(g.r.rows, g.N);
@@ -664,10 +689,9 @@ template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T
     }
 }
 
-template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T> g, const Few& f, const int* rows, float* part, unsigned int* tickets, T* pack_x, T* pack_w,
-                                            hipStream_t st) {
+// the tile kernels' operands, laid out anew where they have to be
+template <class T, bool TRANS> void pack(const scs_lowrank& p, ProjectArgs<T>& g, T* pack_x, T* pack_w, hipStream_t st) {
     g.nw = g.N;
-    if (f.mt) { launch_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
     const Pack k = pack_of(p, g.K, g.N, TRANS, g.x, g.ldx);
     PackArgs pa{};
     int n = 0;
@@ -687,11 +711,19 @@ template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T>
         hipLaunchKernelGGL(pack_kernel<T>, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8192), n), dim3(256), 0, st, pa);
     }
     g.K = (int)k.K;
+}
+
+template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T> g, const Few& f, const int* rows, float* part, unsigned int* tickets, T* pack_x, T* pack_w,
+                                            hipStream_t st) {
+    g.nw = g.N;
+    if (f.mt) { launch_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
+    pack<T, TRANS>(p, g, pack_x, pack_w, st);
     if (g.N % (sizeof(T) == 2 ? 8 : 4) == 0) project_tiles<T, TRANS, true>(g, st);
     else project_tiles<T, TRANS, false>(g, st);
 }
 
-template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&problems)[2], int n, float* slots, hipStream_t st) {
+// beside(arguments, tiles, blocks): whether the partial sums of the by-blocks form are formed in a launch of the caller's
+template <class T, class Beside> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&problems)[2], int n, float* slots, hipStream_t st, Beside&& beside) {
     WgradArgs<T> g{{problems[0], problems[1]}, wgrad_block_rows(p), requests_of(p)};
     const int F = std::max(problems[0].F, n > 1 ? problems[1].F : 0), tiles = (F + 63) / 64;
     if (!g.block_rows) {
@@ -703,7 +735,8 @@ template <class T> void wgrad(const scs_lowrank& p, const WgradProblem<T> (&prob
     const int64_t blocks = (p.rows + g.block_rows - 1) / g.block_rows;
     g.p[0].part = slots;
     g.p[1].part = slots + (p.n_requests + blocks) * p.rank * problems[0].F;
-    by_tiles(p.rank, [&](auto jt) { hipLaunchKernelGGL((wgrad_blocks_kernel<T, jt.value>), dim3(tiles, (unsigned)blocks, n), dim3(256), 0, st, g); });
+    if (!beside(g, tiles, (int)blocks))
+        by_tiles(p.rank, [&](auto jt) { hipLaunchKernelGGL((wgrad_blocks_kernel<T, jt.value>), dim3(tiles, (unsigned)blocks, n), dim3(256), 0, st, g); });
     hipLaunchKernelGGL(wgrad_join_kernel<T>, dim3((unsigned)(((int64_t)p.rank * F + 1023) / 1024), p.n_adapters, n), dim3(256), 0, st, g);
 }
 
@@ -760,9 +793,28 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         typedef std::integral_constant<int, 2> Two;
         if (f.mt == 1) { if (p.rank <= 16) go(One{}, One{}); else go(One{}, Two{}); }
         else { if (p.rank <= 16) go(Two{}, One{}); else go(Two{}, Two{}); }
+    } else if (sizeof(T) == 2 && dx && n && !f.mt && p.rank <= 32 && tile16(p.rows, p.in_features) == 64 && wgrad_block_rows(p)) {
+        // neither dx in small tiles nor the partial sums fill the card: one launch
+        if constexpr (sizeof(T) == 2) {
+            ProjectArgs<T> g = back;
+            pack<T, true>(p, g, (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
+            const int n_tiles = (int)((p.rows + 63) / 64 * ((p.in_features + 63) / 64));
+            wgrad<T>(p, w, n, (float*)(ws + l.slots), st, [&](const WgradArgs<T>& wa, int tiles, int blocks) {
+                auto go = [&](auto jt, auto even) {
+                    hipLaunchKernelGGL((tiles_and_wgrad_kernel<T, jt.value, even.value>), dim3(n_tiles + tiles * blocks * n), dim3(256), 0, st, g, n_tiles, wa, tiles, blocks);
+                };
+                auto by_even = [&](auto jt) {
+                    if (g.N % 8 == 0) go(jt, std::true_type{});
+                    else go(jt, std::false_type{});
+                };
+                if (p.rank <= 16) by_even(std::integral_constant<int, 1>{});
+                else by_even(std::integral_constant<int, 2>{});
+                return true;
+            });
+        }
     } else {
         if (dx) project<T, true>(p, back, f, rows, part, (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
-        if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st);
+        if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st, [](const WgradArgs<T>&, int, int) { return false; });
     }
     SCS_HIP(hipGetLastError());
     return SCS_OK;
