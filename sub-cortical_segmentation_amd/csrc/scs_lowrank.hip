@@ -109,11 +109,37 @@ template <class T> __device__ __forceinline__ void write_pieces(T* pieces, int64
     }
 }
 
+// The tile kernels copy 16-byte pieces: rows that start at any element, or sizes that end inside a piece, are first laid out anew with zeros
+// behind their ends (up to two matrices; their bytes once read and once written), by workgroups of their own in the shrink's launch
+// (1000 x 777 and 1111 x 777, f16: 3 us less than as a launch).
+struct PackMatrix { const void* src; void* dst; int64_t ld; int32_t rows, cols, rows_out, cols_out; };
+struct PackArgs { PackMatrix m[2]; int32_t groups; };             // groups: workgroups that do it (0: nothing to do)
+template <class T> __device__ __forceinline__ void pack_pieces(const PackArgs& g, int group) {
+    constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const PackMatrix& m = g.m[k];
+        const int pieces = m.cols_out / PER;
+        const int64_t n = (int64_t)m.rows_out * pieces;
+        for (int64_t i = (int64_t)group * blockDim.x + threadIdx.x; i < n; i += (int64_t)g.groups * blockDim.x) {
+            const int64_t row = i / pieces;
+            const int col = (int)(i - row * pieces) * PER;
+            ((u32x4*)m.dst)[i] = load16((const T*)m.src + row * m.ld + col, row < m.rows ? m.cols - col : 0);
+        }
+    }
+}
+template <class T> __global__ __launch_bounds__(256) void pack_kernel(PackArgs g) { pack_pieces<T>(g, blockIdx.x); }
+
 template <class T, int JT, int MT, int W>
 __global__ __launch_bounds__(64 * W) void shrink_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ p, int K, float* __restrict__ h, T* __restrict__ pieces, Requests r,
-                                                             int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets) {
+                                                             int* __restrict__ row_adapter, unsigned int* __restrict__ tickets, int n_tickets, PackArgs pk) {
     constexpr int STEP = 64 / sizeof(T), PER = 16 / sizeof(T), UNROLL = JT <= 2 ? 4 : 2, UNIT = UNROLL * STEP;      // contraction values
     __shared__ float s_part[W][MT * JT * 4][64];
+    const int groups = gridDim.x - pk.groups;
+    if ((int)blockIdx.x >= groups) {
+        pack_pieces<T>(pk, blockIdx.x - groups);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lr = lane & 15, kq = lane >> 4;
     const int m0 = blockIdx.x * 16 * MT, m1 = min(m0 + 16 * MT, r.rows);
@@ -133,7 +159,7 @@ __global__ __launch_bounds__(64 * W) void shrink_rows_kernel(const T* __restrict
 #pragma unroll
             for (int i = 0; i < MT; ++i) first[u][i] = at16(xr[i] + k_first + u * STEP);
     }
-    for (int i = blockIdx.x * 64 * W + threadIdx.x; i < n_tickets; i += gridDim.x * 64 * W) tickets[i] = 0;
+    for (int i = blockIdx.x * 64 * W + threadIdx.x; i < n_tickets; i += groups * 64 * W) tickets[i] = 0;
     int mine = -2, q;
     Span sp;
     while (walk.next(q, sp)) {
@@ -282,23 +308,6 @@ struct ProjectArgs {
     Requests r;
 };
 
-// The tile kernels copy 16-byte pieces: rows that start at any element, or sizes that end inside a piece, are first laid out anew with zeros
-// behind their ends (up to two matrices in one launch; their bytes once read and once written).
-struct PackMatrix { const void* src; void* dst; int64_t ld; int32_t rows, cols, rows_out, cols_out; };
-struct PackArgs { PackMatrix m[2]; };
-template <class T>
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs g) {
-    constexpr int PER = 16 / sizeof(T);
-    const PackMatrix& m = g.m[blockIdx.y];
-    const int pieces = m.cols_out / PER;
-    const int64_t n = (int64_t)m.rows_out * pieces;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / pieces;
-        const int col = (int)(i - row * pieces) * PER;
-        ((u32x4*)m.dst)[i] = load16((const T*)m.src + row * m.ld + col, row < m.rows ? m.cols - col : 0);
-    }
-}
-
 }  // namespace
 }  // namespace scs
 #include "lowrank_tiles.h"
@@ -411,7 +420,8 @@ __global__ __launch_bounds__(256) void wgrad_blocks_kernel(WgradArgs<T> g) {
     wgrad_block<T, JT>(g, blockIdx.x, blockIdx.y, blockIdx.z, s_part);
 }
 
-// dx in small tiles and the adapters' gradients by blocks of rows in one launch, the tiles first
+// dx in small tiles and the adapters' gradients by blocks of rows in one launch, the tiles first: neither fills the card (1000 rows, 777 x 1111, f16:
+// 19 us together, 18 and 14 one after the other)
 template <class T, int JT, bool EVEN>
 __global__ __launch_bounds__(256, 2) void tiles_and_wgrad_kernel(ProjectArgs<T> g, int n_tiles, WgradArgs<T> w, int tiles, int blocks) {
     __shared__ union Shared {
@@ -625,9 +635,11 @@ template <class F> void by_tiles(int rank, F&& f) {
     else f(std::integral_constant<int, 8>{});
 }
 
-template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, T* pieces, hipStream_t st, int* row_adapter, unsigned int* tickets = nullptr, int n_tickets = 0) {
+template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, const T* low, int K, float* h, T* pieces, hipStream_t st, int* row_adapter, unsigned int* tickets = nullptr, int n_tickets = 0,
+                               const PackArgs& pk = PackArgs{}) {
     const Requests r = requests_of(p);
     if (p.rows <= kDotRows) {
+        if (pk.groups) hipLaunchKernelGGL(pack_kernel<T>, dim3(pk.groups), dim3(256), 0, st, pk);
         hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets);
         return;
     }
@@ -636,8 +648,8 @@ template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, co
         constexpr int UNIT = (jt.value <= 2 ? 4 : 2) * 64 / (int)sizeof(T);
         const int units = (K + UNIT - 1) / UNIT;
         auto go = [&](auto mt, auto w) {
-            hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, mt.value, w.value>), dim3((unsigned)((p.rows + 16 * mt.value - 1) / (16 * mt.value))), dim3(64 * w.value), 0, st,
-                               x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets);
+            hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, mt.value, w.value>), dim3((unsigned)((p.rows + 16 * mt.value - 1) / (16 * mt.value) + pk.groups)), dim3(64 * w.value), 0, st,
+                               x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets, pk);
         };
         constexpr int MT = jt.value <= 2 ? 2 : 1, MOST = jt.value <= 2 ? 16 : 8;             // (registers)
         typedef std::integral_constant<int, 1> One;
@@ -689,8 +701,8 @@ template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T
     }
 }
 
-// the tile kernels' operands, laid out anew where they have to be
-template <class T, bool TRANS> void pack(const scs_lowrank& p, ProjectArgs<T>& g, T* pack_x, T* pack_w, hipStream_t st) {
+// what has to be laid out anew of the tile kernels' operands (for the shrink's launch), the projection's arguments turned to where it will lie
+template <class T, bool TRANS> PackArgs pack(const scs_lowrank& p, ProjectArgs<T>& g, T* pack_x, T* pack_w) {
     g.nw = g.N;
     const Pack k = pack_of(p, g.K, g.N, TRANS, g.x, g.ldx);
     PackArgs pa{};
@@ -706,19 +718,14 @@ template <class T, bool TRANS> void pack(const scs_lowrank& p, ProjectArgs<T>& g
         g.ldw = k.w_cols;
         g.nw = (int)k.nw;
     }
-    if (n) {
-        const int64_t most = std::max(k.x_bytes, k.w_bytes) / 16;
-        hipLaunchKernelGGL(pack_kernel<T>, dim3((unsigned)std::min<int64_t>((most + 255) / 256, 8192), n), dim3(256), 0, st, pa);
-    }
+    if (n) pa.groups = (int)std::min<int64_t>((int64_t)(std::max(k.x_bytes, k.w_bytes) / 16 + 255) / 256, 8192);
     g.K = (int)k.K;
+    return pa;
 }
 
-template <class T, bool TRANS> void project(const scs_lowrank& p, ProjectArgs<T> g, const Few& f, const int* rows, float* part, unsigned int* tickets, T* pack_x, T* pack_w,
-                                            hipStream_t st) {
-    g.nw = g.N;
-    if (f.mt) { launch_few<T, TRANS>(g, f, rows, part, tickets, st); return; }
-    pack<T, TRANS>(p, g, pack_x, pack_w, st);
-    if (g.N % (sizeof(T) == 2 ? 8 : 4) == 0) project_tiles<T, TRANS, true>(g, st);
+template <class T, bool TRANS> void project(const ProjectArgs<T>& g, const Few& f, const int* rows, float* part, unsigned int* tickets, hipStream_t st) {
+    if (f.mt) launch_few<T, TRANS>(g, f, rows, part, tickets, st);
+    else if (g.N % (sizeof(T) == 2 ? 8 : 4) == 0) project_tiles<T, TRANS, true>(g, st);
     else project_tiles<T, TRANS, false>(g, st);
 }
 
@@ -747,9 +754,10 @@ int forward(const scs_lowrank& p, const void* x, int64_t ldx, void* y, int64_t l
     const Few f = few_of(p, p.in_features, p.out_features);
     int* rows = (int*)(ws + l.rows);
     T* pieces = kPieces<T> && !f.mt ? (T*)(ws + l.pieces) : nullptr;
-    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
-    project<T, false>(p, ProjectArgs<T>{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, 0, requests_of(p)},
-                      f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
+    ProjectArgs<T> g{(const T*)x, ldx, (const T*)p.w, p.ldw, (const T*)p.bias, (const T*)p.b, h, pieces, (T*)y, ldy, (int)p.in_features, (int)p.out_features, (int)p.out_features, requests_of(p)};
+    const PackArgs pk = f.mt ? PackArgs{} : pack<T, false>(p, g, (T*)(ws + l.pack_x), (T*)(ws + l.pack_w));
+    shrink<T>(p, (const T*)x, ldx, (const T*)p.a, (int)p.in_features, h, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets, pk);
+    project<T, false>(g, f, rows, (float*)(ws + l.part), (unsigned int*)(ws + l.tickets), st);
     SCS_HIP(hipGetLastError());
     return SCS_OK;
 }
@@ -765,8 +773,9 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     int* rows = (int*)(ws + l.rows);
     int* rows2 = (int*)(ws + l.rows2);                 // (of the second shrink: the same numbers)
     T* pieces = kPieces<T> && !f.mt ? (T*)(ws + l.pieces) : nullptr;
-    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets);
-    const ProjectArgs<T> back{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, 0, requests_of(p)};
+    ProjectArgs<T> back{(const T*)dy, lddy, (const T*)p.w, p.ldw, nullptr, (const T*)p.a, u, pieces, (T*)dx, lddx, (int)p.out_features, (int)p.in_features, (int)p.in_features, requests_of(p)};
+    const PackArgs pk = f.mt || !dx ? PackArgs{} : pack<T, true>(p, back, (T*)(ws + l.pack_x), (T*)(ws + l.pack_w));
+    if (any && (dx || da)) shrink<T>(p, (const T*)dy, lddy, (const T*)p.b, (int)p.out_features, u, pieces, st, rows, (unsigned int*)(ws + l.tickets), f.tickets, pk);
     WgradProblem<T> w[2]{};
     int n = 0;
     if (da) w[n++] = WgradProblem<T>{u, (const T*)x, ldx, da, nullptr, (int)p.in_features};
@@ -782,12 +791,10 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     if (dx && n && f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && p.n_adapters <= 128 && !wgrad_block_rows(p)) {
         const int tiles = (std::max(w[0].F, n > 1 ? w[1].F : 0) + 63) / 64;
         const FewGrid grid{f.tiles_n, f.tiles_m, f.splits};
-        ProjectArgs<T> g = back;
-        g.nw = g.N;
         const WgradArgs<T> wa{{w[0], w[1]}, 0, requests_of(p)};
         const dim3 all((unsigned)(f.tiles_n * f.tiles_m * f.splits + tiles * p.n_adapters * n));
         auto go = [&](auto mt, auto jt) {
-            hipLaunchKernelGGL((few_and_wgrad_kernel<T, mt.value, jt.value>), all, dim3(64 * kFewWaves), 0, st, g, rows, grid, part, (unsigned int*)(ws + l.tickets), wa, tiles);
+            hipLaunchKernelGGL((few_and_wgrad_kernel<T, mt.value, jt.value>), all, dim3(64 * kFewWaves), 0, st, back, rows, grid, part, (unsigned int*)(ws + l.tickets), wa, tiles);
         };
         typedef std::integral_constant<int, 1> One;
         typedef std::integral_constant<int, 2> Two;
@@ -796,15 +803,13 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
     } else if (sizeof(T) == 2 && dx && n && !f.mt && p.rank <= 32 && tile16(p.rows, p.in_features) == 64 && wgrad_block_rows(p)) {
         // neither dx in small tiles nor the partial sums fill the card: one launch
         if constexpr (sizeof(T) == 2) {
-            ProjectArgs<T> g = back;
-            pack<T, true>(p, g, (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
             const int n_tiles = (int)((p.rows + 63) / 64 * ((p.in_features + 63) / 64));
             wgrad<T>(p, w, n, (float*)(ws + l.slots), st, [&](const WgradArgs<T>& wa, int tiles, int blocks) {
                 auto go = [&](auto jt, auto even) {
-                    hipLaunchKernelGGL((tiles_and_wgrad_kernel<T, jt.value, even.value>), dim3(n_tiles + tiles * blocks * n), dim3(256), 0, st, g, n_tiles, wa, tiles, blocks);
+                    hipLaunchKernelGGL((tiles_and_wgrad_kernel<T, jt.value, even.value>), dim3(n_tiles + tiles * blocks * n), dim3(256), 0, st, back, n_tiles, wa, tiles, blocks);
                 };
                 auto by_even = [&](auto jt) {
-                    if (g.N % 8 == 0) go(jt, std::true_type{});
+                    if (back.N % 8 == 0) go(jt, std::true_type{});
                     else go(jt, std::false_type{});
                 };
                 if (p.rank <= 16) by_even(std::integral_constant<int, 1>{});
@@ -813,7 +818,7 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
             });
         }
     } else {
-        if (dx) project<T, true>(p, back, f, rows, part, (unsigned int*)(ws + l.tickets), (T*)(ws + l.pack_x), (T*)(ws + l.pack_w), st);
+        if (dx) project<T, true>(back, f, rows, part, (unsigned int*)(ws + l.tickets), st);
         if (n) wgrad<T>(p, w, n, (float*)(ws + l.slots), st, [](const WgradArgs<T>&, int, int) { return false; });
     }
     SCS_HIP(hipGetLastError());
