@@ -405,8 +405,9 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
 int scs_adamw_destroy(scs_adamw o);
 
 /* One step.  grads, grad_types: host arrays of one device pointer (n elements, contiguous) and one type per tensor; they are read before
- * the call returns.  Gradients are not changed.  max_norm > 0 clips by the norm over all tensors and leaves it (before clipping) in
- * *norm_dev (device float, may be NULL); where that norm is not finite NOTHING changes - neither parameters, moments nor the step count.
+ * the call returns.  Gradients are not changed; they must not share memory with parameters, masters or arenas.  max_norm > 0 clips by the
+ * norm over all tensors and leaves it (before clipping) in *norm_dev (device float, may be NULL); where that norm is not finite NOTHING
+ * changes - neither parameters, moments nor the step count.
  * Without max_norm a gradient that is not finite makes its element's m, v and p NaN (8 bits: its block's m and v).
  * The step count lives on the device, so that a captured call counts at every replay; lr and the other numbers are the captured call's.
  * Steps of one optimiser must be ordered (one stream, or events): they update the same memory.  The result is the same bits every time. */

@@ -5,6 +5,7 @@ AdamW over many tensors at once, on libscs (scs_adamw_*, include/scs.h): one lau
 The reference trains with lasagne.updates.adam (nets.py:236-237); that update stays the default of Net.fit, this one is what
 Net.fit(optimizer='adamw') and Net.fit_adapters use.
 """
+import bisect
 import ctypes
 import math
 
@@ -93,6 +94,9 @@ class AdamW:
                                          _hip._ptr(self.m_scale), _hip._ptr(self.v_scale), int(step), ctypes.byref(o)), 'scs_adamw_create')
         self._lib, self._o = lib, o
         self._where = [p.data_ptr() for p in self.params]
+        held = self.params + [t for t in self.masters + [self.m, self.v, self.m_scale, self.v_scale] if t is not None]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in held if t.numel())
+        self._starts, self._ends = [a for a, _ in spans], [b for _, b in spans]             # (they share no memory: both ascend)
         self.grads = self._bound = None
         self.grad_norm = torch.zeros((1,), device=dev) if self.max_norm is not None else None      # of the last step, before clipping
 
@@ -115,7 +119,11 @@ class AdamW:
             self._check(g, i, 'gradient', self.device)
             if g.numel() != p.numel():
                 raise ValueError('gradient %d has %d elements, its parameter %d' % (i, g.numel(), p.numel()))
-            ptrs[i], types[i] = g.data_ptr(), self._types[g.dtype]
+            at = ptrs[i] = g.data_ptr()
+            types[i] = self._types[g.dtype]
+            k = bisect.bisect_right(self._ends, at)
+            if g.numel() and k < len(self._starts) and self._starts[k] < at + g.numel() * g.element_size():
+                raise ValueError('gradient %d shares memory with a parameter or a moment' % i)
         return grads, ptrs, types
 
     def bind(self, grads):

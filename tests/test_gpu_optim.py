@@ -338,3 +338,21 @@ def test_refusals(handle):
     opt.close()
     with pytest.raises(RuntimeError, match='closed'):
         opt.step([g])
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_gradients_in_the_optimisers_memory_are_refused(handle, bits):
+    """A gradient that shares memory with a parameter, a master or a moment would be read while it is written."""
+    flat = torch.zeros((4096,), dtype=torch.bfloat16, device='cuda:0')
+    params = [flat[:1000], flat[2000:2600]]
+    opt = AdamW(handle, params, state_bits=bits, master=True)
+    free = [torch.zeros((1000,), device='cuda:0'), torch.zeros((600,), device='cuda:0')]
+    opt.step([flat[1000:2000], flat[2600:3200]])                       # (beside them is fine)
+    taken = [params[0], flat[1999:2999], opt.masters[0]]
+    if bits == 32:
+        taken.append(opt.m[24:1024])
+    for t in taken:
+        with pytest.raises(ValueError, match='shares memory'):
+            opt.step([t, free[1]])
+    opt.step(free)
+    assert opt.step_count == 2
