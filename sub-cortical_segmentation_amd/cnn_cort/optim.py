@@ -160,7 +160,7 @@ class AdamW:
         for t in out:
             if not torch.is_tensor(t) or t.dtype != torch.float32 or t.device != self.device or t.numel() != self.blocks * BLOCK or not t.is_contiguous():
                 raise ValueError('out must be two contiguous float32 tensors of %d elements on %s' % (self.blocks * BLOCK, self.device))
-        _hip._check(self._lib.scs_adamw_states(self._o, out[0].data_ptr(), out[1].data_ptr(), torch.cuda.current_stream(self.device).cuda_stream or None),
+        _hip._check(self._lib.scs_adamw_states(self._o, out[0].data_ptr(), out[1].data_ptr(), torch._C._cuda_getCurrentRawStream(self.handle.device) or None),
                     'scs_adamw_states')
         return tuple(out)
 
