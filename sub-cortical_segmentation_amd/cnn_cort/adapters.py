@@ -31,7 +31,8 @@ class Projection:
       a       [adapters, rank, in], contiguous         b     [adapters, rank, out], contiguous       rank 1..128
       scale   float32 [adapters] or None (1)
     w, bias, a and b share one type: float32, bfloat16 or float16.  The tensors are used where they lie: updating a and b in place
-    (an optimiser's step) is seen by the next call, and one that has moved since is refused.
+    (an optimiser's step) is seen by the next call.  The five stay the ones that were given, and a call is refused when the memory of any of them has
+    been replaced since (its old memory stays allocated as long as the projection does).
 
     Calls run on the current torch stream of the device and may be captured into a graph.  They record nothing for autograd: gradients are
     backward()'s.  An output may not lie inside the span of memory that an input's rows cover, not even between the rows."""
@@ -41,7 +42,7 @@ class Projection:
         self._torch = torch
         self._types = {torch.float32: 4, torch.bfloat16: 6, torch.float16: 7}          # SCS_F32, SCS_BF16, SCS_F16
         self.handle, self.device = handle, torch.device('cuda', handle.device)
-        self.w, self.a, self.b, self.bias, self.scale = w, a, b, bias, scale
+        self._given = {'w': w, 'a': a, 'b': b, 'bias': bias, 'scale': scale}
         if not torch.is_tensor(w) or w.dtype not in self._types or w.dim() != 2:
             raise ValueError('w must be a 2-D float32, bfloat16 or float16 tensor')
         self.dtype = w.dtype
@@ -69,8 +70,10 @@ class Projection:
             if tuple(scale.shape) != (self.n_adapters,) or not scale.is_contiguous():
                 raise ValueError('scale must be a contiguous [%d]' % self.n_adapters)
         self._lib = _hip.load_library()
-        self._where = [t.data_ptr() for t in (w, a, b)]
-        self._at = (w.data_ptr, a.data_ptr, b.data_ptr)
+        given = [t for t in self._given.values() if t is not None]
+        self._held = [t.detach() for t in given]                                        # (of the same memory, whatever becomes of the caller's)
+        self._where = [t.data_ptr() for t in given]
+        self._at = [t.data_ptr for t in given]
         self._tensor, self._int32, self._bytes, self._index = torch.Tensor, torch.int32, torch.uint8, handle.device
         self._empty, self._stream = torch.empty, torch._C._cuda_getCurrentRawStream             # (of a device's current stream, without an object for it)
         self._item = w.element_size()
@@ -79,6 +82,8 @@ class Projection:
         self._reads = [(t.data_ptr(), t.data_ptr() + ((t.shape[0] - 1) * ldw + self.n_out if t is w else t.numel()) * t.element_size())
                        for t in (w, a, b, bias, scale) if t is not None]
         self._sizes, self._tls = {}, threading.local()
+
+    w, a, b, bias, scale = (property(lambda self, k=k: self._given[k]) for k in ('w', 'a', 'b', 'bias', 'scale'))
 
     def _own(self, t, what, dtype):
         if not self._torch.is_tensor(t) or t.dtype != dtype:
@@ -128,7 +133,7 @@ class Projection:
     def _call(self, x, rows, offsets, adapters):
         """The call's description on this thread (one per thread: two threads may call at once)."""
         if [f() for f in self._at] != self._where:
-            raise RuntimeError('w, a or b has moved since the projection was made')
+            raise RuntimeError('w, a, b, bias or scale has moved since the projection was made')
         if x.dim() != 2:
             raise ValueError('x must be [rows, %d], got %r' % (self.n_in, tuple(x.shape)))
         for t, what in ((offsets, 'offsets'), (adapters, 'adapters')):

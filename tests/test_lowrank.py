@@ -50,3 +50,37 @@ def test_rows_beyond_a_launch_are_refused():
     assert b'rows lies in' in lib.scs_last_error()
     call.rows = 1 << 26
     assert lib.scs_lowrank_workspace(some, ctypes.byref(call), 1, None, 64, ctypes.byref(n)) == 0 and n.value > 0
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """Projections over host tensors: what is decided before a launch."""
+    monkeypatch.setattr(Projection, '_own', lambda self, t, what, dtype: None)
+
+
+@pytest.mark.parametrize('which', ['w', 'a', 'b', 'bias', 'scale'])
+def test_a_tensor_that_has_moved_is_refused(on_host, which):
+    """Every tensor whose address the projection holds: its memory replaced, or the attribute itself."""
+    d = {'w': torch.zeros(4, 6), 'a': torch.zeros(2, 3, 4), 'b': torch.zeros(2, 3, 6), 'bias': torch.zeros(6), 'scale': torch.ones(2)}
+    p = Projection(NoDevice, **d)
+    x, off, ids = torch.zeros(5, 4), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    p._call(x, 5, off, ids)
+    old = d[which].data
+    d[which].data = d[which].clone()
+    with pytest.raises(RuntimeError, match='has moved'):
+        p._call(x, 5, off, ids)
+    d[which].data = old
+    p._call(x, 5, off, ids)
+    with pytest.raises(AttributeError):
+        setattr(p, which, d[which].clone())
+    assert getattr(p, which) is d[which]
+
+
+def test_the_memory_of_a_moved_tensor_is_kept(on_host):
+    """A captured call goes on reading where its tensors lay: that memory stays the projection's."""
+    d = {'w': torch.zeros(4, 6), 'a': torch.zeros(2, 3, 4), 'b': torch.zeros(2, 3, 6), 'bias': torch.zeros(6), 'scale': torch.ones(2)}
+    p = Projection(NoDevice, **d)
+    at = [t.data_ptr() for t in d.values()]
+    for t in d.values():
+        t.data = t.clone()
+    assert sorted(t.data_ptr() for t in p._held) == sorted(at)
