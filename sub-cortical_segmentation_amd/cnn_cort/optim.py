@@ -37,7 +37,8 @@ class AdamW:
       states        None (zeros), or (m, v, m_scale, v_scale) of another AdamW over tensors of the same sizes; `step`: steps they have seen
 
     self.m, self.v, self.m_scale, self.v_scale are the arenas: tensor i owns blocks [self.first[i], self.first[i] + blocks_of(n_i)) of 256
-    elements.  step() runs on the current torch stream of the device; it may be captured into a graph, whose replays count as steps."""
+    elements.  The optimiser's tensors stay the ones it was made with (none of these attributes can be set): step() is refused when the memory of one of
+    them has been replaced since, and their old memory stays allocated as long as the optimiser does.  step() runs on the current torch stream of the device; it may be captured into a graph, whose replays count as steps."""
 
     def __init__(self, handle, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, state_bits=32, max_norm=None, master=False,
                  states=None, step=0):
@@ -45,8 +46,8 @@ class AdamW:
         self._torch = torch
         self._o = None
         self.handle = handle
-        self.params = list(params)
-        if not self.params:
+        params = tuple(params)
+        if not params:
             raise ValueError('AdamW needs at least one tensor')
         if state_bits not in (8, 32):
             raise ValueError('state_bits must be 32 or 8, got %r' % (state_bits,))
@@ -56,49 +57,54 @@ class AdamW:
         self.max_norm = None if max_norm is None else float(max_norm)
         if self.max_norm is not None and not self.max_norm > 0:
             raise ValueError('max_norm must be positive, got %r' % (max_norm,))
-        decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(self.params)
-        if len(decays) != len(self.params):
-            raise ValueError('%d weight decays for %d tensors' % (len(decays), len(self.params)))
+        decays = list(weight_decay) if isinstance(weight_decay, (list, tuple)) else [weight_decay] * len(params)
+        if len(decays) != len(params):
+            raise ValueError('%d weight decays for %d tensors' % (len(decays), len(params)))
         self._types = {torch.float32: 4, torch.bfloat16: 6, torch.float16: 7}          # SCS_F32, SCS_BF16, SCS_F16
         dev = torch.device('cuda', handle.device)
-        for i, p in enumerate(self.params):
+        for i, p in enumerate(params):
             self._check(p, i, 'parameter', dev)
         self.device = dev
         self.first, at = [], 0
-        for p in self.params:
+        for p in params:
             self.first.append(at)
             at += blocks_of(p.numel())
         self.blocks = at
         if states is None:
             dt = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
-            self.m, self.v = (torch.zeros((at * BLOCK,), dtype=d, device=dev) for d in dt)
-            self.m_scale, self.v_scale = (torch.zeros((at,), device=dev) if state_bits == 8 else None for _ in range(2))
+            m, v = (torch.zeros((at * BLOCK,), dtype=d, device=dev) for d in dt)
+            m_scale, v_scale = (torch.zeros((at,), device=dev) if state_bits == 8 else None for _ in range(2))
         else:
-            self.m, self.v, self.m_scale, self.v_scale = (tuple(states) + (None, None))[:4]
-        want = [(self.m, at * BLOCK, torch.float32 if state_bits == 32 else torch.int8, 'm'),
-                (self.v, at * BLOCK, torch.float32 if state_bits == 32 else torch.uint8, 'v')]
+            m, v, m_scale, v_scale = (tuple(states) + (None, None))[:4]
+        want = [(m, at * BLOCK, torch.float32 if state_bits == 32 else torch.int8, 'm'),
+                (v, at * BLOCK, torch.float32 if state_bits == 32 else torch.uint8, 'v')]
         if state_bits == 8:
-            want += [(self.m_scale, at, torch.float32, 'm_scale'), (self.v_scale, at, torch.float32, 'v_scale')]
+            want += [(m_scale, at, torch.float32, 'm_scale'), (v_scale, at, torch.float32, 'v_scale')]
         for t, n, dt, what in want:
             if not torch.is_tensor(t) or t.dtype != dt or t.device != dev or t.numel() != n or not t.is_contiguous():
                 raise ValueError('state %s must be a contiguous %s tensor of %d elements on %s' % (what, dt, n, dev))
-        self.masters = [p.detach().float() if master and p.dtype != torch.float32 else None for p in self.params]
-        table = (_Tensor * len(self.params))()
-        for t, p, w, d in zip(table, self.params, self.masters, decays):
+        masters = tuple(p.detach().float() if master and p.dtype != torch.float32 else None for p in params)
+        table = (_Tensor * len(params))()
+        for t, p, w, d in zip(table, params, masters, decays):
             t.param, t.master, t.n = p.data_ptr(), None if w is None else w.data_ptr(), p.numel()
             t.weight_decay, t.type = float(d), self._types[p.dtype]
         o = ctypes.c_void_p()
         lib = _hip.load_library()
         torch.cuda.current_stream(dev).synchronize()           # the masters and zeros are written on this stream; steps may run on another
-        _hip._check(lib.scs_adamw_create(handle.h, table, len(self.params), state_bits, self.m.data_ptr(), self.v.data_ptr(),
-                                         _hip._ptr(self.m_scale), _hip._ptr(self.v_scale), int(step), ctypes.byref(o)), 'scs_adamw_create')
+        _hip._check(lib.scs_adamw_create(handle.h, table, len(params), state_bits, m.data_ptr(), v.data_ptr(),
+                                         _hip._ptr(m_scale), _hip._ptr(v_scale), int(step), ctypes.byref(o)), 'scs_adamw_create')
         self._lib, self._o = lib, o
-        self._where = [p.data_ptr() for p in self.params]
-        held = self.params + [t for t in self.masters + [self.m, self.v, self.m_scale, self.v_scale] if t is not None]
-        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in held if t.numel())
-        self._starts, self._ends = [a for a, _ in spans], [b for _, b in spans]             # (they share no memory: both ascend)
         self.grads = self._bound = None
-        self.grad_norm = torch.zeros((1,), device=dev) if self.max_norm is not None else None      # of the last step, before clipping
+        grad_norm = torch.zeros((1,), device=dev) if self.max_norm is not None else None           # of the last step, before clipping
+        self._given = {'params': params, 'masters': masters, 'm': m, 'v': v, 'm_scale': m_scale, 'v_scale': v_scale, 'grad_norm': grad_norm}
+        self._watched = list(params) + [t for t in masters + (m, v, m_scale, v_scale, grad_norm) if t is not None]
+        self._held = [t.detach() for t in self._watched]               # (of the same memory, whatever becomes of the caller's)
+        self._where = [t.data_ptr() for t in self._watched]
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self._watched if t.numel())
+        self._starts, self._ends = [a for a, _ in spans], [b for _, b in spans]             # (they share no memory: both ascend)
+
+    params, masters, m, v, m_scale, v_scale, grad_norm = (
+        property(lambda self, k=k: self._given[k]) for k in ('params', 'masters', 'm', 'v', 'm_scale', 'v_scale', 'grad_norm'))
 
     def _check(self, t, i, what, dev):
         torch = self._torch
@@ -126,6 +132,10 @@ class AdamW:
                 raise ValueError('gradient %d shares memory with a parameter or a moment' % i)
         return grads, ptrs, types
 
+    def _moved(self):
+        if list(map(self._torch.Tensor.data_ptr, self._watched)) != self._where:
+            raise RuntimeError('a parameter, a master or a moment has moved since the optimiser was made')
+
     def bind(self, grads):
         """The gradient buffers that step() reads when it is given none (a program whose gradients stay where they are): checked once."""
         self.grads, *self._bound = self._gradients(grads)
@@ -142,8 +152,7 @@ class AdamW:
             ptrs, types = self._bound
         else:
             _, ptrs, types = self._gradients(grads)
-        if list(map(self._torch.Tensor.data_ptr, self.params)) != self._where:
-            raise RuntimeError('a parameter has moved since the optimiser was made')
+        self._moved()
         stream = self._torch._C._cuda_getCurrentRawStream(self.handle.device)
         _hip._check(self._lib.scs_adamw_step(self._o, ptrs, types, self.lr if lr is None else float(lr), self.betas[0], self.betas[1], self.eps,
                                              float(grad_scale), self.max_norm or 0.0,
@@ -160,6 +169,7 @@ class AdamW:
         for t in out:
             if not torch.is_tensor(t) or t.dtype != torch.float32 or t.device != self.device or t.numel() != self.blocks * BLOCK or not t.is_contiguous():
                 raise ValueError('out must be two contiguous float32 tensors of %d elements on %s' % (self.blocks * BLOCK, self.device))
+        self._moved()
         _hip._check(self._lib.scs_adamw_states(self._o, out[0].data_ptr(), out[1].data_ptr(), torch._C._cuda_getCurrentRawStream(self.handle.device) or None),
                     'scs_adamw_states')
         return tuple(out)

@@ -42,3 +42,74 @@ def test_c_entries_refuse_null():
 
 def test_blocks():
     assert [blocks_of(n) for n in (0, 1, 256, 257)] == [0, 1, 1, 2]
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    """Optimisers over host tensors, their library a list of the steps it was asked for: what is decided before a launch."""
+    steps = []
+
+    class Library:
+        scs_adamw_create = staticmethod(lambda *a: 0)
+        scs_adamw_destroy = staticmethod(lambda *a: 0)
+        scs_adamw_step = staticmethod(lambda *a: steps.append(a) or 0)
+        scs_adamw_states = staticmethod(lambda *a: steps.append(a) or 0)
+
+    cpu = torch.device('cpu')
+    monkeypatch.setattr(torch, 'device', lambda *a: cpu)
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda *a: type('Stream', (), {'synchronize': lambda self: None})())
+    monkeypatch.setattr(torch._C, '_cuda_getCurrentRawStream', lambda device: 0, raising=False)
+    monkeypatch.setattr(_hip, 'load_library', lambda: Library)
+    return steps
+
+
+def tensors():
+    return [torch.zeros(300, dtype=torch.bfloat16), torch.zeros(5, 7), torch.zeros(0)]
+
+
+def exchange(t):
+    """The tensor's memory replaced; the way back."""
+    old = t.data
+    t.data = t.clone()
+
+    def back():
+        t.data = old
+    return back
+
+
+@pytest.mark.parametrize('what', ['m', 'v', 'm_scale', 'v_scale', 'master', 'parameter', 'grad_norm'])
+def test_what_has_moved_is_refused(on_host, what):
+    """Every tensor whose address the optimiser holds."""
+    params, grads = tensors(), tensors()
+    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
+    opt.step()
+    back = exchange({'master': opt.masters[0], 'parameter': params[1]}[what] if what in ('master', 'parameter') else getattr(opt, what))
+    for call in (opt.step, lambda: opt.step(grads), opt.states):
+        with pytest.raises(RuntimeError, match='has moved'):
+            call()
+    assert len(on_host) == 1
+    back()
+    opt.step()
+    assert len(on_host) == 2
+
+
+def test_the_tensors_of_an_optimiser_cannot_be_exchanged(on_host):
+    """A replaced arena would be read by nobody and its predecessor freed under the next step."""
+    opt = AdamW(NoDevice, tensors(), state_bits=8, master=True, max_norm=1.0)
+    for name in ('params', 'masters', 'm', 'v', 'm_scale', 'v_scale', 'grad_norm'):
+        with pytest.raises(AttributeError):
+            setattr(opt, name, getattr(opt, name))
+    for name in ('params', 'masters'):
+        with pytest.raises(TypeError):
+            getattr(opt, name)[0] = None
+
+
+def test_the_memory_of_what_has_moved_is_kept(on_host):
+    """A captured step goes on using the memory that it was captured with."""
+    params = tensors()[:2]
+    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0)
+    held = params + [opt.masters[0], opt.m, opt.v, opt.m_scale, opt.v_scale, opt.grad_norm]
+    at = {t.data_ptr() for t in held}
+    for t in held:
+        t.data = t.clone()
+    assert at <= {t.data_ptr() for t in opt._held}
