@@ -137,8 +137,12 @@ class AdamW:
             raise RuntimeError('a parameter, a master or a moment has moved since the optimiser was made')
 
     def bind(self, grads):
-        """The gradient buffers that step() reads when it is given none (a program whose gradients stay where they are): checked once."""
+        """The gradient buffers that step() reads when it is given none: their types and places are checked here, once.  One whose memory has been
+        replaced since is refused by step() (bind() again); until then its old memory stays allocated."""
         self.grads, *self._bound = self._gradients(grads)
+        self._bound_grads = tuple(self.grads)
+        self._held_grads = [g.detach() for g in self.grads]
+        self._bound_where = [g.data_ptr() for g in self.grads]
         return self
 
     def step(self, grads=None, grad_scale=1.0, lr=None):
@@ -149,6 +153,8 @@ class AdamW:
         if grads is None:
             if self._bound is None:
                 raise ValueError('step() needs gradients: pass them or bind() them')
+            if list(map(self._torch.Tensor.data_ptr, self._bound_grads)) != self._bound_where:
+                raise RuntimeError('a bound gradient has moved: bind() again')
             ptrs, types = self._bound
         else:
             _, ptrs, types = self._gradients(grads)

@@ -93,6 +93,21 @@ def test_what_has_moved_is_refused(on_host, what):
     assert len(on_host) == 2
 
 
+def test_bound_gradients_that_have_moved_are_refused(on_host):
+    params, grads = tensors(), tensors()
+    opt = AdamW(NoDevice, params).bind(grads)
+    opt.step()
+    back = exchange(grads[1])
+    with pytest.raises(RuntimeError, match='bind'):
+        opt.step()
+    opt.step(grads)
+    opt.bind(grads).step()
+    back()
+    with pytest.raises(RuntimeError, match='bind'):
+        opt.step()
+    assert len(on_host) == 3
+
+
 def test_the_tensors_of_an_optimiser_cannot_be_exchanged(on_host):
     """A replaced arena would be read by nobody and its predecessor freed under the next step."""
     opt = AdamW(NoDevice, tensors(), state_bits=8, master=True, max_norm=1.0)
@@ -106,10 +121,10 @@ def test_the_tensors_of_an_optimiser_cannot_be_exchanged(on_host):
 
 def test_the_memory_of_what_has_moved_is_kept(on_host):
     """A captured step goes on using the memory that it was captured with."""
-    params = tensors()[:2]
-    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0)
-    held = params + [opt.masters[0], opt.m, opt.v, opt.m_scale, opt.v_scale, opt.grad_norm]
+    params, grads = tensors()[:2], tensors()[:2]
+    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
+    held = params + grads + [opt.masters[0], opt.m, opt.v, opt.m_scale, opt.v_scale, opt.grad_norm]
     at = {t.data_ptr() for t in held}
     for t in held:
         t.data = t.clone()
-    assert at <= {t.data_ptr() for t in opt._held}
+    assert at <= {t.data_ptr() for t in opt._held + opt._held_grads}
