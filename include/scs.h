@@ -397,7 +397,7 @@ typedef struct {
 } scs_adamw_tensor;
 
 /* The table is host memory and is copied; the device memory that it and the arenas name is the caller's and must stay until
- * scs_adamw_destroy.  Two tensors that share memory are refused.  `step`: steps already taken (0 for a new optimiser; the caller zeroes
+ * scs_adamw_destroy.  Parameters, masters, moments or scales that share memory are refused.  `step`: steps already taken (0 for a new optimiser; the caller zeroes
  * the arenas).  The optimiser lives on h's device and does not need h afterwards. */
 int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, int state_bits, void* m_dev, void* v_dev,
                      float* m_scale_dev, float* v_scale_dev, int64_t step, scs_adamw* out);

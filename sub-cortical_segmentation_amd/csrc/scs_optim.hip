@@ -458,7 +458,7 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
         std::vector<std::pair<uintptr_t, uintptr_t>> spans;
         scs_adamw_ctx* o = new scs_adamw_ctx();
         struct Drop { scs_adamw_ctx*& o; ~Drop() { if (o) { if (o->mem) (void)hipFree(o->mem); delete o; } } } drop{o};
-        o->device = handle_device(h); o->bits = state_bits; o->n = n;
+        o->bits = state_bits; o->n = n;
         int64_t chunks = 0;
         for (int i = 0; i < n; ++i) if (tensors[i].n > 0) chunks += (tensors[i].n + kChunkBlocks * kOptBlock - 1) / (kChunkBlocks * kOptBlock);
         if (chunks < kManyChunks) o->chunk_blocks = kSmallBlocks;
@@ -487,15 +487,21 @@ int scs_adamw_create(scs_handle h, const scs_adamw_tensor* tensors, int32_t n, i
             o->sizes.push_back(t.n);
         }
         o->chunk0.push_back((int32_t)ch.size());
-        std::sort(spans.begin(), spans.end());
-        for (size_t i = 1; i < spans.size(); ++i)
-            SCS_ARG(spans[i - 1].second <= spans[i].first, "two parameters overlap (the same tensor twice?)");
         SCS_ARG(o->blocks == 0 || (m_dev && v_dev), "the moments are NULL");
         SCS_ARG(state_bits == 32 || o->blocks == 0 || (m_scale_dev && v_scale_dev), "8-bit moments need their scales");
         SCS_ARG((uintptr_t)m_dev % 16 == 0 && (uintptr_t)v_dev % 16 == 0 && (uintptr_t)m_scale_dev % 4 == 0 && (uintptr_t)v_scale_dev % 4 == 0,
                 "the moments must be aligned to 16 bytes");
+        // what a step writes shares no memory: parameters, masters, moments, scales
+        auto arena = [&](const void* p, size_t b) { if (p && o->blocks) spans.emplace_back((uintptr_t)p, (uintptr_t)p + (uintptr_t)o->blocks * b); };
+        arena(m_dev, kOptBlock * (state_bits == 32 ? 4 : 1));
+        arena(v_dev, kOptBlock * (state_bits == 32 ? 4 : 1));
+        if (state_bits == 8) { arena(m_scale_dev, 4); arena(v_scale_dev, 4); }
+        std::sort(spans.begin(), spans.end());
+        for (size_t i = 1; i < spans.size(); ++i)
+            SCS_ARG(spans[i - 1].second <= spans[i].first, "two of the parameters, masters and moments overlap (the same tensor twice?)");
         o->m = m_dev; o->v = v_dev; o->ms = m_scale_dev; o->vs = v_scale_dev;
         o->launches = (n + kGradsPerLaunch - 1) / kGradsPerLaunch;
+        o->device = handle_device(h);
         DeviceGuard dev(o->device);
         if (dev.rc != SCS_OK) return dev.rc;
         auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };

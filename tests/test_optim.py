@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from cnn_cort import _hip
-from cnn_cort.optim import AdamW, blocks_of
+from cnn_cort.optim import BLOCK, AdamW, blocks_of
 
 
 class NoDevice:
@@ -128,3 +128,22 @@ def test_the_memory_of_what_has_moved_is_kept(on_host):
     for t in held:
         t.data = t.clone()
     assert at <= {t.data_ptr() for t in opt._held + opt._held_grads}
+
+
+@pytest.mark.parametrize('bits,case', [(32, 'm and v'), (32, 'm in a parameter'), (32, 'v in a master'), (8, 'm and v'), (8, 'the scales'), (8, 'a scale in v'),
+                                       (8, 'v in a master'), (8, 'a scale in a parameter')])
+def test_moments_that_share_memory_are_refused(bits, case):
+    """The entry looks at sizes and addresses alone before it asks for a device: 1000 and 600 bf16 parameters with masters own 7 blocks."""
+    from cnn_cort.optim import _Tensor
+    lib = _hip.load_library()
+    handle = ctypes.create_string_buffer(1 << 16)                     # (read for its device number alone)
+    table = (_Tensor * 2)(_Tensor(0x100000, 0x200000, 1000, 0.0, 6, 0), _Tensor(0x110000, 0x210000, 600, 0.0, 6, 0))
+    at = {'m': 0x300000, 'v': 0x400000, 'm_scale': 0x500000, 'v_scale': 0x600000}
+    size = 7 * BLOCK * (4 if bits == 32 else 1)
+    at.update({'m and v': {'v': at['m'] + size - 16}, 'm in a parameter': {'m': 0x110000 + 1200 - 16}, 'v in a master': {'v': 0x210000 - size + 16},
+               'the scales': {'v_scale': at['m_scale'] + 24}, 'a scale in v': {'m_scale': at['v'] + size - 4},
+               'a scale in a parameter': {'v_scale': 0x100000 + 1996}}[case])
+    out = ctypes.c_void_p()
+    scales = [at['m_scale'], at['v_scale']] if bits == 8 else [None, None]
+    assert lib.scs_adamw_create(handle, table, 2, bits, at['m'], at['v'], *scales, 0, ctypes.byref(out)) == -1 and not out.value
+    assert b'overlap' in lib.scs_last_error()
