@@ -414,7 +414,8 @@ int scs_adamw_destroy(scs_adamw o);
 int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_types, double lr, double beta1, double beta2, double eps,
                    double grad_scale, double max_norm, float* norm_dev, void* stream);
 
-/* The values that 8-bit moments stand for: f32 [blocks * 256] each, in the arenas' layout (checkpoints, inspection). */
+/* The values that 8-bit moments stand for: f32 [blocks * 256] each, in the arenas' layout (checkpoints, inspection).  The two outputs share no
+ * memory with each other nor with what the optimiser holds. */
 int scs_adamw_states(scs_adamw o, float* m_out_dev, float* v_out_dev, void* stream);
 
 /* Steps taken.  get waits for the stream; set enqueues. */

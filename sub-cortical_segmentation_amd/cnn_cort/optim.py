@@ -115,6 +115,11 @@ class AdamW:
         if not t.is_contiguous():
             raise ValueError('%s %d must be contiguous' % (what, i))
 
+    def _shares(self, t):
+        """Whether t shares memory with what the optimiser holds."""
+        k = bisect.bisect_right(self._ends, t.data_ptr())
+        return bool(t.numel()) and k < len(self._starts) and self._starts[k] < t.data_ptr() + t.numel() * t.element_size()
+
     def _gradients(self, grads):
         grads = list(grads)
         if len(grads) != len(self.params):
@@ -127,8 +132,7 @@ class AdamW:
                 raise ValueError('gradient %d has %d elements, its parameter %d' % (i, g.numel(), p.numel()))
             at = ptrs[i] = g.data_ptr()
             types[i] = self._types[g.dtype]
-            k = bisect.bisect_right(self._ends, at)
-            if g.numel() and k < len(self._starts) and self._starts[k] < at + g.numel() * g.element_size():
+            if self._shares(g):
                 raise ValueError('gradient %d shares memory with a parameter or a moment' % i)
         return grads, ptrs, types
 
@@ -175,6 +179,8 @@ class AdamW:
         for t in out:
             if not torch.is_tensor(t) or t.dtype != torch.float32 or t.device != self.device or t.numel() != self.blocks * BLOCK or not t.is_contiguous():
                 raise ValueError('out must be two contiguous float32 tensors of %d elements on %s' % (self.blocks * BLOCK, self.device))
+        if any(map(self._shares, out)) or (self.blocks and abs(out[0].data_ptr() - out[1].data_ptr()) < self.blocks * BLOCK * 4):
+            raise ValueError('out shares memory with what the optimiser holds, or the two with each other')
         self._moved()
         _hip._check(self._lib.scs_adamw_states(self._o, out[0].data_ptr(), out[1].data_ptr(), torch._C._cuda_getCurrentRawStream(self.handle.device) or None),
                     'scs_adamw_states')

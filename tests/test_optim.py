@@ -147,3 +147,17 @@ def test_moments_that_share_memory_are_refused(bits, case):
     scales = [at['m_scale'], at['v_scale']] if bits == 8 else [None, None]
     assert lib.scs_adamw_create(handle, table, 2, bits, at['m'], at['v'], *scales, 0, ctypes.byref(out)) == -1 and not out.value
     assert b'overlap' in lib.scs_last_error()
+
+
+def test_read_out_into_memory_in_use_is_refused(on_host):
+    opt = AdamW(NoDevice, tensors(), state_bits=8, master=True)
+    free = [torch.zeros(opt.blocks * BLOCK) for _ in range(2)]
+    opt.states(out=free)
+    arena = torch.zeros(opt.blocks * BLOCK + 4)
+    other = AdamW(NoDevice, [torch.zeros(opt.blocks * BLOCK)], state_bits=8)
+    for bad in ([free[0], free[0]], [arena[:-4], arena[4:]]):
+        with pytest.raises(ValueError, match='shares memory'):
+            opt.states(out=bad)
+    with pytest.raises(ValueError, match='shares memory'):
+        other.states(out=[other.params[0], free[1]])
+    assert len(on_host) == 1
