@@ -130,6 +130,8 @@ class AdamW:
             self._check(g, i, 'gradient', self.device)
             if g.numel() != p.numel():
                 raise ValueError('gradient %d has %d elements, its parameter %d' % (i, g.numel(), p.numel()))
+            if g.shape != p.shape and g.dim() != 1 and p.dim() != 1:
+                raise ValueError('gradient %d has the shape %r, its parameter %r' % (i, tuple(g.shape), tuple(p.shape)))
             at = ptrs[i] = g.data_ptr()
             types[i] = self._types[g.dtype]
             if self._shares(g):
@@ -150,8 +152,8 @@ class AdamW:
         return self
 
     def step(self, grads=None, grad_scale=1.0, lr=None):
-        """One update from `grads` (one tensor per parameter, float32 / bfloat16 / float16; default: the bound ones), each multiplied by
-        grad_scale first.  `lr` replaces self.lr for this step."""
+        """One update from `grads` (one tensor per parameter, of its shape or flat, float32 / bfloat16 / float16; default: the bound ones), each
+        multiplied by grad_scale first.  `lr` replaces self.lr for this step."""
         if self._o is None:
             raise RuntimeError('the optimiser is closed')
         if grads is None:

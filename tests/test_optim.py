@@ -161,3 +161,18 @@ def test_read_out_into_memory_in_use_is_refused(on_host):
     with pytest.raises(ValueError, match='shares memory'):
         other.states(out=[other.params[0], free[1]])
     assert len(on_host) == 1
+
+
+def test_gradients_of_another_shape_are_refused(on_host):
+    """As many elements in another order are another gradient; flat ones (slices of a gradient arena) are the parameter's own order."""
+    p = torch.zeros(5, 7)
+    opt = AdamW(NoDevice, [p])
+    for bad in (torch.zeros(7, 5), torch.zeros(35, 1), torch.zeros(1, 5, 7)):
+        with pytest.raises(ValueError, match='shape'):
+            opt.step([bad])
+        with pytest.raises(ValueError, match='shape'):
+            opt.bind([bad])
+    opt.step([torch.zeros(5, 7)])
+    opt.step([torch.zeros(35)])
+    AdamW(NoDevice, [p.view(-1)]).step([torch.zeros(5, 7)])
+    assert len(on_host) == 3
