@@ -33,7 +33,8 @@ class AdamW:
       weight_decay  one number, or one per tensor
       state_bits    32: moments m, v as float32 arenas; 8: int8 / uint8 codes with a float32 scale per 256 elements
       max_norm      None, or the norm over all gradients to clip at; a step whose norm is not finite changes nothing
-      master        True: 16-bit parameters are rounded copies of float32 values that the optimiser keeps (self.masters)
+      master        True: 16-bit parameters are rounded copies of float32 values that the optimiser keeps (self.masters; made from the parameters
+                    as they are), or the masters of another AdamW over the same parameters, to go on from (used where they lie, as `states` are)
       states        None (zeros), or (m, v, m_scale, v_scale) of another AdamW over tensors of the same sizes; `step`: steps they have seen
 
     self.m, self.v, self.m_scale, self.v_scale are the arenas: tensor i owns blocks [self.first[i], self.first[i] + blocks_of(n_i)) of 256
@@ -83,7 +84,18 @@ class AdamW:
         for t, n, dt, what in want:
             if not torch.is_tensor(t) or t.dtype != dt or t.device != dev or t.numel() != n or not t.is_contiguous():
                 raise ValueError('state %s must be a contiguous %s tensor of %d elements on %s' % (what, dt, n, dev))
-        masters = tuple(p.detach().float() if master and p.dtype != torch.float32 else None for p in params)
+        if isinstance(master, (list, tuple)):
+            masters = tuple(master)
+            if len(masters) != len(params):
+                raise ValueError('%d masters for %d tensors' % (len(masters), len(params)))
+            for i, (w, p) in enumerate(zip(masters, params)):
+                if p.dtype == torch.float32:
+                    if w is not None:
+                        raise ValueError('master %d: a float32 parameter takes none' % i)
+                elif not torch.is_tensor(w) or w.dtype != torch.float32 or w.device != dev or w.shape != p.shape or not w.is_contiguous():
+                    raise ValueError('master %d must be a contiguous float32 %r on %s' % (i, tuple(p.shape), dev))
+        else:
+            masters = tuple(p.detach().float() if master and p.dtype != torch.float32 else None for p in params)
         table = (_Tensor * len(params))()
         for t, p, w, d in zip(table, params, masters, decays):
             t.param, t.master, t.n = p.data_ptr(), None if w is None else w.data_ptr(), p.numel()

@@ -356,3 +356,31 @@ def test_gradients_in_the_optimisers_memory_are_refused(handle, bits):
             opt.step([t, free[1]])
     opt.step(free)
     assert opt.step_count == 2
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+@pytest.mark.parametrize('pt', ['bf16', 'f16'])
+def test_a_resumed_run_with_masters_is_the_uninterrupted_one(handle, bits, pt):
+    """Steps far below a 16-bit step of the parameters add up in the masters alone: everything an optimiser holds, through host copies, into another one."""
+    kw = dict(lr=1e-5, weight_decay=0.01, state_bits=bits, max_norm=1.0)
+    whole, part = make(SIZES, TYPES[pt], 61), make(SIZES, TYPES[pt], 61)
+    start = [p.clone() for p in whole]
+    one = AdamW(handle, whole, master=True, **kw)
+    two = AdamW(handle, part, master=True, **kw)
+    for t in range(3):
+        g = gradients(SIZES, TYPES[pt], 70 + t)
+        one.step(g)
+        two.step(g)
+    back = lambda t: None if t is None else t.cpu().clone().to('cuda:0')
+    fresh = [back(p) for p in part]
+    three = AdamW(handle, fresh, master=[back(t) for t in two.masters], states=[back(t) for t in (two.m, two.v, two.m_scale, two.v_scale)],
+                  step=two.step_count, **kw)
+    two.close()
+    for t in range(3, 40):
+        g = gradients(SIZES, TYPES[pt], 70 + t % 5)
+        one.step(g)
+        three.step(g)
+    assert one.step_count == three.step_count == 40
+    for a, b in zip(list(whole) + list(one.masters) + [one.m, one.v], list(fresh) + list(three.masters) + [three.m, three.v]):
+        assert torch.equal(a, b)
+    assert any(not torch.equal(a, b) for a, b in zip(start, whole))

@@ -176,3 +176,17 @@ def test_gradients_of_another_shape_are_refused(on_host):
     opt.step([torch.zeros(35)])
     AdamW(NoDevice, [p.view(-1)]).step([torch.zeros(5, 7)])
     assert len(on_host) == 3
+
+
+def test_masters_are_handed_back(on_host):
+    """A resumed optimiser goes on from the masters it is given, not from their rounded copies."""
+    params = tensors()
+    first = AdamW(NoDevice, params, master=True)
+    first.masters[0].add_(2.0 ** -20)
+    again = AdamW(NoDevice, params, master=first.masters)
+    assert again.masters[0] is first.masters[0] and again.masters[1:] == (None, None)
+    kept = first.masters[0]
+    for bad, match in (([kept], '1 masters'), ([None] * 3, 'master 0'), ([kept[:-1], None, None], 'master 0'), ([kept.bfloat16(), None, None], 'master 0'),
+                       ([kept, torch.zeros(5, 7), None], 'master 1'), ([torch.zeros(600)[::2], None, None], 'master 0')):
+        with pytest.raises(ValueError, match=match):
+            AdamW(NoDevice, params, master=bad)
