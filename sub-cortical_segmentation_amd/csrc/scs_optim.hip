@@ -422,6 +422,7 @@ __global__ __launch_bounds__(256) void adamw_states_kernel(const unsigned int* _
 }
 
 __global__ void adamw_set_step_kernel(OptState* st, int64_t step) { st->step = step; }
+__global__ void adamw_count_kernel(OptState* st, int32_t clipped) { if (!(clipped && st->skip)) st->step += 1; }
 
 }  // namespace
 }  // namespace scs
@@ -579,6 +580,8 @@ int scs_adamw_step(scs_adamw o, const void* const* grads, const int32_t* grad_ty
         const int lo = l * kGradsPerLaunch, hi = std::min(o->n, lo + kGradsPerLaunch);
         if (o->chunk0[hi] > o->chunk0[lo]) last = l;
     }
+    // (no element at all: nothing is updated, the step counts)
+    if (last < 0) hipLaunchKernelGGL(adamw_count_kernel, dim3(1), dim3(1), 0, st, o->st, (int32_t)(max_norm > 0));
     for (int l = 0; l <= last; ++l) {
         const auto c = fill(l);
         if (c.second == c.first) continue;

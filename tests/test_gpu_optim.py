@@ -384,3 +384,18 @@ def test_a_resumed_run_with_masters_is_the_uninterrupted_one(handle, bits, pt):
     for a, b in zip(list(whole) + list(one.masters) + [one.m, one.v], list(fresh) + list(three.masters) + [three.m, three.v]):
         assert torch.equal(a, b)
     assert any(not torch.equal(a, b) for a, b in zip(start, whole))
+
+
+@pytest.mark.parametrize('clip', [None, 1.0])
+def test_steps_over_nothing_are_counted(handle, clip):
+    """Tensors of no element are passed over; the step is one all the same."""
+    opt = AdamW(handle, [torch.zeros((0,), device='cuda:0'), torch.zeros((4, 0), device='cuda:0')], max_norm=clip)
+    grads = [torch.zeros((0,), device='cuda:0'), torch.zeros((4, 0), device='cuda:0')]
+    opt.step(grads)
+    opt.step(grads)
+    assert opt.step_count == 2
+    if clip:
+        assert float(opt.grad_norm) == 0.0
+    opt.step_count = 7
+    opt.step(grads)
+    assert opt.step_count == 8
