@@ -444,10 +444,12 @@ __device__ __forceinline__ void wgrad_direct(const WgradProblem<T>& w, const Req
     f32x4 acc[JT][4];
     wgrad_clear<JT>(acc);
     int turn = 0;                                             // (requests of a row or two each: the waves take them in turn)
+    bool used = false;                                        // (an adapter without rows: zeros, whatever its scale holds)
     for (int q0 = 0; q0 < r.n; q0 += 64) {
         const int q = q0 + lane, c = min(q, r.n - 1);
         const int lo = clamp_row(r.offsets[c], r.rows), hi = clamp_row(r.offsets[c + 1], r.rows);
         unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
+        used |= todo != 0;
         for (; todo; todo &= todo - 1) {
             const int at = __builtin_ctzll(todo);
             const int a = __builtin_amdgcn_readlane(lo, at), b = __builtin_amdgcn_readlane(hi, at);
@@ -455,7 +457,7 @@ __device__ __forceinline__ void wgrad_direct(const WgradProblem<T>& w, const Req
             turn = (turn + (b - a + kWgradRows<JT> - 1) / kWgradRows<JT>) % W;
         }
     }
-    wgrad_store<JT, W>(s_part, acc, wave, r.rank, w.F, col, r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
+    wgrad_store<JT, W>(s_part, acc, wave, r.rank, w.F, col, used && r.scale ? r.scale[s] : 1.f, w.out + (int64_t)s * r.rank * w.F);
 }
 
 template <int JT> constexpr int direct_waves() { return JT <= 2 ? kFewWaves : 4; }             // (the join's LDS)
@@ -494,10 +496,12 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs<T> g) {
     if ((int64_t)blockIdx.x * 1024 >= n) return;
     const int left = (int)min(n - i, (int64_t)4);
     f32x4 sum = f32x4{0.f, 0.f, 0.f, 0.f};
+    bool used = false;                                        // (as in wgrad_direct)
     for (int q0 = 0; q0 < r.n; q0 += 64) {
         const int q = q0 + lane, c = min(q, r.n - 1);
         const int lo = clamp_row(r.offsets[c], r.rows), hi = clamp_row(r.offsets[c + 1], r.rows);
         unsigned long long todo = __ballot(q < r.n && r.adapters[c] == s && lo < hi);
+        used |= todo != 0;
         for (; todo; todo &= todo - 1) {
             const int at = __builtin_ctzll(todo);
             const int b_lo = __builtin_amdgcn_readlane(lo, at) / g.block_rows, b_hi = (__builtin_amdgcn_readlane(hi, at) - 1) / g.block_rows;
@@ -509,7 +513,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs<T> g) {
             }
         }
     }
-    if (left > 0) raw_store<float>(sum * (r.scale ? r.scale[s] : 1.f), w.out + (int64_t)s * n + i, left);
+    if (left > 0) raw_store<float>(sum * (used && r.scale ? r.scale[s] : 1.f), w.out + (int64_t)s * n + i, left);
 }
 
 // ------------------------------------------------------------------------------------------------------------------ host side

@@ -431,3 +431,22 @@ def test_one_row_in_a_graph(handle, t):
         y = p.forward(d['x'], o, i, hidden=h2)
         torch.cuda.synchronize()
         assert torch.equal(out, y) and torch.equal(hidden, h2), 'replay %d' % k
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('rows', [0, 20, 300, 700, 2000])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_an_unused_adapters_gradients_are_zeros_whatever_its_scale(handle, t, rows, bad):
+    """An adapter that no row uses has zero gradients: its scale (an unfinished site's, say) takes no part."""
+    d = data(t, rows, 96, 200, 8, 4, 7)
+    d['scale'][1], d['scale'][3] = bad, bad
+    p = Projection(handle, d['w'], d['a'], d['b'], scale=d['scale'])
+    q = Projection(handle, d['w'], d['a'], d['b'], scale=torch.where(torch.isfinite(d['scale']), d['scale'], torch.ones_like(d['scale'])))
+    # adapter 1: a request without rows, adapter 3: no request; the last rows use none
+    o, i = requests([0, rows // 2, rows // 2, rows - rows // 8, rows], [0, 1, 2, -1])
+    for n in (4, 0):
+        got, want = (x.backward(d['x'], d['dy'], o[:n + 1], i[:n], da=torch.ones(d['a'].shape, device='cuda:0'), db=torch.ones(d['b'].shape, device='cuda:0')) for x in (p, q))
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+        for g in got[1:]:
+            assert not g[1].any() and not g[3].any() and (rows < 8 or n == 0 or g[0].any())
