@@ -39,9 +39,17 @@ __device__ __forceinline__ s16x4 lds_transposed(const void* p) {
 }
 
 // 16 bytes a lane from base + offset (bytes) to LDS byte `lds` + 16 lane; no register is written, so none can be overtaken
+// (m0 belongs to the compiler, which has to be told; it warns that it may not save it across the statement, and nothing needs it saved)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy_to_lds(const void* base, unsigned int offset, unsigned int lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(offset), "s"(base) : "memory", "m0");
 }
+// ... and from an address of the lane's own
+__device__ __forceinline__ void copy_to_lds(const void* src, unsigned int lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
+}
+#pragma clang diagnostic pop
 template <int N> __device__ __forceinline__ void copies_but() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(N) : "memory"); }
 __device__ __forceinline__ void workgroup_barrier() {
     asm volatile("" : : : "memory");

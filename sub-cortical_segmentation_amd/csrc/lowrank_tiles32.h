@@ -14,10 +14,6 @@
 namespace scs {
 namespace {
 
-__device__ __forceinline__ void copy_to_lds(const void* src, unsigned int lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
-}
-
 // EVEN: N is a multiple of 4
 template <int MT, int NT, bool TRANS, bool EVEN>
 __global__ __launch_bounds__(256, NT <= 6 ? 3 : 2) void project_tiles32_kernel(ProjectArgs<float> g) {

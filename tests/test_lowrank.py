@@ -84,3 +84,19 @@ def test_the_memory_of_a_moved_tensor_is_kept(on_host):
     for t in d.values():
         t.data = t.clone()
     assert sorted(t.data_ptr() for t in p._held) == sorted(at)
+
+
+def test_inline_assembly_names_the_register_that_it_overwrites():
+    """m0 is the compiler's: a statement that writes it says so, or a value kept there would be lost without a word."""
+    import glob
+    import os
+    import re
+    from conftest import PKG
+    found = 0
+    for path in glob.glob(os.path.join(PKG, 'csrc', '*.h')) + glob.glob(os.path.join(PKG, 'csrc', '*.hip')):
+        with open(path) as f:
+            for statement in re.findall(r'asm volatile\((.*?)\);', f.read(), re.S):
+                if re.search(r's_mov_b32 m0\b', statement):
+                    found += 1
+                    assert statement.rstrip().endswith('"m0"'), (path, statement)
+    assert found == 2
