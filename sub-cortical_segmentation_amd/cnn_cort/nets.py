@@ -139,6 +139,7 @@ class Net:
             raise ValueError("optimizer must be 'adam' or 'adamw', got %r" % (optimizer,))
         self.optimizer, self.weight_decay = optimizer, float(weight_decay)
         self.optimizer_bits, self.max_norm = int(optimizer_bits), None if max_norm is None else float(max_norm)
+        self._optimiser = None       # the AdamW of fit(): moments and step count go on from one fit to the next until weights are loaded
         self.adapters = None         # SiteAdapters (fit_adapters, load_adapters_from)
         self._adapters_behind = False                # the shared weights have changed since the adapters' layers took them
         self.seed = int(seed)
@@ -184,7 +185,10 @@ class Net:
                 self._params = P.init_params(self.seed)       # Lasagne default initialisers (training from scratch)
                 self._dirty = True
             if self._dirty:
-                self._handle.set_params(P.params_to_flat(self._params))
+                self._handle.set_params(P.params_to_flat(self._params))         # (its Adam starts anew: AdamW as well)
+                if self._optimiser is not None:
+                    self._optimiser.close()
+                    self._optimiser = None
                 self._dirty = False
                 self._dev_newer = False
             return self._handle
@@ -982,15 +986,14 @@ class Net:
             pass
         finally:
             h.set_fused_adam(False)            # the handle goes back to the two-call form (scs_train_step, scs_adam_apply)
-            if adamw is not None:
-                adamw.close()
             if not compact:
                 pool.shutdown(wait=False)
         return self
 
     def _adamw(self, h):
         """AdamW over the trained arrays of the parameter arena (batch-norm mean and inv_std are running statistics); weight decay on
-        the convolution and dense weights alone."""
+        the convolution and dense weights alone.  Made anew for every fit() with the Net's present settings, it takes over the moments and the step
+        count of the one before (unless optimizer_bits has changed: then it starts from zeros)."""
         from . import dist
         from .optim import AdamW
         dev = self._dev()
@@ -1004,7 +1007,14 @@ class Net:
                     grads.append(g[at:at + n])
                     decays.append(self.weight_decay if len(shape) > 1 else 0.0)
                 at += n
-        return AdamW(h, params, lr=self.update_learning_rate, weight_decay=decays, state_bits=self.optimizer_bits, max_norm=self.max_norm).bind(grads)
+        before, states, step = self._optimiser, None, 0
+        if before is not None and before.state_bits == self.optimizer_bits:
+            states, step = (before.m, before.v, before.m_scale, before.v_scale), before.step_count
+        self._optimiser = AdamW(h, params, lr=self.update_learning_rate, weight_decay=decays, state_bits=self.optimizer_bits, max_norm=self.max_norm,
+                                states=states, step=step).bind(grads)
+        if before is not None:
+            before.close()
+        return self._optimiser
 
     def _train_batch(self, h, views, atl, yy, nb, seed, stream, aug_rng, rank):
         if self.augment and nb > 1:

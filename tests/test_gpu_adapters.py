@@ -224,3 +224,29 @@ def test_new_weights_reach_the_adapted_head(weights, batch):
     fitted = net.predict_proba(X)
     assert np.abs(fitted - base).max() > 1e-3
     assert np.abs(net.predict_proba(X, sites=sites) - fitted).max() < 1e-4
+
+
+@pytest.mark.parametrize('bits,clip', [(32, None), (8, 1.0)])
+def test_a_second_fit_goes_on_with_adamw(weights, bits, clip):
+    """fit(epochs=1) three times is fit(epochs=3): moments and step count go on until weights are loaded, as Adam's do."""
+    t = gold('g5_train.npz')
+    X = {'in1': t['ax'], 'in2': t['co'], 'in3': t['sa'], 'in4': t['atlas']}
+    kw = dict(batch_size=X['in1'].shape[0], eval_size=0.0, optimizer='adamw', optimizer_bits=bits, max_norm=clip, weight_decay=0.1, update_learning_rate=1e-3, seed=3)
+    same = lambda a, b: all(np.array_equal(x, y) for k in a for x, y in zip(a[k], b[k]))
+    whole, parts = make_net(weights, **kw), make_net(weights, **kw)
+    whole.fit(X, t['y'], epochs=3)
+    once = None
+    for i in range(3):
+        parts.fit(X, t['y'], epochs=1)
+        once = once or parts.get_all_params_values()
+    assert same(whole.get_all_params_values(), parts.get_all_params_values())
+    # another rate or decay between the calls applies to the steps behind it; moments of other bits start anew
+    assert parts._optimiser.step_count == 3
+    parts.weight_decay, parts.optimizer_bits = 0.0, 40 - bits
+    parts.fit(X, t['y'], epochs=1)
+    assert parts._optimiser.step_count == 1 and parts._optimiser.state_bits == 40 - bits
+    # new weights: the optimiser starts anew with them
+    whole.load_params_from(weights)
+    whole._step = 0
+    whole.fit(X, t['y'], epochs=1)
+    assert same(whole.get_all_params_values(), once)
