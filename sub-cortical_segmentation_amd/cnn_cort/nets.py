@@ -139,6 +139,12 @@ class Net:
             raise ValueError("optimizer must be 'adam' or 'adamw', got %r" % (optimizer,))
         self.optimizer, self.weight_decay = optimizer, float(weight_decay)
         self.optimizer_bits, self.max_norm = int(optimizer_bits), None if max_norm is None else float(max_norm)
+        if self.optimizer_bits not in (8, 32):
+            raise ValueError('optimizer_bits must be 32 or 8, got %r' % (optimizer_bits,))
+        if not np.isfinite(self.weight_decay):
+            raise ValueError('weight_decay must be finite, got %r' % (weight_decay,))
+        if self.max_norm is not None and not self.max_norm > 0:
+            raise ValueError('max_norm must be positive (None: no clipping), got %r' % (max_norm,))
         self._optimiser = None       # the AdamW of fit(): moments and step count go on from one fit to the next until weights are loaded
         self.adapters = None         # SiteAdapters (fit_adapters, load_adapters_from)
         self._adapters_behind = False                # the shared weights have changed since the adapters' layers took them
@@ -778,6 +784,7 @@ class Net:
         if y_all.size and (y_all.min() < 0 or y_all.max() > 14):
             raise ValueError('labels must lie in 0..14')
         h = self._ensure_handle()
+        adamw = self._adamw(h) if self.optimizer == 'adamw' else None          # (refuses impossible settings before anything is started)
         dev = 'cuda:%d' % self._dev()
         stream = torch.cuda.current_stream(self._dev()).cuda_stream
         world, rank = dist.world_size(), dist.rank()
@@ -922,7 +929,6 @@ class Net:
             print('-------  ----------  ----------  ---------  -----------  -----')
         # one rank: nothing sits between a step's gradients and their update, so the step applies lasagne.updates.adam itself,
         # group by group as the gradients become final (scs_set_fused_adam: same arithmetic, no launch behind the step)
-        adamw = self._adamw(h) if self.optimizer == 'adamw' else None
         fused = adamw is None and not dist.is_dist()
         h.set_fused_adam(fused, lr=self.update_learning_rate)
         self._adapters_behind = True

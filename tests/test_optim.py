@@ -190,3 +190,12 @@ def test_masters_are_handed_back(on_host):
                        ([kept, torch.zeros(5, 7), None], 'master 1'), ([torch.zeros(600)[::2], None, None], 'master 0')):
         with pytest.raises(ValueError, match=match):
             AdamW(NoDevice, params, master=bad)
+
+
+def test_a_nets_optimiser_options_are_checked_when_it_is_made():
+    from cnn_cort.nets import Net
+    for bad, match in (({'optimizer_bits': 16}, 'optimizer_bits'), ({'max_norm': 0.0}, 'max_norm'), ({'max_norm': -1.0}, 'max_norm'),
+                       ({'max_norm': float('nan')}, 'max_norm'), ({'weight_decay': float('nan')}, 'weight_decay'), ({'weight_decay': float('inf')}, 'weight_decay')):
+        with pytest.raises(ValueError, match=match):
+            Net(optimizer='adamw', **bad)
+    Net(optimizer='adamw', optimizer_bits=8, max_norm=1.0, weight_decay=0.0)
