@@ -13,6 +13,7 @@
 // the contraction: 14.3 for 14.5 us and 28 for 21.5; twice as many: 17.4 and 29.
 #pragma once
 #include "scs_ops.h"
+#include "lowrank_rules.h"
 #include "lowrank_tiles.h"
 
 namespace scs {
@@ -36,8 +37,6 @@ __device__ __forceinline__ f32x4 coherent_load(__amdgpu_buffer_rsrc_t b, int at)
     return v;
 }
 __device__ __forceinline__ void stores_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-
-constexpr int kFewWaves = 8;
 
 // where four columns from n on can be read from any row but W's last one (from the last one as well where N % 4 == 0)
 __device__ __forceinline__ int few_column(int n, int N) { return min(n, N % 4 ? N - 1 : N - 4); }

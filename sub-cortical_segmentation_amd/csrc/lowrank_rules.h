@@ -1,0 +1,113 @@
+// Which form of the shared projection's kernels a call takes (scs_lowrank.hip): rules on sizes, types and alignment alone, host code without the device's.
+#pragma once
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/scs.h"
+
+namespace scs {
+namespace {
+
+constexpr int kFewWaves = 8;              // waves of a workgroup of the few-rows form (lowrank_few.h)
+
+// directions of an adapter in tiles of 16, as the kernels are compiled: 1, 2, 4, 8
+inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
+
+// ---- shrink
+constexpr int kDotRows = 512;               // up to so many rows the shrink is a wave per row and direction
+
+// Above: waves that share a row tile's contraction, about two units of 256 bytes of a row (128 where many directions fill the registers) each; two row tiles
+// a wave (P read half as often) where workgroups abound.
+struct ShrinkForm { int mt, waves; };
+inline ShrinkForm shrink_form(const scs_lowrank& p, int64_t K) {
+    const int jt = rank_tiles(p.rank), unit = (jt <= 2 ? 4 : 2) * 64 / (p.dtype == SCS_F32 ? 4 : 2);
+    const int64_t units = (K + unit - 1) / unit;
+    if (p.rows >= 16384) return {jt <= 2 ? 2 : 1, units >= 16 ? 8 : 4};
+    return {1, units >= 32 ? (jt <= 2 ? 16 : 8) : units >= 16 ? 8 : 4};
+}
+
+// ---- gradients of the adapters
+// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows (more where a
+// grid's 65535 would not do); direct up to 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank
+// f32 values a column each) would hold more than four times X's own bytes.
+constexpr int kDirectRows = 512;
+int wgrad_block_rows(const scs_lowrank& p) {
+    const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
+    const int64_t rows = std::max<int64_t>(std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64)), (p.rows / 65535 + 64) / 64 * 64);
+    const int64_t blocks = (p.rows + rows - 1) / rows;
+    if (p.rows <= kDirectRows || blocks <= 1 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
+    return (int)rows;
+}
+
+// ---- project: few rows (lowrank_few.h)
+struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; int tickets = 0; };      // mt 0: the tile kernels
+// f32 tiles (lowrank_tiles32.h): columns / 16 of the tile with the least padding; among equals the one that ran fastest at 60 000 x 540 x 540 (6: 306 us,
+// 5: 303, 7: 321, 4: 322; 8 pads there)
+int f32_columns(int64_t N) {
+    int nt = 0;
+    int64_t waste = INT64_MAX;
+    for (const int n : {6, 5, 8, 7, 4}) {
+        const int64_t w = (N + 16 * n - 1) / (16 * n) * 16 * n;
+        if (w < waste) { waste = w; nt = n; }
+    }
+    return nt;
+}
+// ... and its rows / 64: the higher tile where that still gives every CU one, the lower where that gives most of them one, 0: neither does
+int f32_rows(int64_t rows, int64_t N) {
+    const int64_t across = (N + 16 * f32_columns(N) - 1) / (16 * f32_columns(N));
+    return (rows + 127) / 128 * across >= 256 ? 2 : (rows + 63) / 64 * across >= 192 ? 1 : 0;
+}
+// The few-rows form: up to 64 rows in 16 bits (128 rows at 4096 x 4096 take 28 us as tiles), in f32 wherever the tiles would leave CUs idle (512 rows
+// at 540 x 540: 18 us, as tiles 46)
+Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
+    Few f;
+    if (p.rows == 0) return f;
+    if (p.dtype == SCS_F32 ? f32_rows(p.rows, N) != 0 : p.rows > 64) return f;
+    f.mt = p.dtype == SCS_F32 ? (p.rows >= 256 && K * N >= (1 << 21) ? 2 : 1) : (int)(p.rows + 15) / 16;
+    f.tiles_n = (int)((N + 63) / 64);
+    f.tiles_m = (int)((p.rows + 16 * f.mt - 1) / (16 * f.mt));
+    const int64_t steps = (K + 31) / 32;
+    f.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)f.tiles_n * f.tiles_m), steps / (2 * kFewWaves)));
+    if (f.splits > 1) {
+        f.part = (size_t)f.splits * f.tiles_m * 16 * f.mt * f.tiles_n * 64 * 4;
+        f.tickets = f.tiles_n * f.tiles_m;
+    }
+    return f;
+}
+// What of a projection's operands has to be laid out anew for the tile kernels: K up to a multiple of 64 (16-bit) or 4 (f32), rows at multiples
+// of 16 bytes.  `K`, `N`: of this direction; `x`, `ldx`: X as the call gets it.
+struct Pack { bool x = false, w = false; int64_t K = 0, nw = 0, w_rows = 0, w_cols = 0; size_t x_bytes = 0, w_bytes = 0; };
+Pack pack_of(const scs_lowrank& p, int64_t K, int64_t N, bool trans, const void* x, int64_t ldx) {
+    Pack k;
+    const int e = p.dtype == SCS_F32 ? 4 : 2, per = 16 / e, unit = p.dtype == SCS_F32 ? 4 : 64;
+    auto whole = [](int64_t v, int64_t u) { return (v + u - 1) / u * u; };
+    k.K = whole(K, unit);
+    // (2^21: the tile kernels' offsets inside a tile have 32 bits)
+    k.x = k.K != K || ldx % per || (uintptr_t)x % 16 || ldx > (1 << 21);
+    k.w = k.K != K || p.ldw % per || (uintptr_t)p.w % 16 || (!trans && N % per) || p.ldw > (1 << 21);
+    k.nw = trans ? N : whole(N, per);
+    k.w_rows = trans ? N : k.K;
+    k.w_cols = trans ? k.K : k.nw;
+    if (k.x) k.x_bytes = (size_t)p.rows * k.K * e;
+    if (k.w) k.w_bytes = (size_t)k.w_rows * k.w_cols * e;
+    return k;
+}
+
+// ---- project: 16-bit tiles (lowrank_tiles.h)
+// the largest 16-bit tile that still gives most of the 256 CUs one
+int tile16(int64_t rows, int64_t N) {
+    auto tiles = [&](int64_t b) { return (rows + b - 1) / b * ((N + b - 1) / b); };
+    return tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
+}
+
+// ---- launches of two things at once, where neither fills the card and dx does not read what the other writes
+// dx of few rows and the gradients in the direct form (not with thousands of adapters: the one launch's threads along x have to stay below 2^32)
+inline bool few_beside_wgrad(const scs_lowrank& p, const Few& f) { return f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && p.n_adapters <= 128 && !wgrad_block_rows(p); }
+// dx in the smallest 16-bit tiles and the gradients by blocks of rows
+inline bool tiles_beside_wgrad(const scs_lowrank& p, const Few& f) {
+    return p.dtype != SCS_F32 && !f.mt && p.rank <= 32 && tile16(p.rows, p.in_features) == 64 && wgrad_block_rows(p);
+}
+
+}  // namespace
+}  // namespace scs

@@ -310,6 +310,7 @@ struct ProjectArgs {
 
 }  // namespace
 }  // namespace scs
+#include "lowrank_rules.h"
 #include "lowrank_tiles.h"
 #include "lowrank_tiles32.h"
 #include "lowrank_few.h"
@@ -517,75 +518,7 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(WgradArgs<T> g) {
 }
 
 // ------------------------------------------------------------------------------------------------------------------ host side
-constexpr int kDotRows = 512;               // up to so many rows the shrink is a wave per row and direction
-
 size_t up(size_t b) { return (b + 255) & ~(size_t)255; }
-
-// Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows (more where a
-// grid's 65535 would not do); direct up to 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank
-// f32 values a column each) would hold more than four times X's own bytes.
-constexpr int kDirectRows = 512;
-int wgrad_block_rows(const scs_lowrank& p) {
-    const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
-    const int64_t rows = std::max<int64_t>(std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64)), (p.rows / 65535 + 64) / 64 * 64);
-    const int64_t blocks = (p.rows + rows - 1) / rows;
-    if (p.rows <= kDirectRows || blocks <= 1 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
-    return (int)rows;
-}
-
-// ---- few rows (lowrank_few.h)
-struct Few { int mt = 0, splits = 1, tiles_n = 0, tiles_m = 0; size_t part = 0; int tickets = 0; };      // mt 0: the tile kernels
-// f32 tiles (lowrank_tiles32.h): columns / 16 of the tile with the least padding; among equals the one that ran fastest at 60 000 x 540 x 540 (6: 306 us,
-// 5: 303, 7: 321, 4: 322; 8 pads there)
-int f32_columns(int64_t N) {
-    int nt = 0;
-    int64_t waste = INT64_MAX;
-    for (const int n : {6, 5, 8, 7, 4}) {
-        const int64_t w = (N + 16 * n - 1) / (16 * n) * 16 * n;
-        if (w < waste) { waste = w; nt = n; }
-    }
-    return nt;
-}
-// ... and its rows / 64: the higher tile where that still gives every CU one, the lower where that gives most of them one, 0: neither does
-int f32_rows(int64_t rows, int64_t N) {
-    const int64_t across = (N + 16 * f32_columns(N) - 1) / (16 * f32_columns(N));
-    return (rows + 127) / 128 * across >= 256 ? 2 : (rows + 63) / 64 * across >= 192 ? 1 : 0;
-}
-// The few-rows form: up to 64 rows in 16 bits (128 rows at 4096 x 4096 take 28 us as tiles), in f32 wherever the tiles would leave CUs idle (512 rows
-// at 540 x 540: 18 us, as tiles 46)
-Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
-    Few f;
-    if (p.rows == 0) return f;
-    if (p.dtype == SCS_F32 ? f32_rows(p.rows, N) != 0 : p.rows > 64) return f;
-    f.mt = p.dtype == SCS_F32 ? (p.rows >= 256 && K * N >= (1 << 21) ? 2 : 1) : (int)(p.rows + 15) / 16;
-    f.tiles_n = (int)((N + 63) / 64);
-    f.tiles_m = (int)((p.rows + 16 * f.mt - 1) / (16 * f.mt));
-    const int64_t steps = (K + 31) / 32;
-    f.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / ((int64_t)f.tiles_n * f.tiles_m), steps / (2 * kFewWaves)));
-    if (f.splits > 1) {
-        f.part = (size_t)f.splits * f.tiles_m * 16 * f.mt * f.tiles_n * 64 * 4;
-        f.tickets = f.tiles_n * f.tiles_m;
-    }
-    return f;
-}
-// What of a projection's operands has to be laid out anew for the tile kernels: K up to a multiple of 64 (16-bit) or 4 (f32), rows at multiples
-// of 16 bytes.  `K`, `N`: of this direction; `x`, `ldx`: X as the call gets it.
-struct Pack { bool x = false, w = false; int64_t K = 0, nw = 0, w_rows = 0, w_cols = 0; size_t x_bytes = 0, w_bytes = 0; };
-Pack pack_of(const scs_lowrank& p, int64_t K, int64_t N, bool trans, const void* x, int64_t ldx) {
-    Pack k;
-    const int e = p.dtype == SCS_F32 ? 4 : 2, per = 16 / e, unit = p.dtype == SCS_F32 ? 4 : 64;
-    auto whole = [](int64_t v, int64_t u) { return (v + u - 1) / u * u; };
-    k.K = whole(K, unit);
-    // (2^21: the tile kernels' offsets inside a tile have 32 bits)
-    k.x = k.K != K || ldx % per || (uintptr_t)x % 16 || ldx > (1 << 21);
-    k.w = k.K != K || p.ldw % per || (uintptr_t)p.w % 16 || (!trans && N % per) || p.ldw > (1 << 21);
-    k.nw = trans ? N : whole(N, per);
-    k.w_rows = trans ? N : k.K;
-    k.w_cols = trans ? k.K : k.nw;
-    if (k.x) k.x_bytes = (size_t)p.rows * k.K * e;
-    if (k.w) k.w_bytes = (size_t)k.w_rows * k.w_cols * e;
-    return k;
-}
 
 struct Layout { size_t hid = 0, hid2 = 0, part = 0, tickets = 0, rows = 0, rows2 = 0, slots = 0, pieces = 0, pack_x = 0, pack_w = 0, bytes = 0; };
 Layout layout_of(const scs_lowrank& p, bool backward, const void* x, int64_t ldx) {
@@ -632,10 +565,10 @@ int check(const scs_lowrank* p) {
 Requests requests_of(const scs_lowrank& p) { return Requests{p.offsets, p.adapters, p.scale, p.n_requests, p.n_adapters, p.rank, (int32_t)p.rows}; }
 
 template <class F> void by_tiles(int rank, F&& f) {
-    const int t = (rank + 15) / 16;
-    if (t <= 1) f(std::integral_constant<int, 1>{});
-    else if (t <= 2) f(std::integral_constant<int, 2>{});
-    else if (t <= 4) f(std::integral_constant<int, 4>{});
+    const int t = rank_tiles(rank);
+    if (t == 1) f(std::integral_constant<int, 1>{});
+    else if (t == 2) f(std::integral_constant<int, 2>{});
+    else if (t == 4) f(std::integral_constant<int, 4>{});
     else f(std::integral_constant<int, 8>{});
 }
 
@@ -647,21 +580,19 @@ template <class T> void shrink(const scs_lowrank& p, const T* x, int64_t ldx, co
         hipLaunchKernelGGL(shrink_dots_kernel<T>, dim3((unsigned)p.rows, (p.rank + 3) / 4), dim3(256), 0, st, x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets);
         return;
     }
+    const ShrinkForm f = shrink_form(p, K);
     by_tiles(p.rank, [&](auto jt) {
-        // about two units a wave; two row tiles a wave (P read half as often) where workgroups abound
-        constexpr int UNIT = (jt.value <= 2 ? 4 : 2) * 64 / (int)sizeof(T);
-        const int units = (K + UNIT - 1) / UNIT;
         auto go = [&](auto mt, auto w) {
             hipLaunchKernelGGL((shrink_rows_kernel<T, jt.value, mt.value, w.value>), dim3((unsigned)((p.rows + 16 * mt.value - 1) / (16 * mt.value) + pk.groups)), dim3(64 * w.value), 0, st,
                                x, ldx, low, K, h, pieces, r, row_adapter, tickets, n_tickets, pk);
         };
-        constexpr int MT = jt.value <= 2 ? 2 : 1, MOST = jt.value <= 2 ? 16 : 8;             // (registers)
+        constexpr int MT = jt.value <= 2 ? 2 : 1, MOST = jt.value <= 2 ? 16 : 8;
         typedef std::integral_constant<int, 1> One;
-        if (p.rows >= 16384) {
-            if (units >= 16) go(std::integral_constant<int, MT>{}, std::integral_constant<int, 8>{});
+        if (f.mt == 2) {
+            if (f.waves == 8) go(std::integral_constant<int, MT>{}, std::integral_constant<int, 8>{});
             else go(std::integral_constant<int, MT>{}, std::integral_constant<int, 4>{});
-        } else if (units >= 32) go(One{}, std::integral_constant<int, MOST>{});
-        else if (units >= 16) go(One{}, std::integral_constant<int, 8>{});
+        } else if (f.waves == MOST) go(One{}, std::integral_constant<int, MOST>{});
+        else if (f.waves == 8) go(One{}, std::integral_constant<int, 8>{});
         else go(One{}, std::integral_constant<int, 4>{});
     });
 }
@@ -677,12 +608,6 @@ template <class T, bool TRANS> void launch_few(const ProjectArgs<T>& g, const Fe
         if (f.mt == 3) go(std::integral_constant<int, 3>{});
         else go(std::integral_constant<int, 4>{});
     }
-}
-
-// the largest 16-bit tile that still gives most of the 256 CUs one
-int tile16(int64_t rows, int64_t N) {
-    auto tiles = [&](int64_t b) { return (rows + b - 1) / b * ((N + b - 1) / b); };
-    return tiles(256) >= 192 ? 256 : tiles(128) >= 192 ? 128 : 64;
 }
 
 template <class T, bool TRANS, bool EVEN> void project_tiles(const ProjectArgs<T>& g, hipStream_t st) {
@@ -791,8 +716,7 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         }
         w[n++] = WgradProblem<T>{h, (const T*)dy, lddy, db, nullptr, (int)p.out_features};
     }
-    // (not with thousands of adapters: the one launch's threads along x have to stay below 2^32)
-    if (dx && n && f.mt >= 1 && f.mt <= 2 && p.rank <= 32 && p.n_adapters <= 128 && !wgrad_block_rows(p)) {
+    if (dx && n && few_beside_wgrad(p, f)) {
         const int tiles = (std::max(w[0].F, n > 1 ? w[1].F : 0) + 63) / 64;
         const FewGrid grid{f.tiles_n, f.tiles_m, f.splits};
         const WgradArgs<T> wa{{w[0], w[1]}, 0, requests_of(p)};
@@ -804,7 +728,7 @@ int backward(const scs_lowrank& p, const void* x, int64_t ldx, const void* dy, i
         typedef std::integral_constant<int, 2> Two;
         if (f.mt == 1) { if (p.rank <= 16) go(One{}, One{}); else go(One{}, Two{}); }
         else { if (p.rank <= 16) go(Two{}, One{}); else go(Two{}, Two{}); }
-    } else if (sizeof(T) == 2 && dx && n && !f.mt && p.rank <= 32 && tile16(p.rows, p.in_features) == 64 && wgrad_block_rows(p)) {
+    } else if (dx && n && tiles_beside_wgrad(p, f)) {
         // neither dx in small tiles nor the partial sums fill the card: one launch
         if constexpr (sizeof(T) == 2) {
             const int n_tiles = (int)((p.rows + 63) / 64 * ((p.in_features + 63) / 64));

@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+import lowrank_forms
 from cnn_cort import _hip
 from cnn_cort.adapters import Projection
 
@@ -450,3 +451,10 @@ def test_an_unused_adapters_gradients_are_zeros_whatever_its_scale(handle, t, ro
             assert torch.equal(a, b)
         for g in got[1:]:
             assert not g[1].any() and not g[3].any() and (rows < 8 or n == 0 or g[0].any())
+
+
+@pytest.mark.parametrize('t,rows,n_in,n_out,rank', [(t,) + s for t in TYPES for s in lowrank_forms.sizes(t)])
+def test_every_form_against_float64(handle, t, rows, n_in, n_out, rank):
+    """The kernels that the other sizes do not reach (test_lowrank.py sees to it that none is left)."""
+    off, ids = lowrank_forms.requests(rows)
+    check_all(handle, data(t, rows, n_in, n_out, rank, 3, rows + n_in + rank, bias=rank % 2 == 0), off, ids, t)

@@ -100,3 +100,13 @@ def test_inline_assembly_names_the_register_that_it_overwrites():
                     found += 1
                     assert statement.rstrip().endswith('"m0"'), (path, statement)
     assert found == 2
+
+
+@pytest.mark.parametrize('t', ['f32', 'bf16', 'f16'])
+def test_the_device_tests_reach_every_form(t, tmp_path):
+    """Every variant that the rules on sizes can choose is one that a test compares with float64; a rule that is changed shows here."""
+    import lowrank_forms
+    from test_gpu_lowrank import CASES
+    calls = [(t,) + c[:5] + (len(c[6]),) for c in CASES.values()] + [(t,) + s + (3, 5) for s in lowrank_forms.sizes(t)]
+    reached = set().union(*lowrank_forms.forms(calls, tmp_path))
+    assert reached == lowrank_forms.every_form(t)
