@@ -29,14 +29,21 @@ inline ShrinkForm shrink_form(const scs_lowrank& p, int64_t K) {
 
 // ---- gradients of the adapters
 // Rows of a block of the by-blocks form, 0: the direct form.  Blocks so that there are about 2048 workgroups, of 64 to 512 rows (more where a
-// grid's 65535 would not do); direct up to 512 rows (the second launch would cost more than it saves), or where the slots (requests + blocks, rank
-// f32 values a column each) would hold more than four times X's own bytes.
+// grid's 65535 would not do); direct up to 512 rows (the second launch would cost more than it saves), and where the slots (requests + blocks, rank
+// f32 values a column each) would weigh too much: more than four times X's own bytes, or more than X because requests make up four fifths of them (each
+// is written and read once, and a request of a few rows costs a block's waves as much as sixteen).  By blocks / direct, us, dA and dB:
+//   8192 x 4096 + 4096, bf16, rank 16, adapters 1 and 8: 10 requests 75 / 113 and 70 / 65, 100 requests 136 / 135 and 95 / 72, 400 requests 389 / 189 and
+//   204 / 92; 900 requests 403 / 124 (8 adapters), where the slots took 490 MB of workspace
+//   60 000 x 540 + 540, f32, rank 8, adapters 1 and 8: 10 requests 126 / 665 and 102 / 167, 400 requests 345 / 739 and 136 / 136
+//   4096 x 2048 + 2048, bf16, rank 64, adapters 1 and 8: 10 requests 108 / 194 and 103 / 74, 400 requests 618 / 317 and 434 / 87
+// (with several adapters the direct form is the faster one in some of what is left to the blocks, by up to a half; nothing looks at that)
 constexpr int kDirectRows = 512;
 int wgrad_block_rows(const scs_lowrank& p) {
     const int64_t tiles = (std::max(p.in_features, p.out_features) + 63) / 64;
     const int64_t rows = std::max<int64_t>(std::min<int64_t>(512, std::max<int64_t>(64, (p.rows * tiles / 2048 + 63) / 64 * 64)), (p.rows / 65535 + 64) / 64 * 64);
     const int64_t blocks = (p.rows + rows - 1) / rows;
-    if (p.rows <= kDirectRows || blocks <= 1 || (p.n_requests + blocks) * p.rank > p.rows * (p.dtype == SCS_F32 ? 4 : 2)) return 0;
+    const int64_t slots = (p.n_requests + blocks) * p.rank * 4, x = p.rows * (p.dtype == SCS_F32 ? 4 : 2);             // bytes a column
+    if (p.rows <= kDirectRows || blocks <= 1 || slots > 4 * x || (slots > x && p.n_requests > 4 * blocks)) return 0;
     return (int)rows;
 }
 

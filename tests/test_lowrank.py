@@ -110,3 +110,14 @@ def test_the_device_tests_reach_every_form(t, tmp_path):
     calls = [(t,) + c[:5] + (len(c[6]),) for c in CASES.values()] + [(t,) + s + (3, 5) for s in lowrank_forms.sizes(t)]
     reached = set().union(*lowrank_forms.forms(calls, tmp_path))
     assert reached == lowrank_forms.every_form(t)
+
+
+@pytest.mark.parametrize('requests,most', [(10, 1.5), (100, 1.7), (900, 1.2), (8192, 1.2)])
+def test_partial_sums_of_short_requests_do_not_outweigh_the_rows(requests, most):
+    """Workspace of the gradients of 8192 rows of 4096 + 4096 columns in bf16 (128 MB), in their bytes."""
+    from cnn_cort.adapters import _Call
+    lib, n = _hip.load_library(), ctypes.c_size_t(0)
+    some = ctypes.c_void_p(16)
+    call = _Call(6, 16, 8, requests, 8192, 4096, 4096, 4096, some, None, some, some, None, some, some)
+    assert lib.scs_lowrank_workspace(some, ctypes.byref(call), 1, some, 4096, ctypes.byref(n)) == 0
+    assert n.value <= most * 8192 * 8192 * 2
