@@ -15,7 +15,10 @@ constexpr int kFewWaves = 8;              // waves of a workgroup of the few-row
 inline int rank_tiles(int rank) { return rank <= 16 ? 1 : rank <= 32 ? 2 : rank <= 64 ? 4 : 8; }
 
 // ---- shrink
-constexpr int kDotRows = 512;               // up to so many rows the shrink is a wave per row and direction
+// Up to so many rows a workgroup takes four directions of one row (and reads P once for every row), above a tile of rows.  The whole forward call in us, the one
+// way / the other: 540 x 540, f32, rank 8, 128 rows 11.9 / 12.4, 512 rows 17.3 / 17.2, 1024 rows 24.7 / 23.2; 4096 x 512, bf16, rank 16, 26.8 / 31.3, 32.5 / 32.1,
+// 40.9 / 32.1; the same of rank 64 35.8 / 46.5, 58.8 / 45.6, 87.5 / 45.6 (the two meet at 256 rows there, at 384 for rank 32: the rule does not look at the rank)
+constexpr int kDotRows = 512;
 
 // Above: waves that share a row tile's contraction, about two units of 256 bytes of a row (128 where many directions fill the registers) each; two row tiles
 // a wave (P read half as often) where workgroups abound.
@@ -66,7 +69,9 @@ int f32_rows(int64_t rows, int64_t N) {
     return (rows + 127) / 128 * across >= 256 ? 2 : (rows + 63) / 64 * across >= 192 ? 1 : 0;
 }
 // The few-rows form: up to 64 rows in 16 bits (128 rows at 4096 x 4096 take 28 us as tiles), in f32 wherever the tiles would leave CUs idle (512 rows
-// at 540 x 540: 18 us, as tiles 46)
+// at 540 x 540: 18 us, as tiles 46).  Row tiles a workgroup, f32: two halve W's reads and the workgroups.  One / two, us: 128 x 2048 x 2048 20.5 / 22.1,
+// 256 x 540 x 540 12.1 / 16.6, 512 x 1448 x 1448 43.7 / 48.5 are left to one; 300 x 1500 x 1500 30.6 / 27.6, 400 x 2048 x 1024 37.0 / 32.8 and 256 x 1024 x 2048
+// 23.7 / 20.8 gain from two, 256 x 2048 x 1024 20.0 / 21.9 and 700 x 2052 x 1033 62.6 / 69.8 lose a tenth by it
 Few few_of(const scs_lowrank& p, int64_t K, int64_t N) {
     Few f;
     if (p.rows == 0) return f;
