@@ -11,7 +11,11 @@
 // fragment reads, 1024 cycles of the LDS's 128 bytes a cycle against 1024 of MFMA.  Four waves of 128 x 128 would read a third less, but
 // their 256 sums leave the compiler too few registers: 530 us instead of 260 at 8192 x 4096 x 4096.  What hides latency is the pipeline: four slabs
 // of LDS, three in flight while one is read, a slab's fragments read into registers while the slab before is multiplied, one barrier a slab
-// that no copy has to be drained for (drained at every slab: 350 us).  8192 x 4096 x 4096, bf16: about 230 us, 1200 TFLOP/s.
+// that no copy has to be drained for (drained at every slab: 350 us).  8192 x 4096 x 4096, bf16: about 230 us, 1200 TFLOP/s.  The largest tile spills
+// registers (bf16 23 to 26 a lane, f16 54 to 55), all of them behind the loop over the contraction: in the adapters' pass and at the end, once a tile.
+// The adapters' pass costs a tile two barriers and a masked product of the WHOLE tile for every request in it and 16 directions: many requests of a row
+// or two are its worst case (4096 x 4096, bf16, rank 16: 128 rows of 128 requests 97 us, of four requests 30; 1024 rows 394 and 53, the shrink's passes
+// over the contraction, one a request of a row tile, among them).
 //
 // The copies are issued from inline assembly because the compiler, which tracks them, waits for every one of them before the next LDS read; the
 // waits are written out instead (copies return in order: vmcnt(n) leaves the n youngest in flight).

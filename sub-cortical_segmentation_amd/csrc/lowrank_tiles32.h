@@ -3,8 +3,8 @@
 //
 // What bounds it: v_mfma_f32_16x16x4_f32, 32 cycles each on the vector ALUs, which every other vector instruction takes time from: so the copies
 // go to LDS without passing registers and addresses are a uniform base and a fixed offset a lane.  A workgroup of four waves owns
-// 64 MT rows x 16 NT columns (16 MT rows a wave).  60 000 x 540 x 540: 303 us, 115 TFLOP/s, where 154 is what a large library product reaches and
-// 126 to 139 what this instruction sustains back to back.
+// 64 MT rows x 16 NT columns (16 MT rows a wave).  60 000 x 540 x 540: 303 us, 115 TFLOP/s.  This
+// instruction issued back to back sustains 139 (scs_probe_f32_mfma); the library reaches 154 at 8192 x 8192 x 8192 and 87 (401 us) at this size.
 // LDS images of a slab of 16 along the contraction, in 16-byte pieces:
 //   K-major [row][16]: piece c of a row at c ^ (row >> 2 & 3); a lane's piece is its operand of four products.  X, and W^T in the backward pass
 //   N-major [16][BN]:  column n of row k at (n + 16 (k >> 2)) mod BN, so that a fragment's four rows lie at different banks.  W, and P

@@ -80,7 +80,7 @@ struct Walk {
 // rows, each wave a share of the contraction, joined through LDS; operands go from global memory to the matrix cores without a stop (both are
 // contiguous along the contraction: a lane's 16 bytes are its operand of one 16-bit product or of four f32 ones, whose contraction
 // indices are permuted alike on both sides), four steps' loads in flight.  8192 x 4096, bf16, rank 16: 27 us, half the rate of a copy (other
-// numbers of waves and row tiles measured alike); 60 000 x 540, f32: 38 us.
+// numbers of waves and row tiles measured alike); 60 000 x 540, f32: 38 us.  Every request of a row tile is a pass over the whole contraction.
 template <class T> __device__ __forceinline__ f32x4 product16(const u32x4& a, const u32x4& b, f32x4 c) {
     if constexpr (sizeof(T) == 4) {
         f32x4 x, y;
@@ -323,7 +323,7 @@ namespace {
 // turn, sixteen at a time, and are joined through LDS in a fixed order.  dA and dB are one launch.
 //   by blocks: a workgroup owns a block of rows as well and leaves one partial sum for each request in it, in slot request + block (along the
 //              rows one of the two grows from each partial sum to the next: no slot is met twice); wgrad_join_kernel adds an adapter's slots up
-//   direct:    a workgroup owns one adapter and walks its requests (few rows, or requests so many that their slots would outweigh X)
+//   direct:    a workgroup owns one adapter and walks its requests (few rows, or requests so many and short that their slots would outweigh X)
 // 8192 rows of 4096 + 4096 columns, bf16, rank 16, ten requests: 46 us and 8 us of join, 2.9 TB/s of X.
 template <class T> struct WgradProblem { const float* h; const T* x; int64_t ldx; float* out; float* part; int32_t F; };
 template <class T> struct WgradArgs { WgradProblem<T> p[2]; int32_t block_rows; Requests r; };
