@@ -84,7 +84,7 @@ class AdamW:
         for t, n, dt, what in want:
             if not torch.is_tensor(t) or t.dtype != dt or t.device != dev or t.numel() != n or not t.is_contiguous():
                 raise ValueError('state %s must be a contiguous %s tensor of %d elements on %s' % (what, dt, n, dev))
-        if isinstance(master, (list, tuple)):
+        if not isinstance(master, int):                        # (True and False are)
             masters = tuple(master)
             if len(masters) != len(params):
                 raise ValueError('%d masters for %d tensors' % (len(masters), len(params)))

@@ -458,3 +458,28 @@ def test_every_form_against_float64(handle, t, rows, n_in, n_out, rank):
     """The kernels that the other sizes do not reach (test_lowrank.py sees to it that none is left)."""
     off, ids = lowrank_forms.requests(rows)
     check_all(handle, data(t, rows, n_in, n_out, rank, 3, rows + n_in + rank, bias=rank % 2 == 0), off, ids, t)
+
+
+@pytest.mark.parametrize('which', ['w', 'a', 'b', 'bias', 'scale'])
+def test_each_moved_tensor_is_refused_and_captured_calls_keep_theirs(handle, which):
+    """forward() and backward() refuse; a graph captured before reads the memory that it was captured with, which is still the projection's."""
+    d, off, ids = some('bf16', 40)
+    o, i = requests(off, ids)
+    p = Projection(handle, d['w'], d['a'], d['b'], bias=d['bias'], scale=d['scale'])
+    y = torch.zeros((40, 200), dtype=torch.bfloat16, device='cuda:0')
+    want = p.forward(d['x'], o, i)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p.forward(d['x'], o, i, out=y)
+    d[which].data = torch.full_like(d[which], float('nan'))
+    for call in (lambda: p.forward(d['x'], o, i), lambda: p.backward(d['x'], d['dy'], o, i)):
+        with pytest.raises(RuntimeError, match='moved'):
+            call()
+    junk = [torch.full_like(t, 3.0) for t in d.values() for _ in range(4)]             # (would land in memory that had been freed)
+    for _ in range(3):
+        y.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+    del junk

@@ -399,3 +399,40 @@ def test_steps_over_nothing_are_counted(handle, clip):
     opt.step_count = 7
     opt.step(grads)
     assert opt.step_count == 8
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_states_by_tensor_and_their_memory(handle, bits):
+    params = [p.view(s) for p, s in zip(make([35, 600, 0, 1], torch.float32, 81), ((5, 7), (600,), (0, 3), ()))]
+    opt = AdamW(handle, params, state_bits=bits)
+    grads = [torch.randn(p.shape, device='cuda:0') for p in params]
+    opt.step(grads)
+    m, v = opt.states()
+    for i, (p, g) in enumerate(zip(params, grads)):
+        mi, vi = opt.state_of(i)
+        at = opt.first[i] * BLOCK
+        assert mi.shape == vi.shape == p.shape
+        assert torch.equal(mi.reshape(-1), m[at:at + p.numel()]) and torch.equal(vi.reshape(-1), v[at:at + p.numel()])
+        assert ((mi != 0) | (g == 0)).all() or bits == 8
+    assert opt.blocks == 1 + 3 + 0 + 1
+    assert opt.bytes_per_element() == 5 * (BLOCK * 8 if bits == 32 else BLOCK * 2 + 8) / 636
+
+
+@pytest.mark.parametrize('bits', [32, 8])
+def test_a_moved_arena_or_master_is_refused(handle, bits):
+    """Their old memory stays allocated, so that a graph that was captured before goes on with what it had."""
+    params = make([1000, 300], torch.bfloat16, 82)
+    opt = AdamW(handle, params, state_bits=bits, master=True, max_norm=1.0)
+    g = gradients([1000, 300], torch.bfloat16, 83)
+    opt.step(g)
+    for t in [opt.masters[1], opt.m, opt.v, opt.grad_norm] + ([opt.m_scale, opt.v_scale] if bits == 8 else []):
+        old = t.data
+        t.data = t.clone()
+        with pytest.raises(RuntimeError, match='moved'):
+            opt.step(g)
+        t.data = old
+    opt.step(g)
+    assert opt.step_count == 2
+    with pytest.raises(_hip.ScsError, match='overlap'):
+        both = torch.zeros((6 * BLOCK,), device='cuda:0')
+        AdamW(handle, params, states=(both, both, None, None))
