@@ -370,7 +370,9 @@ int scs_lowrank_forward(scs_handle h, const scs_lowrank* p, const void* x_dev, i
                         void* workspace_dev, size_t workspace_bytes, void* stream);
 
 /* hidden: what the forward call left, or NULL (formed again from x).  Each of dx [rows][in], da [n_adapters][rank][in] and
- * db [n_adapters][rank][out] (both f32, written whole) may be NULL and is then not formed.  Sums are formed in a fixed order: the same call gives the same bits. */
+ * db [n_adapters][rank][out] (both f32, written whole) may be NULL and is then not formed.  The outputs share no memory with each other nor with what the
+ * call reads (they are written while it is still read).  An adapter that no row uses gets zeros whatever its scale holds.  Sums are formed in a fixed
+ * order: the same call gives the same bits. */
 int scs_lowrank_backward(scs_handle h, const scs_lowrank* p, const void* x_dev, int64_t ldx, const void* dy_dev, int64_t lddy,
                          const float* hidden_dev, void* dx_dev, int64_t lddx, float* da_dev, float* db_dev,
                          void* workspace_dev, size_t workspace_bytes, void* stream);

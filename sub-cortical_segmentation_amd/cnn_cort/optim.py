@@ -117,7 +117,7 @@ class AdamW:
         self._arenas_where = [f() for f in self._arenas]
         self._norm_at = None if grad_norm is None else grad_norm.data_ptr()
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self._watched if t.numel())
-        self._starts, self._ends = [a for a, _ in spans], [b for _, b in spans]             # (they share no memory: both ascend)
+        self._starts, self._ends = [a for a, _ in spans] + [math.inf], [b for _, b in spans]             # (they share no memory: both ascend)
 
     params, masters, m, v, m_scale, v_scale, grad_norm = (
         property(lambda self, k=k: self._given[k]) for k in ('params', 'masters', 'm', 'v', 'm_scale', 'v_scale', 'grad_norm'))
@@ -135,8 +135,7 @@ class AdamW:
 
     def _shares(self, at, end):
         """Whether memory from `at` to `end` holds some of what the optimiser holds."""
-        k = bisect.bisect_right(self._ends, at)
-        return k < len(self._starts) and self._starts[k] < end and at < end
+        return self._starts[bisect.bisect_right(self._ends, at)] < end and at < end
 
     def _gradients(self, grads):
         grads = list(grads)
@@ -196,10 +195,10 @@ class AdamW:
             out = tuple(torch.empty((n,), device=self.device) for _ in range(2))
         m, v = out
         for t in (m, v):
-            if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.device != self.device or t.numel() != n or not t.is_contiguous():
+            if not isinstance(t, torch.Tensor) or t.dtype is not torch.float32 or t.get_device() != self._index or t.numel() != n or not t.is_contiguous():
                 raise ValueError('out must be two contiguous float32 tensors of %d elements on %s' % (n, self.device))
         at, to = m.data_ptr(), v.data_ptr()
-        if self._shares(at, at + 4 * n) or self._shares(to, to + 4 * n) or (n and abs(at - to) < 4 * n):
+        if n and (abs(at - to) < 4 * n or self._shares(at, at + 4 * n) or self._shares(to, to + 4 * n)):
             raise ValueError('out shares memory with what the optimiser holds, or the two with each other')
         if [f() for f in self._arenas] != self._arenas_where:
             raise RuntimeError('a moment or its scales have moved since the optimiser was made')

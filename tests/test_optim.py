@@ -44,6 +44,10 @@ def test_blocks():
     assert [blocks_of(n) for n in (0, 1, 256, 257)] == [0, 1, 1, 2]
 
 
+class OnHost:
+    device, h = -1, None                               # (what a host tensor says of its device)
+
+
 @pytest.fixture
 def on_host(monkeypatch):
     """Optimisers over host tensors, their library a list of the steps it was asked for: what is decided before a launch."""
@@ -81,7 +85,7 @@ def exchange(t):
 def test_what_has_moved_is_refused(on_host, what):
     """Every tensor whose address the optimiser holds."""
     params, grads = tensors(), tensors()
-    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
+    opt = AdamW(OnHost, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
     opt.step()
     back = exchange({'master': opt.masters[0], 'parameter': params[1]}[what] if what in ('master', 'parameter') else getattr(opt, what))
     reads = opt.states if what in ('m', 'v', 'm_scale', 'v_scale') else opt.step              # (the read-out looks at no parameter)
@@ -97,7 +101,7 @@ def test_what_has_moved_is_refused(on_host, what):
 def test_bound_gradients_are_memory(on_host):
     """step() reads the memory that was bound: tensors of the optimiser's own hold it, whatever becomes of the caller's."""
     params, grads = tensors(), tensors()
-    opt = AdamW(NoDevice, params).bind(grads)
+    opt = AdamW(OnHost, params).bind(grads)
     at = [g.data_ptr() for g in grads]
     for g in grads:
         g.data = g.clone()
@@ -111,7 +115,7 @@ def test_bound_gradients_are_memory(on_host):
 
 def test_the_tensors_of_an_optimiser_cannot_be_exchanged(on_host):
     """A replaced arena would be read by nobody and its predecessor freed under the next step."""
-    opt = AdamW(NoDevice, tensors(), state_bits=8, master=True, max_norm=1.0)
+    opt = AdamW(OnHost, tensors(), state_bits=8, master=True, max_norm=1.0)
     for name in ('params', 'masters', 'm', 'v', 'm_scale', 'v_scale', 'grad_norm'):
         with pytest.raises(AttributeError):
             setattr(opt, name, getattr(opt, name))
@@ -123,7 +127,7 @@ def test_the_tensors_of_an_optimiser_cannot_be_exchanged(on_host):
 def test_the_memory_of_what_has_moved_is_kept(on_host):
     """A captured step goes on using the memory that it was captured with."""
     params, grads = tensors()[:2], tensors()[:2]
-    opt = AdamW(NoDevice, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
+    opt = AdamW(OnHost, params, state_bits=8, master=True, max_norm=1.0).bind(grads)
     held = params + grads + [opt.masters[0], opt.m, opt.v, opt.m_scale, opt.v_scale, opt.grad_norm]
     at = {t.data_ptr() for t in held}
     for t in held:
@@ -151,11 +155,11 @@ def test_moments_that_share_memory_are_refused(bits, case):
 
 
 def test_read_out_into_memory_in_use_is_refused(on_host):
-    opt = AdamW(NoDevice, tensors(), state_bits=8, master=True)
+    opt = AdamW(OnHost, tensors(), state_bits=8, master=True)
     free = [torch.zeros(opt.blocks * BLOCK) for _ in range(2)]
     opt.states(out=free)
     arena = torch.zeros(opt.blocks * BLOCK + 4)
-    other = AdamW(NoDevice, [torch.zeros(opt.blocks * BLOCK)], state_bits=8)
+    other = AdamW(OnHost, [torch.zeros(opt.blocks * BLOCK)], state_bits=8)
     for bad in ([free[0], free[0]], [arena[:-4], arena[4:]]):
         with pytest.raises(ValueError, match='shares memory'):
             opt.states(out=bad)
@@ -167,7 +171,7 @@ def test_read_out_into_memory_in_use_is_refused(on_host):
 def test_gradients_of_another_shape_are_refused(on_host):
     """As many elements in another order are another gradient; flat ones (slices of a gradient arena) are the parameter's own order."""
     p = torch.zeros(5, 7)
-    opt = AdamW(NoDevice, [p])
+    opt = AdamW(OnHost, [p])
     for bad in (torch.zeros(7, 5), torch.zeros(35, 1), torch.zeros(1, 5, 7)):
         with pytest.raises(ValueError, match='shape'):
             opt.step([bad])
@@ -175,22 +179,22 @@ def test_gradients_of_another_shape_are_refused(on_host):
             opt.bind([bad])
     opt.step([torch.zeros(5, 7)])
     opt.step([torch.zeros(35)])
-    AdamW(NoDevice, [p.view(-1)]).step([torch.zeros(5, 7)])
+    AdamW(OnHost, [p.view(-1)]).step([torch.zeros(5, 7)])
     assert len(on_host) == 3
 
 
 def test_masters_are_handed_back(on_host):
     """A resumed optimiser goes on from the masters it is given, not from their rounded copies."""
     params = tensors()
-    first = AdamW(NoDevice, params, master=True)
+    first = AdamW(OnHost, params, master=True)
     first.masters[0].add_(2.0 ** -20)
-    again = AdamW(NoDevice, params, master=first.masters)
+    again = AdamW(OnHost, params, master=first.masters)
     assert again.masters[0] is first.masters[0] and again.masters[1:] == (None, None)
     kept = first.masters[0]
     for bad, match in (([kept], '1 masters'), ([None] * 3, 'master 0'), ([kept[:-1], None, None], 'master 0'), ([kept.bfloat16(), None, None], 'master 0'),
                        ([kept, torch.zeros(5, 7), None], 'master 1'), ([torch.zeros(600)[::2], None, None], 'master 0')):
         with pytest.raises(ValueError, match=match):
-            AdamW(NoDevice, params, master=bad)
+            AdamW(OnHost, params, master=bad)
 
 
 def test_a_nets_optimiser_options_are_checked_when_it_is_made():
