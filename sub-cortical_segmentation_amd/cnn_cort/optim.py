@@ -100,15 +100,15 @@ class AdamW:
         for t, p, w, d in zip(table, params, masters, decays):
             t.param, t.master, t.n = p.data_ptr(), None if w is None else w.data_ptr(), p.numel()
             t.weight_decay, t.type = float(d), self._types[p.dtype]
+        grad_norm = torch.zeros((1,), device=dev) if self.max_norm is not None else None           # of the last step, before clipping
         o = ctypes.c_void_p()
         lib = _hip.load_library()
-        torch.cuda.current_stream(dev).synchronize()           # the masters and zeros are written on this stream; steps may run on another
+        torch.cuda.current_stream(dev).synchronize()           # masters, zeros and the norm are written on this stream; steps may run on another
         _hip._check(lib.scs_adamw_create(handle.h, table, len(params), state_bits, m.data_ptr(), v.data_ptr(),
                                          _hip._ptr(m_scale), _hip._ptr(v_scale), int(step), ctypes.byref(o)), 'scs_adamw_create')
         self._lib, self._o = lib, o
         self._address, self._index, self._stream = torch.Tensor.data_ptr, handle.device, torch._C._cuda_getCurrentRawStream
         self._grads = self._bound = None
-        grad_norm = torch.zeros((1,), device=dev) if self.max_norm is not None else None           # of the last step, before clipping
         self._given = {'params': params, 'masters': masters, 'm': m, 'v': v, 'm_scale': m_scale, 'v_scale': v_scale, 'grad_norm': grad_norm}
         self._watched = list(params) + [t for t in masters + (m, v, m_scale, v_scale, grad_norm) if t is not None]
         self._held = [t.detach() for t in self._watched]               # (of the same memory, whatever becomes of the caller's)

@@ -204,3 +204,15 @@ def test_a_nets_optimiser_options_are_checked_when_it_is_made():
         with pytest.raises(ValueError, match=match):
             Net(optimizer='adamw', **bad)
     Net(optimizer='adamw', optimizer_bits=8, max_norm=1.0, weight_decay=0.0)
+
+
+def test_what_an_optimiser_fills_is_filled_before_it_returns(on_host, monkeypatch):
+    """Steps may run on another stream than the one it was made on: nothing is written there behind the wait (a late fill would wipe out a norm)."""
+    order = []
+    zeros = torch.zeros
+    monkeypatch.setattr(torch, 'zeros', lambda *a, **k: order.append('fill') or zeros(*a, **k))
+    monkeypatch.setattr(torch.cuda, 'current_stream', lambda *a: type('Stream', (), {'synchronize': lambda self: order.append('wait')})())
+    for bits in (32, 8):
+        del order[:]
+        AdamW(OnHost, [torch.ones(300, dtype=torch.bfloat16)], state_bits=bits, master=True, max_norm=1.0)
+        assert 'fill' in order and order[-1] == 'wait' and order.count('wait') == 1
